@@ -53,6 +53,8 @@ typedef struct CUstream_st* gqa_stream_t; /* == cudaStream_t */
 #define GQA_FLAG_CAUSAL 1 /* mask keys j > i (golden :180-181) */
 #define GQA_FLAG_ROPE_Q 2 /* rotate Q in the kernel (golden apply_rope :162-163) */
 #define GQA_FLAG_ROPE_K 4 /* rotate K in the kernel (golden apply_rope :164) */
+#define GQA_FLAG_INTERLEAVED 8 /* rotary pairs (2i, 2i + 1) instead of (i, i + rot/2) */
+#define GQA_FLAG_INVERSE 16    /* rotate backwards (the rotation's gradient) */
 
 #define GQA_MASK_NEG_INF_BF16 0xFF80 /* attention_mask.hpp:16 */
 
@@ -219,6 +221,90 @@ int gqa_decode_paged_bf16(const void* q, const void* kpages, const void* vpages,
                           const int32_t* q_pos, const void* cos, const void* sin, void* o, void* workspace,
                           size_t workspace_bytes, int B, int Hq, int Hkv, int head_dim, int kv_head_begin,
                           int kv_head_count, int split_len, float scale, int flags, gqa_stream_t stream);
+
+/* ---------------------------------------------------------------- serving a paged cache chunk by chunk
+ * No counterpart in the reference.  A step brings a ragged batch of new tokens: sequence
+ * b owns tokens [q_start[b], q_start[b + 1]) of T (q_start int32 [B + 1] on the device,
+ * ascending, inside [0, T]; tokens at q_start[B] and above are padding: neither read nor
+ * written).  lens[b] counts the sequence's cached slots WITH those n tokens, so its
+ * token i sits in slot lens[b] - n + i.  Pages as above, but page_size is any positive
+ * number for the append and the eviction and any multiple of 16 for the attention.
+ * q, k, v and o are [T][H][128] with strides in elements for tokens and heads (the last
+ * dim contiguous): slices of a fused projection and transposed head-major buffers need
+ * no copy.  T = 0 returns GQA_OK without a launch.
+ *
+ * gqa_rope_table_f32: cos/sin [rows][half_dim] = mscale * cos/sin((pos0 + r) *
+ * inv_freq[i]), angles in 64 bits; inv_freq double [half_dim] on the device.
+ *
+ * gqa_rope_positions_{bf16,f32}: y = x rotated at positions[t] (int32 [T]) over its first
+ * rot_dim (even) dims, in pairs (i, i + rot_dim/2) or, with GQA_FLAG_INTERLEAVED,
+ * (2i, 2i + 1); other dims pass through.  x, y [T][H][head_dim] (head_dim <= 512);
+ * cos/sin as above with table_rows rows of rot_dim/2.  GQA_FLAG_INVERSE rotates
+ * backwards: the gradient's direction.  y may be x (same strides); rows of y must not
+ * overlap.  A position outside the table skips its token (GQA_ERR_DEVICE_INPUT).
+ *
+ * gqa_kv_extend_bf16: k and v of the new tokens go to their slots, k rotated at
+ * positions[t] (NULL: at the token's slot); rot_dim = 0 does not rotate.  With q (else
+ * NULL and Hq = 0), q_out receives the rotated queries.  slot_pos (int32
+ * [B][Hkv][capacity], may be NULL) receives positions[t] at each slot written.  A slot
+ * past the capacity, a block-table entry outside [0, num_pages) or a position outside
+ * the table skips the token.
+ *
+ * gqa_attend_chunk_bf16: o[t, h] = softmax over the slots that token t sees of
+ * (q[t, h] . k * scale) times v; GQA_FLAG_CAUSAL: slots up to the token's own, else
+ * all of lens[b].  Any Hq that is a multiple of Hkv.  lse (float [T][Hq], may be NULL)
+ * receives the natural logarithm of the sum of the exponentials.  A row that sees no slot gives
+ * zeros and -inf.  Cache rows past lens[b] may hold anything.  max_q_len is a hint (the
+ * longest sequence's number of new tokens; 0 = unknown) that only chooses the tiling.
+ * workspace: gqa_attend_chunk_workspace_size bytes, 16-byte aligned.
+ *
+ * gqa_attn_weight_sums_f32: acc_out[b, h, j] = (j < lens[b] - n ? acc[b, h, j] : 0) +
+ * the sum of exp(q . k_j * scale - lse) over the group's query heads and the tokens that
+ * see slot j, for j < lens[b]; other entries are left alone.  acc, acc_out float
+ * [B][Hkv][capacity]; acc_out may be acc.  No atomics: runs repeat bit for bit.
+ *
+ * gqa_kv_evict_bf16: keep min(lens[b], budget) slots of each (b, kv head): slots whose
+ * slot_pos is below sink or at least next_pos[b] - recent first, then those with the
+ * largest acc (equal ones: the lower slot; NaN counts as lowest).  The i-th slot below
+ * the new length that goes receives the i-th kept slot above it (K, V, acc, slot_pos).
+ * acc_out, slot_pos_out [B][Hkv][capacity] get the first min(lens[b], budget) entries;
+ * lens_out the new lengths.  Each may be its input.  sink + recent <= budget, capacity
+ * at most 2^20 slots; workspace: gqa_kv_evict_workspace_size bytes.                   */
+int gqa_rope_table_f32(const double* inv_freq, float* cos, float* sin, int rows, int half_dim, int pos0, double mscale,
+                       gqa_stream_t stream);
+int gqa_rope_positions_bf16(const void* x, void* y, const int32_t* positions, const float* cos, const float* sin, int T,
+                            int H, int head_dim, int rot_dim, int table_rows, long long x_token_stride,
+                            long long x_head_stride, long long y_token_stride, long long y_head_stride, int flags,
+                            gqa_stream_t stream);
+int gqa_rope_positions_f32(const void* x, void* y, const int32_t* positions, const float* cos, const float* sin, int T,
+                           int H, int head_dim, int rot_dim, int table_rows, long long x_token_stride,
+                           long long x_head_stride, long long y_token_stride, long long y_head_stride, int flags,
+                           gqa_stream_t stream);
+int gqa_kv_extend_bf16(const void* k, const void* v, long long k_token_stride, long long k_head_stride,
+                       long long v_token_stride, long long v_head_stride, void* kpages, void* vpages,
+                       const int32_t* block_table, int max_pages_per_seq, int page_size, int num_pages,
+                       const int32_t* q_start, const int32_t* lens, const int32_t* positions, const float* cos,
+                       const float* sin, int table_rows, int rot_dim, const void* q, long long q_token_stride,
+                       long long q_head_stride, void* q_out, long long q_out_token_stride, long long q_out_head_stride,
+                       int32_t* slot_pos, int B, int T, int Hq, int Hkv, int head_dim, int flags, gqa_stream_t stream);
+size_t gqa_attend_chunk_workspace_size(int T, int Hq, int Hkv);
+int gqa_attend_chunk_bf16(const void* q, long long q_token_stride, long long q_head_stride, const void* kpages,
+                          const void* vpages, const int32_t* block_table, int max_pages_per_seq, int page_size,
+                          int num_pages, const int32_t* q_start, const int32_t* lens, void* o,
+                          long long o_token_stride, long long o_head_stride, float* lse, void* workspace,
+                          size_t workspace_bytes, int B, int T, int Hq, int Hkv, int head_dim, int max_q_len,
+                          float scale, int flags, gqa_stream_t stream);
+int gqa_attn_weight_sums_f32(const void* q, long long q_token_stride, long long q_head_stride, const void* kpages,
+                             const int32_t* block_table, int max_pages_per_seq, int page_size, int num_pages,
+                             const int32_t* q_start, const int32_t* lens, const float* lse, const float* acc,
+                             float* acc_out, int B, int T, int Hq, int Hkv, int head_dim, int max_q_len, float scale,
+                             int flags, gqa_stream_t stream);
+size_t gqa_kv_evict_workspace_size(int B, int Hkv, int budget);
+int gqa_kv_evict_bf16(void* kpages, void* vpages, const int32_t* block_table, int max_pages_per_seq, int page_size,
+                      int num_pages, const int32_t* lens, int32_t* lens_out, const float* acc, float* acc_out,
+                      const int32_t* slot_pos, int32_t* slot_pos_out, const int32_t* next_pos, void* workspace,
+                      size_t workspace_bytes, int B, int Hkv, int head_dim, int budget, int recent, int sink,
+                      gqa_stream_t stream);
 
 /* ---------------------------------------------------------------- projections
  * The full layer's linear maps (golden run_full_attention,

@@ -25,6 +25,8 @@ GQA_ERR_DEVICE_INPUT = -8
 GQA_FLAG_CAUSAL = 1
 GQA_FLAG_ROPE_Q = 2
 GQA_FLAG_ROPE_K = 4
+GQA_FLAG_INTERLEAVED = 8
+GQA_FLAG_INVERSE = 16
 GQA_MASK_NEG_INF_BF16 = 0xFF80
 GQA_GEMM_OUT_F32 = 1
 
@@ -52,6 +54,17 @@ SIGNATURES = {
                                 _vp]),
     "gqa_decode_paged_bf16": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i, _i, _i, _i,
                                    _i, _i, _i, _f, _i, _vp]),
+    "gqa_rope_table_f32": (_i, [_vp, _vp, _vp, _i, _i, _i, _d, _vp]),
+    "gqa_rope_positions_bf16": (_i, [_vp] * 5 + [_i] * 5 + [_ll] * 4 + [_i, _vp]),
+    "gqa_rope_positions_f32": (_i, [_vp] * 5 + [_i] * 5 + [_ll] * 4 + [_i, _vp]),
+    "gqa_kv_extend_bf16": (_i, [_vp] * 2 + [_ll] * 4 + [_vp] * 3 + [_i] * 3 + [_vp] * 5 + [_i] * 2 +
+                           [_vp, _ll, _ll, _vp, _ll, _ll, _vp] + [_i] * 6 + [_vp]),
+    "gqa_attend_chunk_workspace_size": (_sz, [_i, _i, _i]),
+    "gqa_attend_chunk_bf16": (_i, [_vp, _ll, _ll] + [_vp] * 3 + [_i] * 3 + [_vp] * 3 + [_ll, _ll, _vp, _vp, _sz] +
+                              [_i] * 6 + [_f, _i, _vp]),
+    "gqa_attn_weight_sums_f32": (_i, [_vp, _ll, _ll, _vp, _vp] + [_i] * 3 + [_vp] * 5 + [_i] * 6 + [_f, _i, _vp]),
+    "gqa_kv_evict_workspace_size": (_sz, [_i, _i, _i]),
+    "gqa_kv_evict_bf16": (_i, [_vp] * 3 + [_i] * 3 + [_vp] * 8 + [_sz] + [_i] * 6 + [_vp]),
     "gqa_gemm_bf16": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "gqa_qkv_proj_bf16": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "gqa_o_proj_bf16": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),

@@ -84,13 +84,15 @@ extern "C" const char* gqa_strerror(int code) {
   }
 }
 
-extern "C" int gqa_version(void) { return 1 * 10000 + 0 * 100 + 0; }
+extern "C" int gqa_version(void) { return 1 * 10000 + 1 * 100 + 0; }
 
 extern "C" int gqa_device_check(gqa_stream_t stream, int* site) {
   if (site) *site = 0;
   if (cudaStreamSynchronize(stream) != cudaSuccess) return GQA_ERR_CUDA;
   int (*const readers[])(bool) = {error_flag_stages, error_flag_prefill, error_flag_decode_tc,
-                                   error_flag_gemm,   error_flag_kvcache, error_flag_peer};
+                                   error_flag_gemm,   error_flag_kvcache, error_flag_peer,
+                                   error_flag_rope_positions, error_flag_attend, error_flag_weights,
+                                   error_flag_evict};
   int first = 0;
   for (auto rd : readers) {  // read and clear every file's word; report the first set one
     const int v = rd(true);

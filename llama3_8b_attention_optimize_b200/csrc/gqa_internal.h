@@ -13,6 +13,13 @@ namespace gqa {
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Whether the rows of a [T][H][d] array with these strides (elements) share no memory:
+// token-major or head-major, either way with room for each row.
+inline bool rows_apart(long long T, long long H, long long token_stride, long long head_stride, long long d) {
+  if ((T > 1 && token_stride < d) || (H > 1 && head_stride < d)) return false;
+  return T == 1 || H == 1 || token_stride >= (H - 1) * head_stride + d || head_stride >= (T - 1) * token_stride + d;
+}
+
 // Encode a 3-D bf16 tensor map over a contiguous [dim2][dim1][dim0] array with a
 // (box0, box1, box2) box and 128-byte swizzle (box0 * 2 bytes must be <= 128).
 int make_tmap_3d_bf16(CUtensorMap* map, const void* base, long long dim0, long long dim1, long long dim2, int box0,
@@ -43,6 +50,10 @@ int error_flag_decode_tc(bool clear);
 int error_flag_gemm(bool clear);
 int error_flag_kvcache(bool clear);
 int error_flag_peer(bool clear);
+int error_flag_rope_positions(bool clear);
+int error_flag_attend(bool clear);
+int error_flag_weights(bool clear);
+int error_flag_evict(bool clear);
 
 int launch_prefill(const void* q, const void* k, const void* v, void* o, const void* cos, const void* sin, int B, int S,
                    int Hq, int Hkv, int head_dim, int kv_begin, int kv_count, float scale, int flags,

@@ -11,7 +11,8 @@ import math
 import torch
 
 from . import _lib
-from ._lib import GQA_FLAG_CAUSAL, GQA_FLAG_ROPE_K, GQA_FLAG_ROPE_Q, GQA_GEMM_OUT_F32, GqaError, check
+from ._lib import (GQA_FLAG_CAUSAL, GQA_FLAG_INTERLEAVED, GQA_FLAG_INVERSE, GQA_FLAG_ROPE_K, GQA_FLAG_ROPE_Q,
+                   GQA_GEMM_OUT_F32, GqaError, check)
 
 ROPE_THETA = 500000.0
 HEAD_DIM = 128
@@ -296,6 +297,307 @@ def decode_paged(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, bl
     return out
 
 
+# ------------------------------------------------------------------ serving a paged cache chunk by chunk
+# A step brings a ragged batch of new tokens: sequence b owns tokens
+# [q_start[b], q_start[b + 1]) and lens[b] counts its cached slots with those tokens
+# included, so its token i of n sits in slot lens[b] - n + i.
+
+def _rows3(t: torch.Tensor, name: str, dtype=torch.bfloat16) -> None:
+    """A CUDA [T, H, d] tensor whose last dim is contiguous; any token and head strides."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (the kernels have no CPU path)")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1):
+        raise ValueError(f"{name} must be [T, H, d] with a contiguous last dim")
+
+
+def _same_device(first: torch.Tensor, *rest: torch.Tensor | None) -> None:
+    for t in rest:
+        if t is not None and t.device != first.device:
+            raise ValueError("all tensors must be on one device")
+
+
+def _call(device: torch.device, name: str, *args) -> None:
+    """Enqueue one C entry point on the device's current torch stream."""
+    fn = getattr(_lib.load(), name)
+    if torch.cuda.current_device() == device.index:
+        check(fn(*args, torch.cuda.current_stream(device).cuda_stream), name)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, torch.cuda.current_stream(device).cuda_stream), name)
+
+
+def rope_inv_freq(rot_dim: int, theta: float = ROPE_THETA, *, scaling: str = "none", factor: float = 1.0,
+                  original_len: int = 8192, low_freq: float = 1.0, high_freq: float = 4.0, beta_fast: float = 32.0,
+                  beta_slow: float = 1.0) -> tuple[torch.Tensor, float]:
+    """(inv_freq float64 [rot_dim/2], mscale): theta^(-2i/rot_dim), stretched for contexts
+    ``factor`` times longer than ``original_len``.
+
+    none     as they are
+    linear   every frequency divided by factor (positions interpolated)
+    llama3   wavelengths above original_len/low_freq divided by factor, below
+             original_len/high_freq kept, in between a linear blend in original_len/wavelength
+    yarn     dims that turn at least beta_fast times within original_len kept, at most
+             beta_slow times divided by factor, a linear ramp over the dims in between;
+             mscale = 0.1 ln(factor) + 1 on cos and sin
+    """
+    if rot_dim <= 0 or rot_dim % 2:
+        raise ValueError("rot_dim must be even and positive")
+    if not theta > 1.0 or not factor >= 1.0 or original_len <= 0:
+        raise ValueError("theta > 1, factor >= 1 and original_len > 0 are needed")
+    i = torch.arange(0, rot_dim, 2, dtype=torch.float64)
+    inv = theta ** (-i / rot_dim)
+    if scaling == "none":
+        return inv, 1.0
+    if scaling == "linear":
+        return inv / factor, 1.0
+    if scaling == "llama3":
+        if not 0 < low_freq < high_freq:
+            raise ValueError("0 < low_freq < high_freq is needed")
+        turns = original_len * inv / (2 * math.pi)  # original_len / wavelength
+        keep = ((turns - low_freq) / (high_freq - low_freq)).clamp(0.0, 1.0)
+        return inv * keep + inv / factor * (1.0 - keep), 1.0
+    if scaling == "yarn":
+        if not 0 < beta_slow < beta_fast:
+            raise ValueError("0 < beta_slow < beta_fast is needed")
+        def dim_of(turns: float) -> float:  # the dim pair that turns so often within original_len
+            return rot_dim * math.log(original_len / (turns * 2 * math.pi)) / (2 * math.log(theta))
+        lo = max(math.floor(dim_of(beta_fast)), 0)
+        hi = min(math.ceil(dim_of(beta_slow)), rot_dim - 1)
+        stretch = ((torch.arange(rot_dim // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
+        return inv / factor * stretch + inv * (1.0 - stretch), 0.1 * math.log(factor) + 1.0
+    raise ValueError("scaling must be none, linear, llama3 or yarn")
+
+
+def rope_table(rows: int, rot_dim: int = HEAD_DIM, theta: float = ROPE_THETA, pos0: int = 0, device=None,
+               **scaling) -> tuple[torch.Tensor, torch.Tensor]:
+    """(cos, sin) float32 [rows][rot_dim/2] of positions pos0 .. pos0 + rows - 1 for
+    ``rope_positions`` and ``kv_extend``, from 64-bit angles; ``scaling`` as in ``rope_inv_freq``."""
+    inv, mscale = rope_inv_freq(rot_dim, theta, **scaling)
+    device = torch.device(device or "cuda")
+    inv = inv.to(device)
+    cos = torch.empty(rows, rot_dim // 2, dtype=torch.float32, device=device)
+    sin = torch.empty_like(cos)
+    _call(cos.device, "gqa_rope_table_f32", _ptr(inv), _ptr(cos), _ptr(sin), rows, rot_dim // 2, pos0, mscale)
+    return cos, sin
+
+
+def rope_positions(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *,
+                   interleaved: bool = False, inverse: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """x [T, H, d] (bf16 or float32, any token and head strides) rotated at positions[t]
+    (int32 [T]) over its first 2 * cos.shape[1] dims; the others pass through.
+
+    cos, sin: ``rope_table``.  Pairs are (i, i + rot/2), or (2i, 2i + 1) when ``interleaved``.
+    ``inverse`` rotates backwards, which is the gradient's way through this operator.
+    ``out`` may be x."""
+    if isinstance(x, torch.Tensor) and x.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"x must be bfloat16 or float32, got {x.dtype}")
+    _rows3(x, "x", x.dtype if isinstance(x, torch.Tensor) else None)
+    T, H, d = x.shape
+    _need(positions, "positions", torch.int32)
+    _need(cos, "cos", torch.float32)
+    _need(sin, "sin", torch.float32)
+    if positions.shape != (T,):
+        raise ValueError("positions must be [T]")
+    if cos.dim() != 2 or sin.shape != cos.shape or 2 * cos.shape[1] > d:
+        raise ValueError("cos and sin must be [rows, rot/2] with rot <= d")
+    out = torch.empty(T, H, d, dtype=x.dtype, device=x.device) if out is None else out
+    _rows3(out, "out", x.dtype)
+    if out.shape != x.shape:
+        raise ValueError("out must have x's shape")
+    _same_device(x, positions, cos, sin, out)
+    _call(x.device, "gqa_rope_positions_bf16" if x.dtype == torch.bfloat16 else "gqa_rope_positions_f32", _ptr(x),
+          _ptr(out), _ptr(positions), _ptr(cos), _ptr(sin), T, H, d, 2 * cos.shape[1], cos.shape[0], x.stride(0),
+          x.stride(1), out.stride(0), out.stride(1),
+          (GQA_FLAG_INTERLEAVED if interleaved else 0) | (GQA_FLAG_INVERSE if inverse else 0))
+    return out
+
+
+def _paged(kpages: torch.Tensor, vpages: torch.Tensor | None, block_table: torch.Tensor, q_start: torch.Tensor | None,
+           lens: torch.Tensor) -> tuple[int, int, int, int, int]:
+    """(B, max_pages, page_size, num_pages, Hkv) of checked page pools and tables."""
+    _need(kpages, "kpages")
+    if vpages is not None:
+        _need(vpages, "vpages")
+    _need(block_table, "block_table", torch.int32)
+    _need(lens, "lens", torch.int32)
+    if kpages.dim() != 4 or kpages.shape[3] != HEAD_DIM or (vpages is not None and vpages.shape != kpages.shape):
+        raise ValueError("kpages and vpages must be [num_pages, Hkv, page_size, 128]")
+    num_pages, Hkv, page_size, _ = kpages.shape
+    if block_table.dim() != 2 or lens.shape != (block_table.shape[0],):
+        raise ValueError("block_table must be [B, max_pages] and lens [B]")
+    B, max_pages = block_table.shape
+    if q_start is not None:
+        _need(q_start, "q_start", torch.int32)
+        if q_start.shape != (B + 1,):
+            raise ValueError("q_start must be [B + 1]")
+    return B, max_pages, page_size, num_pages, Hkv
+
+
+def kv_extend(k: torch.Tensor, v: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, block_table: torch.Tensor,
+              q_start: torch.Tensor, lens: torch.Tensor, positions: torch.Tensor | None = None,
+              cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, *, q: torch.Tensor | None = None,
+              q_out: torch.Tensor | None = None, interleaved: bool = False,
+              slot_pos: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Write the new tokens' k and v [T, Hkv, 128] into their slots of the page pools, k
+    rotated at positions[t] (int32 [T]; None: at its slot) when the ``rope_table`` tables
+    are given.  With ``q`` [T, Hq, 128], rotates the queries too and returns them
+    (``q_out``, which may be q).  ``slot_pos`` (int32 [B, Hkv, capacity]) receives the
+    position held by each slot written, for ``kv_evict``."""
+    _rows3(k, "k")
+    _rows3(v, "v")
+    B, max_pages, page_size, num_pages, Hkv = _paged(kpages, vpages, block_table, q_start, lens)
+    T = k.shape[0]
+    if k.shape != (T, Hkv, HEAD_DIM) or v.shape != k.shape:
+        raise ValueError("k and v must be [T, Hkv, 128]")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin come together")
+    rows = rot = 0
+    if cos is not None:
+        _need(cos, "cos", torch.float32)
+        _need(sin, "sin", torch.float32)
+        if cos.dim() != 2 or sin.shape != cos.shape or 2 * cos.shape[1] > HEAD_DIM:
+            raise ValueError("cos and sin must be [rows, rot/2] with rot <= 128")
+        rows, rot = cos.shape[0], 2 * cos.shape[1]
+    if positions is not None:
+        _need(positions, "positions", torch.int32)
+        if positions.shape != (T,):
+            raise ValueError("positions must be [T]")
+    Hq = q_t = q_h = o_t = o_h = 0
+    if q is not None:
+        _rows3(q, "q")
+        if q.shape[0] != T or q.shape[2] != HEAD_DIM:
+            raise ValueError("q must be [T, Hq, 128]")
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+        _rows3(q_out, "q_out")
+        if q_out.shape != q.shape:
+            raise ValueError("q_out must have q's shape")
+        Hq, q_t, q_h, o_t, o_h = q.shape[1], q.stride(0), q.stride(1), q_out.stride(0), q_out.stride(1)
+    elif q_out is not None:
+        raise ValueError("q_out needs q")
+    if slot_pos is not None:
+        _need(slot_pos, "slot_pos", torch.int32)
+        if slot_pos.shape != (B, Hkv, max_pages * page_size):
+            raise ValueError("slot_pos must be [B, Hkv, max_pages * page_size]")
+    _same_device(k, v, kpages, vpages, block_table, q_start, lens, positions, cos, sin, q, q_out, slot_pos)
+    _call(k.device, "gqa_kv_extend_bf16", _ptr(k), _ptr(v), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+          _ptr(kpages), _ptr(vpages), _ptr(block_table), max_pages, page_size, num_pages, _ptr(q_start), _ptr(lens),
+          None if positions is None else _ptr(positions), None if cos is None else _ptr(cos),
+          None if sin is None else _ptr(sin), rows, rot, None if q is None else _ptr(q), q_t, q_h,
+          None if q_out is None else _ptr(q_out), o_t, o_h, None if slot_pos is None else _ptr(slot_pos), B, T, Hq, Hkv,
+          HEAD_DIM, GQA_FLAG_INTERLEAVED if interleaved else 0)
+    return q_out
+
+
+def attend_chunk_workspace_bytes(T: int, Hq: int, Hkv: int) -> int:
+    return int(_lib.load().gqa_attend_chunk_workspace_size(T, Hq, Hkv))
+
+
+def attend_chunk(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, block_table: torch.Tensor,
+                 q_start: torch.Tensor, lens: torch.Tensor, *, causal: bool = True, scale: float | None = None,
+                 max_q_len: int = 0, out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                 workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a ragged chunk of new tokens, q [T, Hq, 128] (rotated), over the pages
+    that already hold their keys and values: token i of sequence b sees its slots up to
+    its own (``causal``) or all lens[b].  ``lse`` (float32 [T, Hq]) receives the natural
+    log of the softmax's sum.  ``max_q_len``: the longest sequence's number of new tokens
+    where the caller knows it (a hint that picks the tiling).  Tokens that see no slot give
+    zeros and -inf."""
+    _rows3(q, "q")
+    B, max_pages, page_size, num_pages, Hkv = _paged(kpages, vpages, block_table, q_start, lens)
+    T, Hq, d = q.shape
+    if d != HEAD_DIM:
+        raise ValueError("q must be [T, Hq, 128]")
+    out = torch.empty(T, Hq, d, dtype=q.dtype, device=q.device) if out is None else out
+    _rows3(out, "out")
+    if out.shape != q.shape:
+        raise ValueError("out must have q's shape")
+    if lse is not None:
+        _need(lse, "lse", torch.float32)
+        if lse.shape != (T, Hq):
+            raise ValueError("lse must be [T, Hq]")
+    if workspace is None:
+        workspace = torch.empty(max(attend_chunk_workspace_bytes(T, Hq, Hkv), 16), dtype=torch.uint8, device=q.device)
+    _need(workspace, "workspace", workspace.dtype)
+    _same_device(q, kpages, vpages, block_table, q_start, lens, out, lse, workspace)
+    _call(q.device, "gqa_attend_chunk_bf16", _ptr(q), q.stride(0), q.stride(1), _ptr(kpages), _ptr(vpages),
+          _ptr(block_table), max_pages, page_size, num_pages, _ptr(q_start), _ptr(lens), _ptr(out), out.stride(0),
+          out.stride(1), None if lse is None else _ptr(lse), _ptr(workspace),
+          workspace.numel() * workspace.element_size(), B, T, Hq, Hkv, d, max_q_len,
+          default_scale(d) if scale is None else float(scale), GQA_FLAG_CAUSAL if causal else 0)
+    return out
+
+
+def attn_weight_sums(q: torch.Tensor, kpages: torch.Tensor, block_table: torch.Tensor, q_start: torch.Tensor,
+                     lens: torch.Tensor, lse: torch.Tensor, acc: torch.Tensor, *, causal: bool = True,
+                     scale: float | None = None, max_q_len: int = 0,
+                     acc_out: torch.Tensor | None = None) -> torch.Tensor:
+    """Add each cached slot's attention weight from this chunk: acc_out[b, h, j] = acc[b, h, j]
+    (zero for slots the chunk wrote) + the sum of exp(q . k_j * scale - lse) over the
+    group's query heads and the chunk's tokens that see slot j.  acc, acc_out float32
+    [B, Hkv, capacity]; entries at lens[b] and above are left alone; acc_out defaults to
+    acc (in place).  q, q_start, lens and ``lse`` are those of ``attend_chunk``."""
+    _rows3(q, "q")
+    B, max_pages, page_size, num_pages, Hkv = _paged(kpages, None, block_table, q_start, lens)
+    T, Hq, d = q.shape
+    if d != HEAD_DIM:
+        raise ValueError("q must be [T, Hq, 128]")
+    _need(lse, "lse", torch.float32)
+    if lse.shape != (T, Hq):
+        raise ValueError("lse must be [T, Hq]")
+    acc_out = acc if acc_out is None else acc_out
+    for t, n in ((acc, "acc"), (acc_out, "acc_out")):
+        _need(t, n, torch.float32)
+        if t.shape != (B, Hkv, max_pages * page_size):
+            raise ValueError(f"{n} must be [B, Hkv, max_pages * page_size]")
+    _same_device(q, kpages, block_table, q_start, lens, lse, acc, acc_out)
+    _call(q.device, "gqa_attn_weight_sums_f32", _ptr(q), q.stride(0), q.stride(1), _ptr(kpages), _ptr(block_table),
+          max_pages, page_size, num_pages, _ptr(q_start), _ptr(lens), _ptr(lse), _ptr(acc), _ptr(acc_out), B, T, Hq, Hkv,
+          d, max_q_len, default_scale(d) if scale is None else float(scale), GQA_FLAG_CAUSAL if causal else 0)
+    return acc_out
+
+
+def kv_evict_workspace_bytes(B: int, Hkv: int, budget: int) -> int:
+    return int(_lib.load().gqa_kv_evict_workspace_size(B, Hkv, budget))
+
+
+def kv_evict(kpages: torch.Tensor, vpages: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
+             acc: torch.Tensor, slot_pos: torch.Tensor, next_pos: torch.Tensor, budget: int, *, recent: int = 0,
+             sink: int = 0, acc_out: torch.Tensor | None = None, slot_pos_out: torch.Tensor | None = None,
+             lens_out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> None:
+    """Keep min(lens[b], budget) slots of every (sequence, kv head): those that hold one of
+    the first ``sink`` positions or of the last ``recent`` before next_pos[b] (int32 [B]),
+    then those with the largest ``acc``, equal ones by the lower slot.  The i-th slot
+    below the new length that goes receives the i-th kept one above it; K and V rows move
+    in place.  acc, slot_pos [B, Hkv, capacity] (float32, int32) follow into acc_out,
+    slot_pos_out, the lengths into lens_out; each defaults to its input."""
+    B, max_pages, page_size, num_pages, Hkv = _paged(kpages, vpages, block_table, None, lens)
+    acc_out = acc if acc_out is None else acc_out
+    slot_pos_out = slot_pos if slot_pos_out is None else slot_pos_out
+    lens_out = lens if lens_out is None else lens_out
+    for t, n, dt in ((acc, "acc", torch.float32), (acc_out, "acc_out", torch.float32),
+                     (slot_pos, "slot_pos", torch.int32), (slot_pos_out, "slot_pos_out", torch.int32)):
+        _need(t, n, dt)
+        if t.shape != (B, Hkv, max_pages * page_size):
+            raise ValueError(f"{n} must be [B, Hkv, max_pages * page_size]")
+    for t, n in ((next_pos, "next_pos"), (lens_out, "lens_out")):
+        _need(t, n, torch.int32)
+        if t.shape != (B,):
+            raise ValueError(f"{n} must be [B]")
+    if workspace is None:
+        workspace = torch.empty(max(kv_evict_workspace_bytes(B, Hkv, budget), 16), dtype=torch.uint8,
+                                device=kpages.device)
+    _need(workspace, "workspace", workspace.dtype)
+    _same_device(kpages, vpages, block_table, lens, acc, slot_pos, next_pos, acc_out, slot_pos_out, lens_out, workspace)
+    _call(kpages.device, "gqa_kv_evict_bf16", _ptr(kpages), _ptr(vpages), _ptr(block_table), max_pages, page_size,
+          num_pages, _ptr(lens), _ptr(lens_out), _ptr(acc), _ptr(acc_out), _ptr(slot_pos), _ptr(slot_pos_out),
+          _ptr(next_pos), _ptr(workspace), workspace.numel() * workspace.element_size(), B, Hkv, HEAD_DIM, budget,
+          recent, sink)
+
+
 def linear(x: torch.Tensor, w: torch.Tensor, *, out_f32: bool = False,
            out: torch.Tensor | None = None) -> torch.Tensor:
     """bf16(x @ w^T) (or the fp32 sums with ``out_f32``) for x [..., K], w [N, K] in the
@@ -423,4 +725,6 @@ def ctypes_int():
 
 
 __all__ = ["rope_cache", "rope", "scores", "mask", "attention_mask_words", "softmax", "pv", "prefill", "decode",
-           "decode_workspace_bytes", "device_check", "default_scale", "GqaError"]
+           "decode_workspace_bytes", "device_check", "default_scale", "GqaError", "rope_inv_freq", "rope_table",
+           "rope_positions", "kv_extend", "attend_chunk", "attend_chunk_workspace_bytes", "attn_weight_sums", "kv_evict",
+           "kv_evict_workspace_bytes"]
