@@ -314,6 +314,12 @@ def _rows3(t: torch.Tensor, name: str, dtype=torch.bfloat16) -> None:
         raise ValueError(f"{name} must be [T, H, d] with a contiguous last dim")
 
 
+def _no_broadcast(t: torch.Tensor) -> torch.Tensor:
+    """t itself, or a copy where tokens or heads share memory (TMA reads along strides above zero)."""
+    T, H, _ = t.shape
+    return t.contiguous() if (T > 1 and t.stride(0) == 0) or (H > 1 and t.stride(1) == 0) else t
+
+
 def _same_device(first: torch.Tensor, *rest: torch.Tensor | None) -> None:
     for t in rest:
         if t is not None and t.device != first.device:
@@ -511,6 +517,7 @@ def attend_chunk(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, bl
     T, Hq, d = q.shape
     if d != HEAD_DIM:
         raise ValueError("q must be [T, Hq, 128]")
+    q = _no_broadcast(q)
     out = torch.empty(T, Hq, d, dtype=q.dtype, device=q.device) if out is None else out
     _rows3(out, "out")
     if out.shape != q.shape:
