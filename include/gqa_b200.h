@@ -262,6 +262,7 @@ int gqa_decode_paged_bf16(const void* q, const void* kpages, const void* vpages,
  * the sum of exp(q . k_j * scale - lse) over the group's query heads and the tokens that
  * see slot j, for j < lens[b]; other entries are left alone.  acc, acc_out float
  * [B][Hkv][capacity]; acc_out may be acc.  No atomics: runs repeat bit for bit.
+ * workspace: gqa_attn_weight_sums_workspace_size bytes, 16-byte aligned.
  *
  * gqa_kv_evict_bf16: keep min(lens[b], budget) slots of each (b, kv head): slots whose
  * slot_pos is below sink or at least next_pos[b] - recent first, then those with the
@@ -294,11 +295,12 @@ int gqa_attend_chunk_bf16(const void* q, long long q_token_stride, long long q_h
                           long long o_token_stride, long long o_head_stride, float* lse, void* workspace,
                           size_t workspace_bytes, int B, int T, int Hq, int Hkv, int head_dim, int max_q_len,
                           float scale, int flags, gqa_stream_t stream);
+size_t gqa_attn_weight_sums_workspace_size(void);
 int gqa_attn_weight_sums_f32(const void* q, long long q_token_stride, long long q_head_stride, const void* kpages,
                              const int32_t* block_table, int max_pages_per_seq, int page_size, int num_pages,
                              const int32_t* q_start, const int32_t* lens, const float* lse, const float* acc,
-                             float* acc_out, int B, int T, int Hq, int Hkv, int head_dim, int max_q_len, float scale,
-                             int flags, gqa_stream_t stream);
+                             float* acc_out, void* workspace, size_t workspace_bytes, int B, int T, int Hq, int Hkv,
+                             int head_dim, float scale, int flags, gqa_stream_t stream);
 size_t gqa_kv_evict_workspace_size(int B, int Hkv, int budget);
 int gqa_kv_evict_bf16(void* kpages, void* vpages, const int32_t* block_table, int max_pages_per_seq, int page_size,
                       int num_pages, const int32_t* lens, int32_t* lens_out, const float* acc, float* acc_out,

@@ -62,7 +62,9 @@ SIGNATURES = {
     "gqa_attend_chunk_workspace_size": (_sz, [_i, _i, _i]),
     "gqa_attend_chunk_bf16": (_i, [_vp, _ll, _ll] + [_vp] * 3 + [_i] * 3 + [_vp] * 3 + [_ll, _ll, _vp, _vp, _sz] +
                               [_i] * 6 + [_f, _i, _vp]),
-    "gqa_attn_weight_sums_f32": (_i, [_vp, _ll, _ll, _vp, _vp] + [_i] * 3 + [_vp] * 5 + [_i] * 6 + [_f, _i, _vp]),
+    "gqa_attn_weight_sums_workspace_size": (_sz, []),
+    "gqa_attn_weight_sums_f32": (_i, [_vp, _ll, _ll, _vp, _vp] + [_i] * 3 + [_vp] * 6 + [_sz] + [_i] * 5 +
+                                 [_f, _i, _vp]),
     "gqa_kv_evict_workspace_size": (_sz, [_i, _i, _i]),
     "gqa_kv_evict_bf16": (_i, [_vp] * 3 + [_i] * 3 + [_vp] * 8 + [_sz] + [_i] * 6 + [_vp]),
     "gqa_gemm_bf16": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),

@@ -13,11 +13,10 @@
 // for all heads of the group and for NT * 128 / G tokens.  A unit walks its K/V tiles of
 // 128 slots with an online softmax.
 //
-// Split: all units' K/V tiles form one line, cut into equal parts, one per CTA (one CTA per
-// SM).  A part may begin and end inside a unit; such segments leave (O, m, l) in the
-// workspace and a second kernel merges them.  One long sequence of a single token so
-// keeps every SM busy, a ragged batch needs no plan from the host, and the workspace is
-// two segments a CTA whatever the lengths.
+// Split: all units' K/V tiles form one line, cut into equal parts, one per CTA and SM
+// (ragged.cuh).  A part may begin and end inside a unit; such segments leave (O, m, l) in
+// the workspace and a second kernel merges them.  So one long sequence of a single token
+// keeps every SM busy.
 //
 // Pipeline (per CTA): a producer warp loads Q by TMA and streams K and V tiles through a ring, one
 // box per page (or per part of a page inside a tile); one warp per Q tile issues S = Q K^T
@@ -35,6 +34,7 @@
 #include "attn_common.cuh"
 #include "common.cuh"
 #include "gqa_internal.h"
+#include "ragged.cuh"
 
 namespace gqa {
 namespace attend {
@@ -44,14 +44,20 @@ using attn::fmax3;
 using attn::load_idx_k;
 using attn::load_idx_v;
 using attn::sw128_chunk;
+using ragged::Boxes;
+using ragged::Desc;
+using ragged::kMaxB;
+using ragged::kMaxCtas;
+using ragged::Part;
+using ragged::Seq;
+using ragged::seq_of;
+using ragged::Walk;
 
 constexpr int kD = 128;
 constexpr int kBN = 128;                   // slots per K/V tile
 constexpr int kTileBytes = 128 * 128 * 2;  // Q, P, K and V tiles: 32 KB
 constexpr int kHalf = kTileBytes / 2;      // one 64-column swizzle block of 128 rows
 constexpr float kRescaleLog2 = 16.0f;
-constexpr int kMaxCtas = 148;              // workspace slots are sized for so many
-constexpr int kMaxB = 8192;                // sequences (prefix of their tiles in shared memory)
 constexpr float kLn2 = 0.6931471805599453f;
 
 template <int NT>
@@ -76,6 +82,7 @@ struct Cfg {
   static constexpr int kOffTmemPtr = kOffX + NT * 2 * 128 * 4;
   static constexpr int kOffStart = kOffTmemPtr + 16;  // this CTA's part: first unit, tile, count
   static constexpr int kSmemBytes = kOffStart + 32;
+  static_assert(sizeof(Walk) <= 32, "room for the start");
   static_assert(kSmemBytes <= 232448, "shared memory over the per-block limit");
   static_assert(kMaxB * 8 + 64 * 8 <= kStages * kTileBytes, "the plan's scratch lies in the ring");
 };
@@ -106,115 +113,59 @@ enum : int {
   SITE_BAD_PAGE = 0x622,  // block-table entry outside [0, num_pages)
 };
 
-struct Desc {  // a unit split over CTAs c .. last, written by CTA c
-  int valid, token0, n_tok, h, last, pad[3];
-};
-
 struct Params {
-  const int32_t *table, *q_start, *lens;
+  ragged::Batch batch;
   uint16_t* o;
   float* lse;
   float4* part_o;  // [2 * grid][32][part_rows]
   float* part_ml;  // [2 * grid][3][part_rows]
   Desc* desc;      // [grid]
   long long o_t, o_h;
-  int B, T, G, Hq, Hkv, capacity, max_pages, page_size, num_pages, causal;
+  int G, Hq, causal;
   int tpt, tu;     // query tokens per tile, per unit
   int box;         // rows of one K/V box: the largest power of two dividing page_size, <= 128
   int part_rows;
   float scale_log2;
 };
 
-// ------------------------------------------------------------------ the line of tiles
-struct Seq {
-  int a, n, L;  // first token, tokens, slots
+// Units: blocks of tu query tokens.  Steps: K/V tiles over the slots [0, limit) that some
+// row of the unit sees; one at least, so that rows without any slot are written too.
+struct Line {
+  int tu, causal;
+  __device__ __forceinline__ Line(const Params& p) : tu(p.tu), causal(p.causal) {}
+  __device__ __forceinline__ int units(const Seq& s) const { return (s.n + tu - 1) / tu; }
+  __device__ __forceinline__ int limit(const Seq& s, int u) const {
+    return causal ? max(0, s.L - s.n + min(s.n, (u + 1) * tu)) : s.L;
+  }
+  __device__ __forceinline__ int count(const Seq& s, int u) const { return max(1, (limit(s, u) + kBN - 1) / kBN); }
+  __device__ __forceinline__ long long before(const Seq& s, int k) const {
+    const int n = units(s);
+    if (!causal) return static_cast<long long>(k) * count(s, 0);
+    const int m = min(k, n - 1);  // the last unit may be shorter
+    const long long base = s.L - s.n;
+    // units whose limit is at most one tile
+    const int one = base >= kBN ? 0 : static_cast<int>(min(static_cast<long long>(m), (kBN - base) / tu));
+    long long sum = one;
+    if (m > one)
+      sum += ragged::floor_sum(m - one, kBN, tu, base + static_cast<long long>(one + 1) * tu + kBN - 1);
+    if (k == n) sum += count(s, n - 1);
+    return sum;
+  }
 };
 
-__device__ __forceinline__ Seq seq_of(const Params& p, int b) {
-  Seq s;
-  s.a = __ldg(p.q_start + b);
-  const int z = __ldg(p.q_start + b + 1);
-  s.n = (s.a < 0 || z < s.a || z > p.T) ? 0 : z - s.a;
-  s.L = min(max(__ldg(p.lens + b), 0), p.capacity);
-  return s;
-}
-
-// Slots [0, limit) that some row of unit qb sees, and the unit's tiles: one at least, so
-// that rows without any slot are written too.
-__device__ __forceinline__ int limit_of(const Params& p, const Seq& s, int qb) {
-  return p.causal ? max(0, s.L - s.n + min(s.n, (qb + 1) * p.tu)) : s.L;
-}
-__device__ __forceinline__ int tiles_of(int limit) { return max(1, (limit + kBN - 1) / kBN); }
-
-// sum_{i < n} floor((a i + b) / m), by Euclid's steps on (a, m); a, b >= 0, m > 0.
-__device__ __forceinline__ long long floor_sum(long long n, long long m, long long a, long long b) {
-  long long sum = 0;
-  while (n > 0) {
-    sum += (a / m) * (n * (n - 1) / 2) + (b / m) * n;
-    a %= m;
-    b %= m;
-    const long long top = a * n + b;
-    if (top < m) break;
-    // count lattice points the other way round
-    n = top / m;
-    b = top % m;
-    const long long x = m;
-    m = a;
-    a = x;
-  }
-  return sum;
-}
-
-// Tiles of the first k units of one head of a sequence.
-__device__ __forceinline__ long long tiles_before(const Params& p, const Seq& s, int k) {
-  const int units = (s.n + p.tu - 1) / p.tu;
-  if (!p.causal) return static_cast<long long>(k) * tiles_of(s.L);
-  const int m = min(k, units - 1);  // the last unit may be shorter
-  const long long base = s.L - s.n;
-  // units whose limit is at most one tile
-  const int one = base >= kBN ? 0 : static_cast<int>(min(static_cast<long long>(m), (kBN - base) / p.tu));
-  long long sum = one;
-  if (m > one) sum += floor_sum(m - one, kBN, p.tu, base + static_cast<long long>(one + 1) * p.tu + kBN - 1);
-  if (k == units) sum += tiles_of(limit_of(p, s, units - 1));
-  return sum;
-}
-
-struct Walk {
-  int b, h, qb, kv0, left;
+struct Seg : Part {
+  int tok0, n_tok, base, limit;
+  // the unit's last slots lie in this segment and do not fill their tile
+  __device__ __forceinline__ bool tail() const { return k1 == count && limit < count * kBN; }
 };
 
-struct Seg {
-  int b, a, h, tok0, n_tok, base, limit, L, kv0, kv1, n_kv;
-  __device__ __forceinline__ bool tail() const { return kv1 == n_kv && (limit < n_kv * kBN); }
-};
-
-__device__ __forceinline__ bool next_seg(const Params& p, Walk& w, Seg& s) {
-  if (w.left <= 0 || w.b >= p.B) return false;
-  Seq q = seq_of(p, w.b);
-  while (q.n == 0) {
-    if (++w.b >= p.B) return false;
-    q = seq_of(p, w.b);
-  }
-  s.b = w.b;
-  s.a = q.a;
-  s.h = w.h;
-  s.tok0 = w.qb * p.tu;
-  s.n_tok = min(p.tu, q.n - s.tok0);
-  s.base = q.L - q.n;
-  s.L = q.L;
-  s.limit = limit_of(p, q, w.qb);
-  s.n_kv = tiles_of(s.limit);
-  s.kv0 = w.kv0;
-  s.kv1 = min(s.n_kv, w.kv0 + w.left);
-  w.left -= s.kv1 - s.kv0;
-  w.kv0 = 0;
-  if (++w.qb * p.tu >= q.n) {
-    w.qb = 0;
-    if (++w.h == p.Hkv) {
-      w.h = 0;
-      ++w.b;
-    }
-  }
+__device__ __forceinline__ bool next_seg(const Params& p, Walk& w, Seg& x) {
+  const Line line(p);
+  if (!ragged::next_part(p.batch, line, w, x)) return false;
+  x.tok0 = x.u * p.tu;
+  x.n_tok = min(p.tu, x.s.n - x.tok0);
+  x.base = x.s.L - x.s.n;
+  x.limit = line.limit(x.s, x.u);
   return true;
 }
 
@@ -263,7 +214,6 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   auto bar = [&](int i) -> uint32_t { return sbase + C::kOffBar + 8 * i; };
-  int* start = reinterpret_cast<int*>(smem + C::kOffStart);
 
   if (threadIdx.x == 0) {
     for (int t = 0; t < NT; ++t) {
@@ -292,105 +242,13 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
     tma_prefetch_desc(&tmV);
   }
 
-  // ---- plan: prefix of the sequences' tiles, then this CTA's part of the line
-  {
-    long long* prefix = reinterpret_cast<long long*>(smem + C::kOffKV);  // [B + 1]
-    long long* wsum = prefix + kMaxB;                                    // [warps]; reuses no prefix entry
-    long long carry = 0;
-    for (int b0 = 0; b0 < p.B; b0 += C::kThreads) {
-      const int b = b0 + threadIdx.x;
-      long long mine = 0;
-      if (b < p.B) {
-        const Seq s = seq_of(p, b);
-        if (s.n > 0) mine = tiles_before(p, s, (s.n + p.tu - 1) / p.tu) * p.Hkv;
-        if (blockIdx.x == 0) {  // report what seq_of replaced
-          const int z = __ldg(p.q_start + b + 1), L = __ldg(p.lens + b);
-          if (s.a < 0 || z < s.a || z > p.T) record_input_error(SITE_Q_START);
-          if (L < 0 || L > p.capacity) record_input_error(SITE_LENGTH);
-        }
-      }
-      long long scan = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, scan, o);
-        if (lane >= o) scan += x;
-      }
-      if (lane == 31) wsum[warp] = scan;
-      __syncthreads();
-      long long before = carry, all = 0;
-      for (int w = 0; w < C::kThreads / 32; ++w) {
-        if (w < warp) before += wsum[w];
-        all += wsum[w];
-      }
-      if (b < p.B) prefix[b] = before + scan - mine;
-      carry += all;
-      __syncthreads();
-    }
-    const long long W = carry;
-    const long long ctas = min(static_cast<long long>(gridDim.x), W);
-    const long long c = blockIdx.x;
-    auto locate = [&](long long x) -> Walk {  // the unit and tile at place x < W of the line
-      int lo = 0, hi = p.B;                   // the last b with prefix[b] <= x
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (prefix[mid] <= x) lo = mid;
-        else hi = mid;
-      }
-      const Seq s = seq_of(p, lo);
-      const int units = (s.n + p.tu - 1) / p.tu;
-      const long long head = tiles_before(p, s, units);
-      const long long rem = x - prefix[lo];
-      Walk w;
-      w.b = lo;
-      w.h = static_cast<int>(rem / head);
-      const long long r = rem - w.h * head;
-      int u0 = 0, u1 = units;  // the last unit with tiles_before <= r
-      while (u1 - u0 > 1) {
-        const int mid = (u0 + u1) >> 1;
-        if (tiles_before(p, s, mid) <= r) u0 = mid;
-        else u1 = mid;
-      }
-      w.qb = u0;
-      w.kv0 = static_cast<int>(r - tiles_before(p, s, u0));
-      w.left = 0;
-      return w;
-    };
-    if (threadIdx.x == 0) {
-      Walk w = {0, 0, 0, 0, 0};
-      if (c < ctas) {
-        const long long r0 = c * W / ctas, r1 = (c + 1) * W / ctas;
-        w = locate(r0);
-        w.left = static_cast<int>(r1 - r0);
-      }
-      start[0] = w.b;
-      start[1] = w.h;
-      start[2] = w.qb;
-      start[3] = w.kv0;
-      start[4] = w.left;
-    }
-    if (threadIdx.x == 32) {  // is the unit at this part's end split here first?
-      Desc d = {0, 0, 0, 0, 0, {0, 0, 0}};
-      if (c + 1 < ctas) {
-        const long long r0 = c * W / ctas, r1 = (c + 1) * W / ctas;
-        const Walk w = locate(r1);
-        if (w.kv0 > 0 && r1 - w.kv0 >= r0) {
-          const Seq s = seq_of(p, w.b);
-          d.valid = 1;
-          d.token0 = s.a + w.qb * p.tu;
-          d.n_tok = min(p.tu, s.n - w.qb * p.tu);
-          d.h = w.h;
-          const long long end = r1 - w.kv0 + tiles_of(limit_of(p, s, w.qb));
-          d.last = static_cast<int>((end * ctas - 1) / W);
-        }
-      }
-      p.desc[c] = d;
-    }
-  }
+  ragged::plan<C::kThreads>(p.batch, Line(p), reinterpret_cast<long long*>(smem + C::kOffKV),
+                            reinterpret_cast<Walk*>(smem + C::kOffStart), p.desc, SITE_Q_START, SITE_LENGTH);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + C::kOffTmemPtr);
-  Walk walk = {start[0], start[1], start[2], start[3], start[4]};
+  Walk walk = *reinterpret_cast<const Walk*>(smem + C::kOffStart);
   auto colS = [](int t) -> uint32_t { return static_cast<uint32_t>(t * 128); };
   auto colO = [](int t) -> uint32_t { return static_cast<uint32_t>(NT * 128 + t * 128); };
   // The plan's scratch (generic writes) lies where TMA will write.
@@ -404,10 +262,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
     uint32_t L = 0;               // K/V loads issued by this CTA (ring position)
     uint32_t n_q[2] = {0, 0};     // Q tiles loaded
     uint32_t n_seg = 0;
-    const int boxes = kBN / p.box;  // of one tile; lane 2i + e loads half e of box i
-    const int my_slot = (lane >> 1) * p.box;
-    const bool loader = (lane >> 1) < boxes;
-    const uint32_t my_dst = (lane & 1) * kHalf + my_slot * 128;
+    const Boxes boxes(p.box, lane);
     Seg s;
     while (ok && next_seg(p, walk, s)) {
       // Q tiles are reused once the previous segment's last QK^T is done
@@ -421,29 +276,14 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
             const uint32_t dst = sbase + C::kOffQ + t * kTileBytes;
             mbar_expect_tx(bar(B_QFULL + t), 2 * 128 * p.G * p.tpt);
             for (int e = 0; e < 2; ++e)
-              tma_load_4d(dst + e * kHalf, &tmQ, bar(B_QFULL + t), 64 * e, s.h * p.G, s.a + s.tok0 + t * p.tpt, 0);
+              tma_load_4d(dst + e * kHalf, &tmQ, bar(B_QFULL + t), 64 * e, s.h * p.G, s.s.a + s.tok0 + t * p.tpt, 0);
           }
         }
       }
       ++n_seg;
-      const int n = s.kv1 - s.kv0;
-      const int32_t* table = p.table + static_cast<size_t>(s.b) * p.max_pages;
-      // This lane's box of tile j: its page from the block table, and its first pool row
-      // (-1: past the last slot seen).  The table is read one K tile ahead.
-      auto page_of = [&](int j) -> int {
-        const int slot = j * kBN + my_slot;
-        return loader && j < s.n_kv && slot < s.limit ? __ldg(table + slot / p.page_size) : -1;
-      };
-      auto row_of = [&](int j, int page) -> int {
-        const int slot = j * kBN + my_slot;
-        if (!loader || slot >= s.limit) return -1;
-        if (page < 0 || page >= p.num_pages) {
-          record_input_error(SITE_BAD_PAGE);
-          page = 0;  // keep the pipeline flowing; the call reports the input error
-        }
-        return (page * p.Hkv + s.h) * p.page_size + slot % p.page_size;
-      };
-      int page_next = page_of(s.kv0);
+      const int n = s.k1 - s.k0;
+      const int32_t* table = p.batch.table + static_cast<size_t>(s.b) * p.batch.max_pages;
+      int page_next = boxes.page(p.batch, table, s.k0 * kBN, s.limit);  // read one K tile ahead
       int row_k = -1, row_v = -1;  // rows of the latest K tile and of the tile whose V comes next
       for (int li = 0; ok && li < 2 * n; ++li) {
         const int st = static_cast<int>(L % kStages);
@@ -454,10 +294,10 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
         if (is_v) {
           row = li == 2 * n - 1 ? row_k : row_v;
         } else {
-          const int j = s.kv0 + (li == 0 ? 0 : (li + 1) >> 1);
+          const int slot0 = (s.k0 + (li == 0 ? 0 : (li + 1) >> 1)) * kBN;
           row_v = row_k;
-          row_k = row_of(j, page_next);
-          page_next = page_of(j + 1);
+          row_k = boxes.row(p.batch, page_next, s.h, slot0, s.limit, SITE_BAD_PAGE);
+          page_next = boxes.page(p.batch, table, slot0 + kBN, s.limit);
           row = row_k;
         }
         if (r > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_KVEMPTY + st), (r - 1) & 1u, SITE_PRODUCER));
@@ -466,8 +306,8 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
         if (lane == 0) mbar_expect_tx(bar(B_KVFULL + st), __popc(mine) * p.box * 128);
         __syncwarp();
         if (row >= 0)
-          tma_load_3d(sbase + C::kOffKV + st * kTileBytes + my_dst, is_v ? &tmV : &tmK, bar(B_KVFULL + st),
-                      (lane & 1) * 64, row, 0);
+          tma_load_3d(sbase + C::kOffKV + st * kTileBytes + boxes.offset, is_v ? &tmV : &tmK, bar(B_KVFULL + st),
+                      boxes.half * 64, row, 0);
         ++L;
       }
     }
@@ -516,7 +356,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
       uint32_t uc = 0;                // segments with this tile
       Seg s;
       while (ok && next_seg(p, walk, s)) {
-        const int n = s.kv1 - s.kv0;
+        const int n = s.k1 - s.k0;
         auto wait_kv = [&](uint32_t ii) -> bool {
           return mbar_wait_spin(bar(B_KVFULL + ii % kStages), (ii / kStages) & 1u, SITE_MMA);
         };
@@ -579,13 +419,13 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
     uint32_t L = 0, Z = 0;
     Seg s;
     while (ok && next_seg(p, walk, s)) {
-      const int n = s.kv1 - s.kv0;
+      const int n = s.k1 - s.k0;
       for (int li = 0; ok && li < 2 * n; ++li) {  // a reader like the issuers, in step with the ring
         const int st = static_cast<int>((L + li) % kStages);
         ok = __all_sync(0xffffffffu, mbar_wait(bar(B_KVFULL + st), ((L + li) / kStages) & 1u, SITE_HELPER));
         if (!ok) break;
         if (li == 2 * n - 1 && s.tail()) {
-          const int first = s.limit - (s.n_kv - 1) * kBN;  // rows [first, 128) of the V tile
+          const int first = s.limit - (s.count - 1) * kBN;  // rows [first, 128) of the V tile
           uint8_t* v = smem + C::kOffKV + st * kTileBytes;
           for (int i = first * 8 + lane; i < kBN * 8; i += 32) {
             *reinterpret_cast<uint4*>(v + i * 16) = make_uint4(0, 0, 0, 0);
@@ -624,10 +464,10 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
     // the two halves of a tile can never wait on each other forever.
     while (next_seg(p, walk, s)) {
       if (t * p.tpt >= s.n_tok) continue;  // no rows in this tile
-      const int n = s.kv1 - s.kv0;
+      const int n = s.k1 - s.k0;
       // last slot this row sees (a row without a token computes what nobody reads, unmasked,
       // so that its warp takes the masked path only where a real row needs it)
-      const int lim = my_tok < s.n_tok ? (p.causal ? s.base + s.tok0 + my_tok : s.L - 1) : 0x3FFFFFFF;
+      const int lim = my_tok < s.n_tok ? (p.causal ? s.base + s.tok0 + my_tok : s.s.L - 1) : 0x3FFFFFFF;
       // warps without any token's row only keep the hand-offs going
       const bool work = __any_sync(0xffffffffu, my_tok < s.n_tok);
       float m_run = -INFINITY, l_run = 0.0f, lf_run = 0.0f;
@@ -636,7 +476,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_SFULL + t), gi & 1u, SITE_SOFTMAX));
         uint32_t s0[32], s1[32];
         float mx0 = -INFINITY, mx1 = -INFINITY;
-        const int rel = lim - (s.kv0 + j) * kBN - 64 * h;  // columns (of this half) > rel are masked
+        const int rel = lim - (s.k0 + j) * kBN - 64 * h;  // columns (of this half) > rel are masked
         if (ok && work) {
           tc_fence_after();
           tmem_ld32(tS + 0, s0);
@@ -724,11 +564,11 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
       if (ok && work) {
         tc_fence_after();
         const bool mine = my_tok < s.n_tok;
-        const bool whole = s.kv0 == 0 && s.kv1 == s.n_kv;
+        const bool whole = s.whole();
         const int hd = r % p.G;
         if (whole) {
           const float inv_l = l_tot > 0.0f ? 1.0f / l_tot : 0.0f;
-          const long long tok = s.a + s.tok0 + my_tok;
+          const long long tok = s.s.a + s.tok0 + my_tok;
           const int head = s.h * p.G + hd;
           uint16_t* dst = p.o + tok * p.o_t + head * p.o_h + 64 * h;
 #pragma unroll 1
@@ -752,7 +592,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
             p.lse[tok * p.Hq + head] = lf_tot > 0.0f ? (m_run + log2f(lf_tot)) * kLn2 : -INFINITY;
         } else {
           // a segment: (O, m, l) to this CTA's slot, 16 bytes of 32 rows side by side
-          const int slot = 2 * blockIdx.x + (s.kv0 == 0 ? 1 : 0);
+          const int slot = 2 * blockIdx.x + (s.k0 == 0 ? 1 : 0);
           const int row = t * 128 + r;
           float4* dst = p.part_o + (static_cast<size_t>(slot) * 32 + 16 * h) * p.part_rows + row;
 #pragma unroll 1
@@ -799,8 +639,10 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const Params p, in
   const int c0 = blockIdx.x;
   const Desc d = p.desc[c0];
   if (!d.valid) return;
+  const Seq s = seq_of(p.batch, d.b);
+  const int n_tok = min(p.tu, s.n - d.u * p.tu);
   const int rows_tile = p.tpt * p.G;
-  const int rows = (d.n_tok > p.tpt ? 128 : 0) + (d.n_tok - (d.n_tok > p.tpt ? p.tpt : 0)) * p.G;
+  const int rows = n_tok > p.tpt ? 128 + (n_tok - p.tpt) * p.G : n_tok * p.G;
   const int lane = threadIdx.x & 31;
   const int items = ((rows + 31) / 32) * 16;  // (32 rows, 8 dims) per warp
   for (int it = blockIdx.y * (kMergeThreads / 32) + (threadIdx.x >> 5); it < items;
@@ -828,7 +670,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const Params p, in
       acc[4] += b.x * w, acc[5] += b.y * w, acc[6] += b.z * w, acc[7] += b.w * w;
     }
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    const long long tok = d.token0 + t * p.tpt + r / p.G;
+    const long long tok = s.a + d.u * p.tu + t * p.tpt + r / p.G;
     const int head = d.h * p.G + r % p.G;
     *reinterpret_cast<uint4*>(p.o + tok * p.o_t + head * p.o_h + 8 * d8) =
         make_uint4(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv),
@@ -920,9 +762,7 @@ extern "C" int gqa_attend_chunk_bf16(const void* q, long long q_token_stride, lo
   if (!workspace || workspace_bytes < w.bytes) return GQA_ERR_WORKSPACE;
 
   Params p;
-  p.table = block_table;
-  p.q_start = q_start;
-  p.lens = lens;
+  p.batch = {block_table, q_start, lens, B, T, Hkv, static_cast<int>(capacity), max_pages_per_seq, page_size, num_pages};
   p.o = static_cast<uint16_t*>(o);
   p.lse = lse;
   char* ws = static_cast<char*>(workspace);
@@ -932,9 +772,7 @@ extern "C" int gqa_attend_chunk_bf16(const void* q, long long q_token_stride, lo
   p.part_rows = w.rows;
   p.o_t = o_token_stride;
   p.o_h = o_head_stride;
-  p.B = B, p.T = T, p.G = G, p.Hq = Hq, p.Hkv = Hkv;
-  p.capacity = static_cast<int>(capacity);
-  p.max_pages = max_pages_per_seq, p.page_size = page_size, p.num_pages = num_pages;
+  p.G = G, p.Hq = Hq;
   p.causal = (flags & GQA_FLAG_CAUSAL) != 0;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.box = std::min(128, page_size & -page_size);

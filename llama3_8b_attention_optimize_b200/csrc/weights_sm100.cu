@@ -1,88 +1,425 @@
-// weights_sm100.cu -- accumulated attention weight of every cached slot.
+// weights_sm100.cu -- accumulated attention weight of every cached slot, on the sm_100a
+// tensor core.
 //
 // For the chunk of attend_sm100.cu (same q_start, lens, slots and mask) and its lse,
 //   acc_out[b, h, j] = (j < lens[b] - n ? acc[b, h, j] : 0)
 //                      + sum over the group's heads and the chunk's tokens that see slot j
 //                        of exp(q . K[b, h, j] * scale - lse),
-// for j < lens[b]; entries at lens[b] and above are left alone.  Slots that the chunk itself wrote start
-// from zero.  Each sum is taken by one thread in token order: no atomics, the same bits on every run.
+// for j < lens[b]; entries at lens[b] and above are left alone.  Slots that the chunk
+// itself wrote start from zero.
 //
-// One thread per slot, K's row in registers, a query row at a time in shared memory.
+// With the lse known nothing has to be normalised, so the scores are computed transposed:
+// S^T = K Q^T puts a slot on a TMEM lane and the (token, head) rows on columns, and a
+// slot's sum stays in one thread's registers.  K is read once, no score is written, and
+// the order of every sum is fixed: runs repeat bit for bit.
+//
+// Unit of work: (sequence, kv head, block of 256 slots), two 128-slot K tiles side by side
+// that share the query tiles (128 rows: G heads of 128 / G tokens) it walks as steps; the
+// steps of all units are cut into equal parts, one per CTA and SM (ragged.cuh).  Parts of
+// one unit leave 256 sums each, which a second kernel adds in order.
+//
+// Pipeline: a producer warp (K tiles two units ahead, query tiles in a ring of 3), one
+// MMA-issuing warp per K tile (two S^T buffers each: all 512 TMEM columns), a helper warp
+// that stages each query tile's lse, and eight softmax warps per K tile (a thread: one
+// slot, 64 of the 128 rows).
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "attn_common.cuh"
 #include "common.cuh"
 #include "gqa_internal.h"
+#include "ragged.cuh"
 
 namespace gqa {
 namespace weights {
 
+using ragged::Boxes;
+using ragged::Desc;
+using ragged::kMaxB;
+using ragged::kMaxCtas;
+using ragged::Part;
+using ragged::Seq;
+using ragged::seq_of;
+using ragged::Walk;
+
 constexpr int kD = 128;
+constexpr int kBlock = 256;                // slots of a unit: two K tiles
+constexpr int kTileBytes = 128 * 128 * 2;  // K and Q tiles: 32 KB
+constexpr int kHalf = kTileBytes / 2;
+constexpr int kQStages = 3;
+constexpr float kLog2e = 1.4426950408889634f;
+
+constexpr int kSoftmaxWarps = 16;
+constexpr int kWarpProducer = 16;
+constexpr int kWarpMma = 17;  // and 18: one per K tile
+constexpr int kWarpHelper = 19;
+constexpr int kThreads = 640;
+
+constexpr int kOffQ = 0;
+constexpr int kOffK = kOffQ + kQStages * kTileBytes;  // [unit % 2][K tile]
+constexpr int kOffBar = kOffK + 4 * kTileBytes;
+constexpr int kNumBars = 32;
+constexpr int kOffLse = kOffBar + kNumBars * 8;     // [2][128] -lse * log2(e)
+constexpr int kOffSum = kOffLse + 2 * 128 * 4;      // [K tile][128] sums of the rows' second half
+constexpr int kOffTok = kOffSum + 2 * 128 * 4;      // [128] token of a row in its tile
+constexpr int kOffTmemPtr = kOffTok + 128;
+constexpr int kOffStart = kOffTmemPtr + 16;
+constexpr int kSmemBytes = kOffStart + 32;
+static_assert(kSmemBytes <= 232448, "shared memory over the per-block limit");
+static_assert(kMaxB * 8 + 64 * 8 <= 4 * kTileBytes, "the plan's scratch lies in the K tiles");
+static_assert(sizeof(Walk) <= 32, "room for the start");
 
 enum : int {
+  B_QFULL = 0,    // [3]
+  B_QEMPTY = 3,   // [3] one arrival per issuer
+  B_KFULL = 6,    // [4]
+  B_KEMPTY = 10,  // [4]
+  B_SFULL = 14,   // [K tile][2]
+  B_SFREE = 18,   // [K tile][2] one arrival per softmax warp
+  B_LFULL = 22,   // [2] lse of a query tile staged
+  B_LEMPTY = 24,  // [2] one arrival per softmax warp
+  B_DRAIN = 26,   // [2]
+};
+
+enum : int {
+  SITE_PRODUCER = 0x711,
+  SITE_MMA = 0x712,
+  SITE_SOFTMAX = 0x713,
+  SITE_HELPER = 0x714,
+  SITE_DRAIN = 0x716,
+  SITE_SMEM_ALIGN = 0x717,
   SITE_Q_START = 0x630,   // q_start not ascending or outside [0, T]
   SITE_LENGTH = 0x631,    // lens[b] outside [0, capacity]
   SITE_BAD_PAGE = 0x632,  // block-table entry outside [0, num_pages)
 };
 
 struct Params {
-  const uint16_t *q, *kp;
+  ragged::Batch batch;
   const float *lse, *acc;
   float* acc_out;
-  const int32_t *table, *q_start, *lens;
-  long long q_t, q_h;
-  int B, T, Hq, Hkv, max_pages, page_size, num_pages, causal;
-  float scale;
+  float* part;  // [2 * grid][kBlock]
+  Desc* desc;   // [grid]
+  int G, Hq, causal, tpt, box;
+  float scale_log2;
 };
 
-__global__ void __launch_bounds__(128) weights_kernel(const Params p) {
-  __shared__ float sq[kD];
-  const int hk = blockIdx.y % p.Hkv, b = blockIdx.y / p.Hkv, G = p.Hq / p.Hkv;
-  const long long capacity = static_cast<long long>(p.max_pages) * p.page_size;
-  int len = p.lens[b], a = p.q_start[b], z = p.q_start[b + 1];
-  if (len < 0 || len > capacity) {
-    if (threadIdx.x == 0) record_input_error(SITE_LENGTH);
-    len = static_cast<int>(min(max(static_cast<long long>(len), 0ll), capacity));
+// Units: blocks of 256 slots.  Steps: the query tiles of which some row sees the block; one
+// (empty) step where the sequence brings no tokens, to pass its sums on.
+struct Line {
+  int tpt, causal;
+  __device__ __forceinline__ Line(const Params& p) : tpt(p.tpt), causal(p.causal) {}
+  __device__ __forceinline__ int units(const Seq& s) const { return (s.L + kBlock - 1) / kBlock; }
+  __device__ __forceinline__ int tiles(const Seq& s) const { return (s.n + tpt - 1) / tpt; }
+  // first query tile that sees slot kBlock * u: floor((kBlock u - (L - n)) / tpt), at least 0
+  __device__ __forceinline__ int first(const Seq& s, int u) const {
+    const long long x = static_cast<long long>(u) * kBlock - (s.L - s.n);
+    return !causal || x <= 0 ? 0 : static_cast<int>(x / tpt);
   }
-  if (a < 0 || z < a || z > p.T) {
-    if (threadIdx.x == 0) record_input_error(SITE_Q_START);
-    a = z = 0;
+  __device__ __forceinline__ int count(const Seq& s, int u) const { return s.n == 0 ? 1 : tiles(s) - first(s, u); }
+  __device__ __forceinline__ long long before(const Seq& s, int k) const {
+    if (s.n == 0) return k;
+    long long sum = static_cast<long long>(k) * tiles(s);
+    const long long base = s.L - s.n;
+    const int u1 = base > 0 ? static_cast<int>((base + kBlock - 1) / kBlock) : 0;  // first unit past the old slots
+    if (causal && k > u1) sum -= ragged::floor_sum(k - u1, tpt, kBlock, static_cast<long long>(u1) * kBlock - base);
+    return sum;
   }
-  if (static_cast<int>(blockIdx.x) * 128 >= len) return;  // the whole block
-  const int j = blockIdx.x * 128 + threadIdx.x;
-  uint32_t k[64];
-  if (j < len) {
-    int page = p.table[static_cast<long long>(b) * p.max_pages + j / p.page_size];
-    if (page < 0 || page >= p.num_pages) {
-      record_input_error(SITE_BAD_PAGE);
-      page = 0;
+};
+
+// p = 2^(s * sl2 + nl) of 32 rows that all see the slot
+__device__ __forceinline__ void add_all(const uint32_t (&s)[32], const float* nl, float2 sl2, float2& a0, float2& a1) {
+#pragma unroll
+  for (int c = 0; c < 32; c += 4) {
+    const float4 l = *reinterpret_cast<const float4*>(nl + c);
+    const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sl2, make_float2(l.x, l.y));
+    const float2 y =
+        __ffma2_rn(make_float2(__uint_as_float(s[c + 2]), __uint_as_float(s[c + 3])), sl2, make_float2(l.z, l.w));
+    a0 = __fadd2_rn(a0, make_float2(ex2_approx(x.x), ex2_approx(x.y)));
+    a1 = __fadd2_rn(a1, make_float2(ex2_approx(y.x), ex2_approx(y.y)));
+  }
+}
+
+// the same where rows end (nv of them) or see only some slots: row c sees the slot if
+// its token is at least `from` within the tile
+__device__ __forceinline__ void add_some(const uint32_t (&s)[32], const float* nl, const uint8_t* tok, int nv, int from,
+                                         float sl2, float2& a0) {
+#pragma unroll
+  for (int c = 0; c < 32; ++c) {
+    const float e = ex2_approx(fmaf(__uint_as_float(s[c]), sl2, nl[c]));
+    if (c < nv && static_cast<int>(tok[c]) >= from) a0.x += e;  // anything else may be NaN
+  }
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+    weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const Params p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0) record_error(SITE_SMEM_ALIGN);
+    return;
+  }
+  const uint32_t sbase = smem_u32(smem);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  auto bar = [&](int i) -> uint32_t { return sbase + kOffBar + 8 * i; };
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kQStages; ++i) {
+      mbar_init(bar(B_QFULL + i), 1);
+      mbar_init(bar(B_QEMPTY + i), 2);
     }
-    const uint4* row = reinterpret_cast<const uint4*>(
-        p.kp + ((static_cast<size_t>(page) * p.Hkv + hk) * p.page_size + j % p.page_size) * kD);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) *reinterpret_cast<uint4*>(k + 4 * i) = row[i];
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(bar(B_KFULL + i), 1);
+      mbar_init(bar(B_KEMPTY + i), 1);
+      mbar_init(bar(B_SFULL + i), 1);
+      mbar_init(bar(B_SFREE + i), 8);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(B_LFULL + i), 32);
+      mbar_init(bar(B_LEMPTY + i), kSoftmaxWarps);
+      mbar_init(bar(B_DRAIN + i), 1);
+    }
+    fence_mbar_init();
   }
-  float sum = 0.0f;
-  for (int t = a; t < z; ++t) {
-    const int last = p.causal ? len - z + t : len - 1;
-    for (int h = hk * G; h < (hk + 1) * G; ++h) {
-      __syncthreads();
-      sq[threadIdx.x] = bf2f_bits(p.q[t * p.q_t + h * p.q_h + threadIdx.x]);
-      __syncthreads();
-      const float lse = p.lse[static_cast<size_t>(t) * p.Hq + h];
-      if (j < len && j <= last && lse != -INFINITY) {
-        float s = 0.0f;
+  if (threadIdx.x < 128) smem[kOffTok + threadIdx.x] = static_cast<uint8_t>(threadIdx.x / p.G);
+  if (warp == kWarpMma) {
+    tmem_alloc(sbase + kOffTmemPtr, 512);
+    tmem_relinquish();
+  }
+  if (warp == kWarpProducer && lane == 0) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+  }
+  const Line line(p);
+  ragged::plan<kThreads>(p.batch, line, reinterpret_cast<long long*>(smem + kOffK),
+                         reinterpret_cast<Walk*>(smem + kOffStart), p.desc, SITE_Q_START, SITE_LENGTH);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + kOffTmemPtr);
+  Walk walk = *reinterpret_cast<const Walk*>(smem + kOffStart);
+  // The plan's scratch (generic writes) lies where TMA will write.
+  fence_proxy_async_smem();
+  __syncthreads();
+  Part s;
+
+  if (warp == kWarpProducer) {
+    // ------------------------------------------------------------ TMA producer (whole warp)
+    bool ok = true;
+    uint32_t g = 0, m = 0;  // query tiles and units loaded
+    const Boxes boxes(p.box, lane);
+    while (ok && ragged::next_part(p.batch, line, walk, s)) {
+      if (s.s.n == 0) continue;
+      const int32_t* table = p.batch.table + static_cast<size_t>(s.b) * p.batch.max_pages;
+      const int slot0 = s.u * kBlock;
+      int page[2];
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
-          s = fmaf(sq[2 * i], bf16_lo(k[i]), s);
-          s = fmaf(sq[2 * i + 1], bf16_hi(k[i]), s);
+      for (int kt = 0; kt < 2; ++kt) page[kt] = boxes.page(p.batch, table, slot0 + 128 * kt, s.s.L);
+      for (int kt = 0; ok && kt < 2 && m >= 2; ++kt)
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(B_KEMPTY + 2 * (m & 1) + kt), (m / 2 - 1) & 1u, SITE_PRODUCER));
+      if (!ok) break;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        const int st = 2 * (m & 1) + kt;
+        const int row = boxes.row(p.batch, page[kt], s.h, slot0 + 128 * kt, s.s.L, SITE_BAD_PAGE);
+        const uint32_t mine = __ballot_sync(0xffffffffu, row >= 0);
+        if (lane == 0) mbar_expect_tx(bar(B_KFULL + st), __popc(mine) * p.box * 128);
+        __syncwarp();
+        if (row >= 0)
+          tma_load_3d(sbase + kOffK + st * kTileBytes + boxes.offset, &tmK, bar(B_KFULL + st), boxes.half * 64, row, 0);
+      }
+      ++m;
+      const int first = line.first(s.s, s.u);
+      for (int k = s.k0; k < s.k1; ++k, ++g) {
+        const int st = static_cast<int>(g % kQStages);
+        if (g >= kQStages)
+          ok = __all_sync(0xffffffffu, mbar_wait(bar(B_QEMPTY + st), (g / kQStages - 1) & 1u, SITE_PRODUCER));
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_expect_tx(bar(B_QFULL + st), 2 * 128 * p.G * p.tpt);
+          for (int e = 0; e < 2; ++e)
+            tma_load_4d(sbase + kOffQ + st * kTileBytes + e * kHalf, &tmQ, bar(B_QFULL + st), 64 * e, s.h * p.G,
+                        s.s.a + (first + k) * p.tpt, 0);
         }
-        sum += expf(fmaf(s, p.scale, -lse));
+      }
+    }
+    // Drain: every load this warp issued must land before the CTA may exit.
+    for (uint32_t i = g > kQStages ? g - kQStages : 0u; i < g; ++i)
+      mbar_wait_drain(bar(B_QFULL + static_cast<int>(i % kQStages)), (i / kQStages) & 1u, SITE_DRAIN);
+    for (uint32_t i = m > 2 ? m - 2 : 0u; i < m; ++i)
+      for (int kt = 0; kt < 2; ++kt) mbar_wait_drain(bar(B_KFULL + 2 * (i & 1) + kt), (i / 2) & 1u, SITE_DRAIN);
+    __syncwarp();
+  } else if (warp == kWarpMma || warp == kWarpMma + 1) {
+    // ------------------------------------------------------------ MMA issuers, one per K tile
+    const int kt = warp - kWarpMma;
+    if (lane == 0) {
+      constexpr uint32_t kHi = sdesc_hi_sw128(1024);
+      const uint32_t k_lo = sdesc_lo(sbase + kOffK + kt * kTileBytes, 16);
+      const uint32_t q_lo = sdesc_lo(sbase + kOffQ, 16);
+      constexpr uint32_t kTile16 = kTileBytes / 16;
+      bool ok = true;
+      uint32_t g = 0, m = 0;
+      while (ok && ragged::next_part(p.batch, line, walk, s)) {
+        if (s.s.n == 0) continue;
+        const int ks = 2 * (m & 1) + kt;
+        const uint32_t a0 = k_lo + 2 * (m & 1) * kTile16;
+        ok = mbar_wait_spin(bar(B_KFULL + ks), (m / 2) & 1u, SITE_MMA);
+        const int first = line.first(s.s, s.u);
+        for (int k = s.k0; ok && k < s.k1; ++k, ++g) {
+          const int st = static_cast<int>(g % kQStages), bb = static_cast<int>(g & 1);
+          ok = mbar_wait_spin(bar(B_QFULL + st), (g / kQStages) & 1u, SITE_MMA) &&
+               (g < 2 || mbar_wait_spin(bar(B_SFREE + 2 * kt + bb), (g / 2 - 1) & 1u, SITE_MMA));
+          if (!ok) break;
+          // only as many columns as the tile has rows, in the MMA's steps of 16
+          const int nv = min(p.tpt, s.s.n - (first + k) * p.tpt) * p.G;
+          const uint32_t id = idesc_bf16_f32(128, (nv + 15) / 16 * 16, false);
+          const uint32_t b0 = q_lo + st * kTile16;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            const uint32_t off = ((kk >> 2) * kHalf + (kk & 3) * 32) / 16;
+            umma_ss_lohi(tmem + 256 * kt + 128 * bb, a0 + off, b0 + off, kHi, id, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(bar(B_SFULL + 2 * kt + bb));
+          umma_commit(bar(B_QEMPTY + st));
+          if (k + 1 == s.k1) umma_commit(bar(B_KEMPTY + ks));
+        }
+        ++m;
+      }
+      umma_commit(bar(B_DRAIN + kt));
+      mbar_wait_drain(bar(B_DRAIN + kt), 0, SITE_DRAIN);
+    }
+    __syncwarp();
+  } else if (warp == kWarpHelper) {
+    // ------------------------------------------------------------ lse of each query tile
+    bool ok = true;
+    uint32_t g = 0;
+    int tok[4], head[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      tok[i] = (lane + 32 * i) / p.G;
+      head[i] = (lane + 32 * i) % p.G;
+    }
+    while (ok && ragged::next_part(p.batch, line, walk, s)) {
+      if (s.s.n == 0) continue;
+      const int first = line.first(s.s, s.u);
+      for (int k = s.k0; ok && k < s.k1; ++k, ++g) {
+        const int t0 = (first + k) * p.tpt, bb = static_cast<int>(g & 1);
+        float nl[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          nl[i] = -INFINITY;  // no row, or one that saw nothing
+          if (tok[i] < p.tpt && t0 + tok[i] < s.s.n) {
+            const float x = __ldg(p.lse + static_cast<size_t>(s.s.a + t0 + tok[i]) * p.Hq + s.h * p.G + head[i]);
+            if (x != -INFINITY) nl[i] = -x * kLog2e;
+          }
+        }
+        if (g >= 2) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_LEMPTY + bb), (g / 2 - 1) & 1u, SITE_HELPER));
+        if (!ok) break;
+        float* dst = reinterpret_cast<float*>(smem + kOffLse) + 128 * bb;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dst[lane + 32 * i] = nl[i];
+        mbar_arrive(bar(B_LFULL + bb));
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ softmax warps
+    const int kt = warp >> 3;          // K tile
+    const int ch = (warp >> 2) & 1;    // rows [64 ch, 64 ch + 64) of each query tile
+    const int r = (warp & 3) * 32 + lane;  // slot in the K tile == TMEM lane
+    const uint32_t tS = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + 256 * kt + 64 * ch;
+    const float* lse = reinterpret_cast<const float*>(smem + kOffLse);
+    const uint8_t* tok = smem + kOffTok;
+    float* xsum = reinterpret_cast<float*>(smem + kOffSum) + 128 * kt;
+    const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
+    bool ok = true;
+    uint32_t g = 0;
+    // Every warp meets the named barriers of every unit, even after a failed wait.
+    while (ragged::next_part(p.batch, line, walk, s)) {
+      const int slot = s.u * kBlock + 128 * kt + r;
+      const int warp_last = min(s.s.L, s.u * kBlock + 128 * kt + (warp & 3) * 32 + 32) - 1;
+      float sum = 0.0f;
+      if (s.s.n > 0) {
+        const int first = line.first(s.s, s.u);
+        for (int k = s.k0; k < s.k1; ++k, ++g) {
+          const int bb = static_cast<int>(g & 1);
+          const int t0 = (first + k) * p.tpt;
+          const int nv = min(p.tpt, s.s.n - t0) * p.G - 64 * ch;  // rows of this half
+          // the tile's first token sees slots up to see0, each next token one more
+          const int see0 = p.causal ? s.s.L - s.s.n + t0 : s.s.L - 1;
+          if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_SFULL + 2 * kt + bb), (g / 2) & 1u, SITE_SOFTMAX));
+          if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_LFULL + bb), (g / 2) & 1u, SITE_SOFTMAX));
+          if (!ok) continue;
+          uint32_t s0[32], s1[32];
+          if (nv > 0) {
+            tc_fence_after();
+            tmem_ld32(tS + 128 * bb, s0);
+            if (nv > 32) tmem_ld32(tS + 128 * bb + 32, s1);
+            tmem_wait_ld_dep(s0);
+            reg_dep(s1);
+            tc_fence_before();
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(B_SFREE + 2 * kt + bb));
+          if (nv > 0) {
+            const float* nl = lse + 128 * bb + 64 * ch;
+            float2 a0 = make_float2(0.f, 0.f), a1 = make_float2(0.f, 0.f);
+            const bool all = see0 >= warp_last;
+            const int from = slot - see0;  // a row of a token below this does not see the slot
+            if (all && nv >= 32)
+              add_all(s0, nl, sl2, a0, a1);
+            else
+              add_some(s0, nl, tok + 64 * ch, nv, p.causal ? from : 0, p.scale_log2, a0);
+            if (all && nv >= 64)
+              add_all(s1, nl + 32, sl2, a0, a1);
+            else if (nv > 32)
+              add_some(s1, nl + 32, tok + 64 * ch + 32, nv - 32, p.causal ? from : 0, p.scale_log2, a0);
+            sum += (a0.x + a0.y) + (a1.x + a1.y);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(B_LEMPTY + bb));
+        }
+      }
+      named_bar_sync(3 + kt, 256);  // the previous unit's exchange has been read
+      if (ch == 1) xsum[r] = sum;
+      named_bar_sync(1 + kt, 256);
+      if (ok && ch == 0 && slot < s.s.L) {
+        sum += xsum[r];
+        if (s.whole()) {
+          const size_t at = (static_cast<size_t>(s.b) * p.batch.Hkv + s.h) * p.batch.capacity + slot;
+          p.acc_out[at] = (slot < s.s.L - s.s.n ? p.acc[at] : 0.0f) + sum;
+        } else {
+          p.part[static_cast<size_t>(2 * blockIdx.x + (s.k0 == 0 ? 1 : 0)) * kBlock + 128 * kt + r] = sum;
+        }
       }
     }
   }
-  if (j < len) {
-    const size_t at = static_cast<size_t>(blockIdx.y) * capacity + j;
-    p.acc_out[at] = (j < len - (z - a) ? p.acc[at] : 0.0f) + sum;
+
+  // ---- teardown: everyone done with TMEM and shared memory
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kWarpMma) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
 }
+
+// Add a split unit's parts in order: block c takes the unit that CTA c began, if any.
+__global__ void __launch_bounds__(kBlock) merge_kernel(const Params p) {
+  cudaGridDependencySynchronize();
+  const Desc d = p.desc[blockIdx.x];
+  if (!d.valid) return;
+  const Seq s = seq_of(p.batch, d.b);
+  const int slot = d.u * kBlock + threadIdx.x;
+  if (slot >= s.L) return;
+  float sum = 0.0f;
+  for (int c = blockIdx.x; c <= d.last; ++c)
+    sum += p.part[static_cast<size_t>(2 * c + (c == static_cast<int>(blockIdx.x) ? 1 : 0)) * kBlock + threadIdx.x];
+  const size_t at = (static_cast<size_t>(d.b) * p.batch.Hkv + d.h) * p.batch.capacity + slot;
+  p.acc_out[at] = (slot < s.L - s.n ? p.acc[at] : 0.0f) + sum;
+}
+
+constexpr size_t kPartBytes = static_cast<size_t>(2 * kMaxCtas) * kBlock * sizeof(float);
 
 }  // namespace weights
 
@@ -92,34 +429,76 @@ GQA_ERROR_FLAG_ACCESSOR(error_flag_weights)
 
 using namespace gqa;
 
+extern "C" size_t gqa_attn_weight_sums_workspace_size(void) {
+  return weights::kPartBytes + weights::kMaxCtas * sizeof(ragged::Desc);
+}
+
 extern "C" int gqa_attn_weight_sums_f32(const void* q, long long q_token_stride, long long q_head_stride,
                                         const void* kpages, const int32_t* block_table, int max_pages_per_seq,
                                         int page_size, int num_pages, const int32_t* q_start, const int32_t* lens,
-                                        const float* lse, const float* acc, float* acc_out, int B, int T, int Hq,
-                                        int Hkv, int head_dim, int max_q_len, float scale, int flags,
-                                        gqa_stream_t stream) {
+                                        const float* lse, const float* acc, float* acc_out, void* workspace,
+                                        size_t workspace_bytes, int B, int T, int Hq, int Hkv, int head_dim, float scale,
+                                        int flags, gqa_stream_t stream) {
   using namespace weights;
   if (B <= 0 || T < 0 || Hq <= 0 || Hkv <= 0 || max_pages_per_seq <= 0 || page_size <= 0 || num_pages <= 0)
     return GQA_ERR_INVALID_ARGUMENT;
   if (head_dim != kD || Hq % Hkv || page_size % 16) return GQA_ERR_UNSUPPORTED;
-  if (!(scale > 0.0f) || !(scale < 1e30f) || (flags & ~GQA_FLAG_CAUSAL) || max_q_len < 0) return GQA_ERR_INVALID_ARGUMENT;
+  if (!(scale > 0.0f) || !(scale < 1e30f) || (flags & ~GQA_FLAG_CAUSAL)) return GQA_ERR_INVALID_ARGUMENT;
   if (q_token_stride < 0 || q_head_stride < 0) return GQA_ERR_INVALID_ARGUMENT;
   if (!kpages || !block_table || !q_start || !lens || !acc || !acc_out || (T > 0 && (!q || !lse)))
     return GQA_ERR_INVALID_ARGUMENT;
   auto odd = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr) % 4 != 0; };
   if (!aligned16(q) || !aligned16(kpages) || odd(block_table) || odd(q_start) || odd(lens) || odd(lse) || odd(acc) ||
-      odd(acc_out))
+      odd(acc_out) || !aligned16(workspace))
     return GQA_ERR_MISALIGNED;
   if ((T > 1 && q_token_stride % 8) || (Hq > 1 && q_head_stride % 8)) return GQA_ERR_MISALIGNED;
+  const int G = Hq / Hkv;
   const long long capacity = static_cast<long long>(max_pages_per_seq) * page_size;
+  const long long pool_rows = static_cast<long long>(num_pages) * Hkv * page_size;
+  if (G > 128 || B > kMaxB || capacity > 0x7FFFFE00LL || pool_rows > 0x7FFFFFFFLL) return GQA_ERR_UNSUPPORTED;
+  // a TMA dimension needs a stride: heads or tokens that share one row are the caller's to expand
+  if ((T > 1 && q_token_stride == 0) || (Hq > 1 && q_head_stride == 0)) return GQA_ERR_UNSUPPORTED;
+  if (!workspace || workspace_bytes < gqa_attn_weight_sums_workspace_size()) return GQA_ERR_WORKSPACE;
+
   Params p;
-  p.q = static_cast<const uint16_t*>(q);
-  p.kp = static_cast<const uint16_t*>(kpages);
-  p.lse = lse, p.acc = acc, p.acc_out = acc_out;
-  p.table = block_table, p.q_start = q_start, p.lens = lens;
-  p.q_t = q_token_stride, p.q_h = q_head_stride;
-  p.B = B, p.T = T, p.Hq = Hq, p.Hkv = Hkv, p.max_pages = max_pages_per_seq, p.page_size = page_size;
-  p.num_pages = num_pages, p.causal = (flags & GQA_FLAG_CAUSAL) != 0, p.scale = scale;
-  weights_kernel<<<dim3(static_cast<unsigned>((capacity + 127) / 128), B * Hkv), 128, 0, stream>>>(p);
-  return cudaGetLastError() == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
+  p.batch = {block_table, q_start, lens, B, T, Hkv, static_cast<int>(capacity), max_pages_per_seq, page_size, num_pages};
+  p.lse = lse;
+  p.acc = acc;
+  p.acc_out = acc_out;
+  p.part = static_cast<float*>(workspace);
+  p.desc = reinterpret_cast<Desc*>(static_cast<char*>(workspace) + kPartBytes);
+  p.G = G;
+  p.Hq = Hq;
+  p.causal = (flags & GQA_FLAG_CAUSAL) != 0;
+  p.tpt = 128 / G;
+  p.box = std::min(128, page_size & -page_size);
+  p.scale_log2 = scale * kLog2e;
+
+  CUtensorMap tmQ, tmK;
+  int rc;
+  // without tokens nothing is loaded through the query map, but it needs an address
+  const long long ht = Hq > 1 ? q_head_stride : kD, tt = T > 1 ? q_token_stride : static_cast<long long>(Hq) * kD;
+  const long long qd[4] = {kD, Hq, std::max(T, 1), 1}, qs[3] = {ht * 2, tt * 2, tt * 2};
+  const int qb[4] = {64, G, p.tpt, 1};
+  if ((rc = make_tmap_4d(&tmQ, T > 0 ? q : kpages, 2, qd, qs, qb)) != GQA_OK) return rc;
+  if ((rc = make_tmap_3d_bf16(&tmK, kpages, kD, pool_rows, 1, 64, p.box, 1)) != GQA_OK) return rc;
+  static std::atomic<uint64_t> attr_done{0};
+  if ((rc = ensure_smem_attr(weights_kernel, kSmemBytes, attr_done)) != GQA_OK) return rc;
+  int dev = 0, sms = kMaxCtas;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int grid = std::min(sms, kMaxCtas);
+  weights_kernel<<<grid, kThreads, kSmemBytes, stream>>>(tmQ, tmK, p);
+  if (cudaGetLastError() != cudaSuccess) return GQA_ERR_CUDA;
+  // The merge starts while the first kernel drains and waits for it on the device.
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kBlock);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, merge_kernel, static_cast<const Params>(p)) == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }

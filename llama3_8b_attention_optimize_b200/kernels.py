@@ -538,15 +538,22 @@ def attend_chunk(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, bl
     return out
 
 
+def attn_weight_sums_workspace_bytes() -> int:
+    return int(_lib.load().gqa_attn_weight_sums_workspace_size())
+
+
 def attn_weight_sums(q: torch.Tensor, kpages: torch.Tensor, block_table: torch.Tensor, q_start: torch.Tensor,
                      lens: torch.Tensor, lse: torch.Tensor, acc: torch.Tensor, *, causal: bool = True,
-                     scale: float | None = None, max_q_len: int = 0,
-                     acc_out: torch.Tensor | None = None) -> torch.Tensor:
+                     scale: float | None = None, max_q_len: int = 0, acc_out: torch.Tensor | None = None,
+                     workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Add each cached slot's attention weight from this chunk: acc_out[b, h, j] = acc[b, h, j]
     (zero for slots the chunk wrote) + the sum of exp(q . k_j * scale - lse) over the
     group's query heads and the chunk's tokens that see slot j.  acc, acc_out float32
     [B, Hkv, capacity]; entries at lens[b] and above are left alone; acc_out defaults to
-    acc (in place).  q, q_start, lens and ``lse`` are those of ``attend_chunk``."""
+    acc (in place).  q, q_start, lens and ``lse`` are those of ``attend_chunk``, whose
+    ``max_q_len`` is accepted too (this kernel has one tiling)."""
+    if max_q_len < 0:
+        raise ValueError("max_q_len must not be negative")
     _rows3(q, "q")
     B, max_pages, page_size, num_pages, Hkv = _paged(kpages, None, block_table, q_start, lens)
     T, Hq, d = q.shape
@@ -560,10 +567,14 @@ def attn_weight_sums(q: torch.Tensor, kpages: torch.Tensor, block_table: torch.T
         _need(t, n, torch.float32)
         if t.shape != (B, Hkv, max_pages * page_size):
             raise ValueError(f"{n} must be [B, Hkv, max_pages * page_size]")
-    _same_device(q, kpages, block_table, q_start, lens, lse, acc, acc_out)
+    if workspace is None:
+        workspace = torch.empty(attn_weight_sums_workspace_bytes(), dtype=torch.uint8, device=q.device)
+    _need(workspace, "workspace", workspace.dtype)
+    _same_device(q, kpages, block_table, q_start, lens, lse, acc, acc_out, workspace)
+    q = _no_broadcast(q)
     _call(q.device, "gqa_attn_weight_sums_f32", _ptr(q), q.stride(0), q.stride(1), _ptr(kpages), _ptr(block_table),
-          max_pages, page_size, num_pages, _ptr(q_start), _ptr(lens), _ptr(lse), _ptr(acc), _ptr(acc_out), B, T, Hq, Hkv,
-          d, max_q_len, default_scale(d) if scale is None else float(scale), GQA_FLAG_CAUSAL if causal else 0)
+          max_pages, page_size, num_pages, _ptr(q_start), _ptr(lens), _ptr(lse), _ptr(acc), _ptr(acc_out), _ptr(workspace),
+          workspace.numel() * workspace.element_size(), B, T, Hq, Hkv, d, default_scale(d) if scale is None else float(scale), GQA_FLAG_CAUSAL if causal else 0)
     return acc_out
 
 
@@ -733,5 +744,6 @@ def ctypes_int():
 
 __all__ = ["rope_cache", "rope", "scores", "mask", "attention_mask_words", "softmax", "pv", "prefill", "decode",
            "decode_workspace_bytes", "device_check", "default_scale", "GqaError", "rope_inv_freq", "rope_table",
-           "rope_positions", "kv_extend", "attend_chunk", "attend_chunk_workspace_bytes", "attn_weight_sums", "kv_evict",
+           "rope_positions", "kv_extend", "attend_chunk", "attend_chunk_workspace_bytes", "attn_weight_sums",
+           "attn_weight_sums_workspace_bytes", "kv_evict",
            "kv_evict_workspace_bytes"]

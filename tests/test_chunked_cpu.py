@@ -45,18 +45,20 @@ def test_attend_validates_on_the_host(lib):
 def test_weight_sums_validate_on_the_host(lib):
     def call(**kw):
         a = dict(q=FAKE, qt=1024, qh=128, kp=FAKE, table=FAKE, max_pages=4, page=16, pages=8, q_start=FAKE, lens=FAKE,
-                 lse=FAKE, acc=FAKE, acc_out=FAKE, B=2, T=3, Hq=8, Hkv=2, d=128, hint=0, scale=0.1, flags=1)
+                 lse=FAKE, acc=FAKE, acc_out=FAKE, ws=FAKE, ws_bytes=1 << 30, B=2, T=3, Hq=8, Hkv=2, d=128, scale=0.1,
+                 flags=1)
         a.update(kw)
         return lib.gqa_attn_weight_sums_f32(*a.values(), None)
 
     for bad in (dict(q=None), dict(kp=None), dict(table=None), dict(q_start=None), dict(lens=None), dict(lse=None),
-                dict(acc=None), dict(acc_out=None), dict(B=0), dict(T=-1), dict(scale=-1.0), dict(flags=4), dict(hint=-1),
-                dict(qh=-8)):
+                dict(acc=None), dict(acc_out=None), dict(B=0), dict(T=-1), dict(scale=-1.0), dict(flags=4), dict(qh=-8)):
         assert call(**bad) == E.GQA_ERR_INVALID_ARGUMENT, bad
     for bad in (dict(d=64), dict(Hq=9), dict(page=24)):
         assert call(**bad) == E.GQA_ERR_UNSUPPORTED, bad
-    for bad in (dict(q=ODD), dict(kp=ODD), dict(acc=ODD), dict(qt=4)):
+    for bad in (dict(q=ODD), dict(kp=ODD), dict(acc=ODD), dict(qt=4), dict(ws=ODD)):
         assert call(**bad) == E.GQA_ERR_MISALIGNED, bad
+    assert call(ws=None) == E.GQA_ERR_WORKSPACE
+    assert call(ws_bytes=lib.gqa_attn_weight_sums_workspace_size() - 1) == E.GQA_ERR_WORKSPACE
 
 
 def test_extend_and_rope_validate_on_the_host(lib):
