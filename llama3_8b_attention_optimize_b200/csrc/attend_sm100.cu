@@ -9,24 +9,31 @@
 // zeros and -inf.
 //
 // Unit of work: (sequence, kv head, block of query tokens); its rows are (token, head of the
-// group) pairs, packed G to a token into NT tiles of 128 rows, so K and V are read once
-// for all heads of the group and for NT * 128 / G tokens.  A unit walks its K/V tiles of
-// 128 slots with an online softmax.
+// group) pairs, so K and V are read once for all heads of the group and all tokens of
+// the block.  A unit walks its K/V tiles of 128 slots with an online softmax, O rescaled
+// only when a running maximum grows by more than 2^16.
 //
-// Split: all units' K/V tiles form one line, cut into equal parts, one per CTA and SM
-// (ragged.cuh).  A part may begin and end inside a unit; such segments leave (O, m, l) in
-// the workspace and a second kernel merges them.  So one long sequence of a single token
-// keeps every SM busy.
+// Two forms, chosen per sequence by its rows n G:
+//  many  units of 256 rows, two Q tiles of 128 with one MMA issuer each.  S = Q K^T has a
+//        row per TMEM lane; P goes to shared memory as the A operand of O += P V.
+//  few   n G <= 32 (single tokens, short drafts): transposed, S^T = K Q^T and
+//        O^T += V^T P^T with N = 16 or 32, so that the tensor core does no more work than
+//        there are rows.  Such units are bound by memory, and padding 4 rows to 128
+//        drew the GPU's whole power budget (1000 W at 1.39 GHz instead of 1.97: 64 tokens
+//        over 1024..32768 slots 813 us instead of what the header of few_rows says).
 //
-// Pipeline (per CTA): a producer warp loads Q by TMA and streams K and V tiles through a ring, one
-// box per page (or per part of a page inside a tile); one warp per Q tile issues S = Q K^T
-// and O += P V (tcgen05, accumulators in TMEM); eight softmax warps per Q tile (two
-// halves of 64 slots) turn S into P in shared memory, rescaling O only when the running
-// maximum grows by more than 2^16; a helper warp clears V rows past the last slot that the unit
-// sees (P is zero there, but a cache may hold anything, and 0 * NaN would spread).
+// Split: the units' K/V tiles form one line per form, and the CTAs (one per SM) are dealt
+// out to the two lines by what a tile of each costs; each line is cut into equal parts
+// (ragged.cuh).  A part may begin and end inside a unit; such segments leave (O, m, l) in the
+// workspace and a second kernel merges them.  So one long sequence of a single token keeps
+// every SM busy, and a prompt chunk uses the tensor cores of some SMs while the decode
+// beside it streams the cache on the others.
 //
-// Two tilings: NT = 2 (256 rows, ring of 3 tiles) where sequences bring more rows than a
-// tile holds; NT = 1 (128 rows, ring of 5) for single tokens, which are bound by memory.
+// Pipeline (per CTA): a producer warp loads Q by TMA and streams K and V tiles through a
+// ring, one box per page (or per part of a page inside a tile); issuer warps drive
+// tcgen05.mma with accumulators in TMEM; softmax warps turn S into P; a helper warp clears
+// V rows past the last slot that the unit sees (P is zero there, but a cache may hold
+// anything, and 0 * NaN would spread).
 #include <cuda.h>
 
 #include <algorithm>
@@ -60,44 +67,64 @@ constexpr int kHalf = kTileBytes / 2;      // one 64-column swizzle block of 128
 constexpr float kRescaleLog2 = 16.0f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-template <int NT>
-struct Cfg {
-  static constexpr int kStages = NT == 2 ? 3 : 5;
-  static constexpr int kSoftmaxWarps = 8 * NT;
-  static constexpr int kWarpProducer = kSoftmaxWarps;
-  static constexpr int kWarpMma = kSoftmaxWarps + 1;  // one issuer per Q tile
-  static constexpr int kWarpHelper = kSoftmaxWarps + 3;
-  static constexpr int kThreads = (kSoftmaxWarps + 4) * 32;
-  // Register split of the 640-thread tiling, as in the prefill: the sum must stay within
-  // the launch allocation (the host checks the compiled count before the first launch).
-  static constexpr bool kSplitRegs = NT == 2;
-  static constexpr int kRegsLaunch = 96, kRegsHelper = 64, kRegsSoftmax = 104;
-  static_assert(4 * 128 * kRegsSoftmax + 128 * kRegsHelper <= 640 * kRegsLaunch, "register split over budget");
-  static constexpr int kOffQ = 0;
-  static constexpr int kOffP = kOffQ + NT * kTileBytes;
-  static constexpr int kOffKV = kOffP + NT * kTileBytes;
-  static constexpr int kOffBar = kOffKV + kStages * kTileBytes;
-  static constexpr int kNumBars = 40;
-  static constexpr int kOffX = kOffBar + kNumBars * 8;  // row exchange [tile][half][128]
-  static constexpr int kOffTmemPtr = kOffX + NT * 2 * 128 * 4;
-  static constexpr int kOffStart = kOffTmemPtr + 16;  // this CTA's part: first unit, tile, count
-  static constexpr int kSmemBytes = kOffStart + 32;
-  static_assert(sizeof(Walk) <= 32, "room for the start");
-  static_assert(kSmemBytes <= 232448, "shared memory over the per-block limit");
-  static_assert(kMaxB * 8 + 64 * 8 <= kStages * kTileBytes, "the plan's scratch lies in the ring");
+constexpr int kFewRows = 32;               // rows of a unit of the few-row form
+// What one K/V tile costs in each form, for dealing out the CTAs: a tile of the few form is
+// 64 KB from memory, one of the many form two tiles' softmax.
+constexpr int kCostFew = 3, kCostMany = 5;
+// and what a unit's beginning and end cost, in tiles.
+constexpr int kExtraFew = 1, kExtraMany = 2;
+
+constexpr int kWarpProducer = 16;
+constexpr int kWarpMma = 17;  // and 18 for the second Q tile
+constexpr int kWarpHelper = 19;
+constexpr int kThreads = 640;
+// Register split (setmaxnreg): the launch gives every thread kRegsLaunch registers; the sum
+// of each form's shares must stay within the launch allocation, or setmaxnreg.inc would
+// wait forever; the host checks the compiled count before the first launch.
+constexpr int kRegsLaunch = 96, kRegsHelper = 64, kRegsMany = 104, kRegsFew = 128;
+static_assert(4 * 128 * kRegsMany + 128 * kRegsHelper <= kThreads * kRegsLaunch, "register split over budget");
+static_assert(2 * 128 * kRegsFew + 3 * 128 * kRegsHelper <= kThreads * kRegsLaunch, "register split over budget");
+
+// Shared memory; the 1024-byte-aligned tiles come first.
+struct Many {
+  static constexpr int kStages = 3;
+  static constexpr int kOffQ = 0, kQHalf = kHalf;  // [2 tiles][2 halves of 64 dims]
+  static constexpr int kOffP = 2 * kTileBytes;
+  static constexpr int kOffKV = 4 * kTileBytes;
 };
+struct Few {
+  static constexpr int kStages = 6;
+  static constexpr int kOffKV = 0;
+  static constexpr int kSmall = kFewRows * 128;  // one 64-column block of 32 rows: 4 KB
+  static constexpr int kOffQ = 6 * kTileBytes, kQHalf = kSmall;
+  static constexpr int kOffP = kOffQ + 2 * kSmall;    // [2 buffers][2 halves of 64 slots]
+  static constexpr int kOffRed = kOffP + 4 * kSmall;  // [2 warpgroups][4 warps][16] floats
+  static constexpr int kOffLim = kOffRed + 512;       // [32] token of a row
+};
+constexpr int kOffBar = 7 * kTileBytes;
+constexpr int kNumBars = 33;
+constexpr int kOffX = kOffBar + 40 * 8;  // row exchange [tile][half][128]
+constexpr int kOffTmemPtr = kOffX + 2 * 2 * 128 * 4;
+constexpr int kOffStart = kOffTmemPtr + 16;  // this CTA's place on its line
+constexpr int kOffCold = kOffStart + 32;  // [tile] what the many form's softmax needs only between segments
+constexpr int kSmemBytes = kOffCold + 2 * 64;
+static_assert(Few::kOffLim + 128 <= kOffBar, "the few form's buffers");
+static_assert(sizeof(Walk) <= 32, "room for the start");
+static_assert(kSmemBytes <= 232448, "shared memory over the per-block limit");
+static_assert(ragged::kPlanBytes <= kOffBar, "the plan's scratch lies in the tiles");
 
 enum : int {
-  B_QFULL = 0,     // [2] Q tile t of the current unit landed
+  // [2]: by Q tile in the many form, by parity of the K/V tile in the few form
+  B_QFULL = 0,     // [2] Q tile of the current unit landed (few: [0] alone)
   B_QEMPTY = 2,    // [1] last QK^T of the segment complete (one arrival per issuer)
-  B_KVFULL = 3,    // [5] K/V stage landed
-  B_KVEMPTY = 8,   // [5] MMAs reading the stage completed (issuers + helper)
-  B_SFULL = 13,    // [2] S_t = Q_t K^T complete
-  B_SFREE = 15,    // [2] S_t copied to registers
-  B_PREADY = 17,   // [2] P_t in shared memory, O_t rescaled
-  B_PVDONE = 19,   // [2] O_t += P_t V complete
-  B_VZERO = 21,    // [4] rows past the last seen slot cleared (event k in slot k % 4)
-  B_DRAIN = 25,    // [2] every MMA of issuer t complete
+  B_KVFULL = 3,    // [6] K/V stage landed
+  B_KVEMPTY = 9,   // [6] MMAs reading the stage completed (issuers + helper)
+  B_SFULL = 15,    // [2] S = Q K^T complete
+  B_SFREE = 17,    // [2] S copied to registers
+  B_PREADY = 19,   // [2] P in shared memory, O rescaled
+  B_PVDONE = 21,   // [2] O += P V complete
+  B_VZERO = 23,    // [8] rows past the last seen slot cleared (event k in slot k % 8)
+  B_DRAIN = 31,    // [2] every MMA of issuer t complete
 };
 
 enum : int {
@@ -122,7 +149,8 @@ struct Params {
   Desc* desc;      // [grid]
   long long o_t, o_h;
   int G, Hq, causal;
-  int tpt, tu;     // query tokens per tile, per unit
+  int tpt, tu;     // query tokens per tile and per unit of the many form
+  int few;         // most new tokens of a sequence of the few form, its unit
   int box;         // rows of one K/V box: the largest power of two dividing page_size, <= 128
   int part_rows;
   float scale_log2;
@@ -131,25 +159,31 @@ struct Params {
 // Units: blocks of tu query tokens.  Steps: K/V tiles over the slots [0, limit) that some
 // row of the unit sees; one at least, so that rows without any slot are written too.
 struct Line {
-  int tu, causal;
-  __device__ __forceinline__ Line(const Params& p) : tu(p.tu), causal(p.causal) {}
+  int tu, causal, from, to;  // sequences with from <= n <= to new tokens
+  int extra;
+  __device__ __forceinline__ Line(const Params& p, bool many)
+      : tu(many ? p.tu : p.few), causal(p.causal), from(many ? p.few + 1 : 1), to(many ? 0x7FFFFFFF : p.few),
+        extra(many ? kExtraMany : kExtraFew) {}
+  __device__ __forceinline__ bool has(const Seq& s) const { return s.n >= from && s.n <= to; }
   __device__ __forceinline__ int units(const Seq& s) const { return (s.n + tu - 1) / tu; }
+  __device__ __forceinline__ bool ends(const Seq& s, int u) const { return (u + 1) * tu >= s.n; }
   __device__ __forceinline__ int limit(const Seq& s, int u) const {
     return causal ? max(0, s.L - s.n + min(s.n, (u + 1) * tu)) : s.L;
   }
   __device__ __forceinline__ int count(const Seq& s, int u) const { return max(1, (limit(s, u) + kBN - 1) / kBN); }
-  __device__ __forceinline__ long long before(const Seq& s, int k) const {
+  __device__ __forceinline__ uint32_t before(const Seq& s, int k) const {
+    if (!causal) return static_cast<uint32_t>(k) * (count(s, 0) + extra);
     const int n = units(s);
-    if (!causal) return static_cast<long long>(k) * count(s, 0);
+    uint32_t sum = 0;
     const int m = min(k, n - 1);  // the last unit may be shorter
-    const long long base = s.L - s.n;
-    // units whose limit is at most one tile
-    const int one = base >= kBN ? 0 : static_cast<int>(min(static_cast<long long>(m), (kBN - base) / tu));
-    long long sum = one;
-    if (m > one)
-      sum += ragged::floor_sum(m - one, kBN, tu, base + static_cast<long long>(one + 1) * tu + kBN - 1);
+    if (m > 0) {
+      const int base = s.L - s.n;
+      const int one = base >= kBN ? 0 : min(m, (kBN - base) / tu);  // units whose limit is at most one tile
+      sum = one;
+      if (m > one) sum += ragged::floor_sum(m - one, kBN, tu, base + (one + 1) * tu + kBN - 1);
+    }
     if (k == n) sum += count(s, n - 1);
-    return sum;
+    return sum + k * extra;
   }
 };
 
@@ -160,10 +194,10 @@ struct Seg : Part {
 };
 
 __device__ __forceinline__ bool next_seg(const Params& p, Walk& w, Seg& x) {
-  const Line line(p);
+  const Line line(p, w.line != 0);
   if (!ragged::next_part(p.batch, line, w, x)) return false;
-  x.tok0 = x.u * p.tu;
-  x.n_tok = min(p.tu, x.s.n - x.tok0);
+  x.tok0 = x.u * line.tu;
+  x.n_tok = min(line.tu, x.s.n - x.tok0);
   x.base = x.s.L - x.s.n;
   x.limit = line.limit(x.s, x.u);
   return true;
@@ -199,12 +233,709 @@ __device__ __forceinline__ void exp_chunk_store(const uint32_t (&s)[32], uint8_t
   }
 }
 
-template <int NT, bool kLse>
-__global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
-    attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                  const __grid_constant__ CUtensorMap tmV, const Params p) {
-  using C = Cfg<NT>;
+// ------------------------------------------------------------------ shared roles
+// Producer warp (all lanes): per segment K0, its Q tile(s), K1 V0 K2 V1 ...; K and V through the
+// ring of C::kStages tiles.
+template <class C, int kQTiles>
+__device__ __forceinline__ void produce(const Params& p, const CUtensorMap* tmQ, const CUtensorMap* tmK,
+                                        const CUtensorMap* tmV, uint32_t sbase, Walk walk, int lane) {
   constexpr int kStages = C::kStages;
+  auto bar = [&](int i) -> uint32_t { return sbase + kOffBar + 8 * i; };
+  const int q_tokens = kQTiles == 2 ? p.tpt : p.few;  // tokens of one Q box
+  bool ok = true;
+  uint32_t L = 0;               // K/V loads issued by this CTA (ring position)
+  uint32_t n_q[kQTiles] = {};   // Q tiles loaded
+  uint32_t n_seg = 0;
+  const Boxes boxes(p.box, lane);
+  Seg s;
+  while (ok && next_seg(p, walk, s)) {
+    const int n = s.k1 - s.k0;
+    const int32_t* table = p.batch.table + static_cast<size_t>(s.b) * p.batch.max_pages;
+    int page_next = boxes.page(p.batch, table, s.k0 * kBN, s.limit);  // read one K tile ahead
+    int row_k = -1, row_v = -1;  // rows of the latest K tile and of the tile whose V comes next
+    for (int li = 0; ok && li < 2 * n; ++li) {
+      const int st = static_cast<int>(L % kStages);
+      const uint32_t r = L / kStages;
+      // li -> (tile, K or V): K one tile ahead of V
+      const bool is_v = (li == 2 * n - 1) || (li >= 2 && (li & 1) == 0);
+      int row;
+      if (is_v) {
+        row = li == 2 * n - 1 ? row_k : row_v;
+      } else {
+        const int slot0 = (s.k0 + (li == 0 ? 0 : (li + 1) >> 1)) * kBN;
+        row_v = row_k;
+        row_k = boxes.row(p.batch, page_next, s.h, slot0, s.limit, SITE_BAD_PAGE);
+        page_next = boxes.page(p.batch, table, slot0 + kBN, s.limit);
+        row = row_k;
+      }
+      if (r > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_KVEMPTY + st), (r - 1) & 1u, SITE_PRODUCER));
+      if (!ok) break;
+      const uint32_t mine = __ballot_sync(0xffffffffu, row >= 0);
+      if (lane == 0) mbar_expect_tx(bar(B_KVFULL + st), __popc(mine) * p.box * 128);
+      __syncwarp();
+      if (row >= 0)
+        tma_load_3d(sbase + C::kOffKV + st * kTileBytes + boxes.offset, is_v ? tmV : tmK, bar(B_KVFULL + st),
+                    boxes.half * 64, row, 0);
+      ++L;
+      if (li > 0) continue;
+      // The first K tile is on its way.  The Q tiles are reused once the previous segment's
+      // last QK^T is done.
+      if (n_seg > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_QEMPTY), (n_seg - 1) & 1, SITE_PRODUCER));
+      if (!ok) break;
+#pragma unroll
+      for (int t = 0; t < kQTiles; ++t) {
+        if (t * q_tokens < s.n_tok) {
+          ++n_q[t];
+          if (lane == 0) {
+            const uint32_t dst = sbase + C::kOffQ + t * kTileBytes;
+            mbar_expect_tx(bar(B_QFULL + t), 2 * 128 * p.G * q_tokens);
+            for (int e = 0; e < 2; ++e)
+              tma_load_4d(dst + e * C::kQHalf, tmQ, bar(B_QFULL + t), 64 * e, s.h * p.G, s.s.a + s.tok0 + t * q_tokens, 0);
+          }
+        }
+      }
+      ++n_seg;
+    }
+  }
+  // Drain: every load this warp issued must land before the CTA may exit.
+  for (uint32_t i = L > static_cast<uint32_t>(kStages) ? L - kStages : 0u; i < L; ++i)
+    mbar_wait_drain(bar(B_KVFULL + static_cast<int>(i % kStages)), (i / kStages) & 1u, SITE_DRAIN);
+#pragma unroll
+  for (int t = 0; t < kQTiles; ++t)
+    if (n_q[t] > 0) mbar_wait_drain(bar(B_QFULL + t), (n_q[t] - 1) & 1, SITE_DRAIN);
+  __syncwarp();
+}
+
+// Helper warp: a reader of the ring like the issuers, in step with it, that clears the rows
+// of a unit's last V tile past its last slot.
+template <class C>
+__device__ __forceinline__ void clear_tails(const Params& p, uint8_t* smem, uint32_t sbase, Walk walk, int lane) {
+  constexpr int kStages = C::kStages;
+  auto bar = [&](int i) -> uint32_t { return sbase + kOffBar + 8 * i; };
+  bool ok = true;
+  uint32_t L = 0, Z = 0;
+  Seg s;
+  while (ok && next_seg(p, walk, s)) {
+    const int n = s.k1 - s.k0;
+    for (int li = 0; ok && li < 2 * n; ++li) {
+      const int st = static_cast<int>((L + li) % kStages);
+      ok = __all_sync(0xffffffffu, mbar_wait(bar(B_KVFULL + st), ((L + li) / kStages) & 1u, SITE_HELPER));
+      if (!ok) break;
+      if (li == 2 * n - 1 && s.tail()) {
+        const int first = s.limit - (s.count - 1) * kBN;  // rows [first, 128) of the V tile
+        uint8_t* v = smem + C::kOffKV + st * kTileBytes;
+        for (int i = first * 8 + lane; i < kBN * 8; i += 32) {
+          *reinterpret_cast<uint4*>(v + i * 16) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(v + kHalf + i * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(bar(B_VZERO + Z % 8));
+        __syncwarp();
+      }
+      if (lane == 0) mbar_arrive(bar(B_KVEMPTY + st));
+    }
+    if (s.tail()) ++Z;
+    L += 2 * n;
+  }
+}
+
+// ------------------------------------------------------------------ many rows
+// MMA issuer of Q tile tq (one thread).  One per tile: a single thread starts a 128x128x16
+// MMA only every ~85 cycles, a third slower than the tensor core runs it.
+__device__ __forceinline__ void issue_many(const Params& p, uint32_t sbase, uint32_t tmem, Walk walk, int tq) {
+  using C = Many;
+  constexpr int kStages = C::kStages;
+  auto bar = [&](int i) -> uint32_t { return sbase + kOffBar + 8 * i; };
+  constexpr uint32_t kIdQK = idesc_bf16_f32(128, kBN, false);
+  constexpr uint32_t kIdPV = idesc_bf16_f32(128, kD, true);
+  constexpr uint32_t kHi = sdesc_hi_sw128(1024);
+  const uint32_t q_lo = sdesc_lo(sbase + C::kOffQ + tq * kTileBytes, 16);
+  const uint32_t p_lo = sdesc_lo(sbase + C::kOffP + tq * kTileBytes, 16);
+  const uint32_t kv_lo = sdesc_lo(sbase + C::kOffKV, 16);
+  const uint32_t v_lo = sdesc_lo(sbase + C::kOffKV, kHalf);
+  constexpr uint32_t kTile16 = kTileBytes / 16;
+  const uint32_t dS = tmem + 128 * tq, dO = tmem + 256 + 128 * tq;
+  auto issue_qk = [&](int st) {  // S_t = Q_t K^T over d = 128
+    const uint32_t b0 = kv_lo + st * kTile16;
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+      const uint32_t off = ((kk >> 2) * kHalf + (kk & 3) * 32) / 16;
+      umma_ss_lohi(dS, q_lo + off, b0 + off, kHi, kIdQK, kk > 0 ? 1u : 0u);
+    }
+  };
+  auto issue_pv = [&](int st, uint32_t acc) {  // O_t (+)= P_t V over 128 slots
+    const uint32_t b0 = v_lo + st * kTile16;
+    umma_ss_lohi(dO, p_lo, b0, kHi, kIdPV, acc);
+#pragma unroll
+    for (int kk = 1; kk < 8; ++kk) {
+      const uint32_t off = ((kk >> 2) * kHalf + (kk & 3) * 32) / 16;
+      umma_ss_lohi(dO, p_lo + off, b0 + kk * (2048 / 16), kHi, kIdPV, 1u);
+    }
+  };
+  bool ok = true;
+  uint32_t L = 0, Gb = 0, Z = 0;  // ring position, iterations of this tile, clearing events
+  uint32_t uc = 0;                // segments with this tile
+  auto wait_kv = [&](uint32_t ii) -> bool {
+    return mbar_wait_spin(bar(B_KVFULL + ii % kStages), (ii / kStages) & 1u, SITE_MMA);
+  };
+  Seg s;
+  while (ok && next_seg(p, walk, s)) {
+    const int n = s.k1 - s.k0;
+    if (tq * p.tpt >= s.n_tok) {
+      // no rows in this tile: pass the stages on, in step with the ring
+      for (int li = 0; ok && li < 2 * n; ++li) {
+        ok = wait_kv(L + li);
+        if (ok) mbar_arrive(bar(B_KVEMPTY + (L + li) % kStages));
+      }
+      if (ok) mbar_arrive(bar(B_QEMPTY));
+    } else {
+      ok = mbar_wait_spin(bar(B_QFULL + tq), uc & 1u, SITE_MMA) && wait_kv(L + load_idx_k(0)) &&
+           (Gb == 0 || mbar_wait_spin(bar(B_SFREE + tq), (Gb - 1) & 1u, SITE_MMA));
+      if (!ok) break;
+      {
+        const int sk = static_cast<int>((L + load_idx_k(0)) % kStages);
+        tc_fence_after();
+        issue_qk(sk);
+        umma_commit(bar(B_SFULL + tq));
+        umma_commit(bar(B_KVEMPTY + sk));
+        if (n == 1) umma_commit(bar(B_QEMPTY));
+      }
+      for (int j = 0; ok && j < n; ++j) {
+        const uint32_t g = Gb + j;
+        const uint32_t iv = L + load_idx_v(j, n);
+        const int sv = static_cast<int>(iv % kStages);
+        if (j + 1 < n) {
+          // next S as soon as this tile's softmax holds S(j) in registers
+          const uint32_t ik = L + load_idx_k(j + 1);
+          ok = wait_kv(ik) && mbar_wait_spin(bar(B_SFREE + tq), g & 1u, SITE_MMA);
+          if (!ok) break;
+          tc_fence_after();
+          issue_qk(static_cast<int>(ik % kStages));
+          umma_commit(bar(B_SFULL + tq));
+          umma_commit(bar(B_KVEMPTY + ik % kStages));
+          if (j + 1 == n - 1) umma_commit(bar(B_QEMPTY));
+        }
+        ok = wait_kv(iv) && mbar_wait_spin(bar(B_PREADY + tq), g & 1u, SITE_MMA);
+        if (ok && j == n - 1 && s.tail()) ok = mbar_wait_spin(bar(B_VZERO + Z % 8), (Z / 8) & 1u, SITE_MMA);
+        if (!ok) break;
+        tc_fence_after();
+        issue_pv(sv, j > 0 ? 1u : 0u);
+        umma_commit(bar(B_PVDONE + tq));
+        umma_commit(bar(B_KVEMPTY + sv));
+      }
+      Gb += n;
+      ++uc;
+    }
+    if (s.tail()) ++Z;
+    L += 2 * n;
+  }
+  umma_commit(bar(B_DRAIN + tq));
+  mbar_wait_drain(bar(B_DRAIN + tq), 0, SITE_DRAIN);
+}
+
+struct Cold {
+  Walk walk;
+  int a, tok0, n_tok, h, k0, whole;
+};
+static_assert(sizeof(Cold) <= 64, "room for it");
+
+// Softmax warps of the many form: four warpgroups, two per Q tile.
+template <bool kLse>
+__device__ __forceinline__ void softmax_many(const Params& p, uint8_t* smem, uint32_t sbase, uint32_t tmem, Walk walk,
+                                             int warp) {
+  using C = Many;
+  auto bar = [&](int i) -> uint32_t { return sbase + kOffBar + 8 * i; };
+  const int g = warp >> 2;
+  const int t = g >> 1;             // Q tile
+  const int h = g & 1;              // slots [64h, 64h+64) of each K tile; O dims [64h, 64h+64)
+  const int r = threadIdx.x & 127;  // row in tile == TMEM lane
+  const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+  const uint32_t tS = tmem + lane_off + 128 * t + 64 * h;
+  const uint32_t tO = tmem + lane_off + 256 + 128 * t + 64 * h;
+  uint8_t* ptile = smem + C::kOffP + t * kTileBytes;
+  float* xchg = reinterpret_cast<float*>(smem + kOffX) + t * 256;  // [half][row]
+  const int bar_x = 1 + t;     // named barrier: both halves of tile t (256 threads)
+  const int bar_free = 3 + t;  // named barrier: exchange slots may be rewritten
+  const float sl2 = p.scale_log2;
+  constexpr int kNoToken = 0x3FFFFFFF;
+  volatile Cold* cold = reinterpret_cast<volatile Cold*>(smem + kOffCold + 64 * t);
+  bool ok = true;
+  uint32_t Gb = 0;
+  // Every warp of the tile runs every iteration of every segment and meets every named
+  // barrier, even after a bounded wait failed (ok == false only skips the work), so
+  // the two halves of a tile can never wait on each other forever.
+  for (;;) {
+    int n, slot0, lim;
+    {
+      Seg s;
+      if (!next_seg(p, walk, s)) break;
+      if (t * p.tpt >= s.n_tok) continue;  // no rows in this tile
+      n = s.k1 - s.k0;
+      slot0 = s.k0 * kBN + 64 * h;
+      const int my_tok = r < p.tpt * p.G ? t * p.tpt + r / p.G : kNoToken;  // token in the unit
+      // last slot this row sees (a row without a token computes what nobody reads, unmasked,
+      // so that its warp takes the masked path only where a real row needs it)
+      lim = my_tok < s.n_tok ? (p.causal ? s.base + s.tok0 + my_tok : s.s.L - 1) : kNoToken;
+      // every warp of the tile writes the same values; all have read them before the
+      // first barrier of the epilogue
+      cold->walk.b = walk.b, cold->walk.h = walk.h, cold->walk.u = walk.u, cold->walk.k = walk.k;
+      cold->walk.left = walk.left;
+      cold->a = s.s.a, cold->tok0 = s.tok0, cold->n_tok = s.n_tok, cold->h = s.h, cold->k0 = s.k0;
+      cold->whole = s.whole();
+    }
+    // warps without any token's row only keep the hand-offs going
+    const bool work = __any_sync(0xffffffffu, lim != kNoToken);
+    float m_run = -INFINITY, l_run = 0.0f, lf_run = 0.0f;
+    for (int j = 0; j < n; ++j) {
+      const uint32_t gi = Gb + j;
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_SFULL + t), gi & 1u, SITE_SOFTMAX));
+      uint32_t s0[32], s1[32];
+      float mx0 = -INFINITY, mx1 = -INFINITY;
+      const int rel = lim - slot0 - j * kBN;  // columns (of this half) > rel are masked
+      if (ok && work) {
+        tc_fence_after();
+        tmem_ld32(tS + 0, s0);
+        tmem_ld32(tS + 32, s1);
+        tmem_wait_ld_dep(s0);
+        reg_dep(s1);
+        tc_fence_before();
+      }
+      if (ok) mbar_arrive(bar(B_SFREE + t));  // S_t may now be overwritten by the next QK^T
+      if (ok && work) {
+        if (rel < 63) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            if (k > rel) s0[k] = 0xFF800000u;
+            if (k + 32 > rel) s1[k] = 0xFF800000u;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+          mx0 = fmax3(mx0, __uint_as_float(s0[k]), __uint_as_float(s0[k + 1]));
+          mx1 = fmax3(mx1, __uint_as_float(s1[k]), __uint_as_float(s1[k + 1]));
+        }
+      }
+      // row max over both halves: slot [h][r] <-> [1-h][r]
+      named_bar_sync(bar_free, 256);  // everyone has read the previous exchange's slots
+      xchg[h * 128 + r] = fmaxf(mx0, mx1);
+      named_bar_sync(bar_x, 256);
+      const float m_tile = fmaxf(fmaxf(mx0, mx1), xchg[(1 - h) * 128 + r]) * sl2;
+      const float m_new = fmaxf(m_run, m_tile);
+      const bool need = m_new > m_run + kRescaleLog2;
+      const float m_use = need ? m_new : m_run;
+      const float alpha = need ? ex2_approx(m_run - m_new) : 1.0f;
+      const float moff = (m_use == -INFINITY) ? 0.0f : m_use;
+      // P_t's buffer (and O_t) are free once the previous PV finished
+      if (ok && j > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_PVDONE + t), (gi - 1) & 1u, SITE_SOFTMAX));
+      float2 sum = make_float2(0.f, 0.f), sumf = make_float2(0.f, 0.f);
+      if (ok && work) {
+        const float2 sc2 = make_float2(sl2, sl2), nm2 = make_float2(-moff, -moff);
+        // Chunks with no masked entry may evaluate part of the exponentials on the FMA
+        // pipe; its cubic is good to 7.5e-5, enough for a weight that is rounded to
+        // bf16 but not for the log-sum-exp.
+        if (rel >= 63) {
+          exp_chunk_store<!kLse, kLse>(s0, ptile, r, 8 * h, sc2, nm2, sum, sumf);
+          exp_chunk_store<!kLse, kLse>(s1, ptile, r, 8 * h + 4, sc2, nm2, sum, sumf);
+        } else {
+          exp_chunk_store<false, kLse>(s0, ptile, r, 8 * h, sc2, nm2, sum, sumf);
+          exp_chunk_store<false, kLse>(s1, ptile, r, 8 * h + 4, sc2, nm2, sum, sumf);
+        }
+        fence_proxy_async_smem();
+        if (j > 0 && __any_sync(0xffffffffu, need)) {
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            uint32_t o[32];
+            tmem_ld32(tO + 32 * c, o);
+            tmem_wait_ld_dep(o);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+            tmem_st32(tO + 32 * c, o);
+          }
+          tmem_wait_st();
+        }
+        tc_fence_before();
+      }
+      if (ok) mbar_arrive(bar(B_PREADY + t));
+      l_run = l_run * alpha + (sum.x + sum.y);
+      if (kLse) lf_run = lf_run * alpha + (sumf.x + sumf.y);
+      m_run = m_use;
+    }
+
+    // ---- epilogue
+    const uint32_t last = Gb + n - 1;
+    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_PVDONE + t), last & 1u, SITE_EPILOGUE));
+    walk.b = cold->walk.b, walk.h = cold->walk.h, walk.u = cold->walk.u, walk.k = cold->walk.k;
+    walk.left = cold->walk.left;
+    const int tok0 = cold->tok0, seq_a = cold->a, kv_head = cold->h, k0 = cold->k0;
+    const bool whole = cold->whole != 0;
+    named_bar_sync(bar_free, 256);
+    xchg[h * 128 + r] = l_run;
+    named_bar_sync(bar_x, 256);
+    const float l_tot = l_run + xchg[(1 - h) * 128 + r];
+    float lf_tot = 0.0f;
+    if (kLse) {
+      named_bar_sync(bar_free, 256);
+      xchg[h * 128 + r] = lf_run;
+      named_bar_sync(bar_x, 256);
+      lf_tot = lf_run + xchg[(1 - h) * 128 + r];
+    }
+    if (ok && work) {
+      tc_fence_after();
+      const bool mine = lim != kNoToken;
+      if (whole) {
+        const float inv_l = l_tot > 0.0f ? 1.0f / l_tot : 0.0f;
+        const long long tok = seq_a + tok0 + t * p.tpt + r / p.G;
+        const int head = kv_head * p.G + r % p.G;
+        uint16_t* dst = p.o + tok * p.o_t + head * p.o_h + 64 * h;
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+          uint32_t o[32];
+          tmem_ld32(tO + 32 * c, o);
+          tmem_wait_ld_dep(o);
+          if (mine) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint4 v;
+              v.x = pack_bf16x2(__uint_as_float(o[q * 8 + 0]) * inv_l, __uint_as_float(o[q * 8 + 1]) * inv_l);
+              v.y = pack_bf16x2(__uint_as_float(o[q * 8 + 2]) * inv_l, __uint_as_float(o[q * 8 + 3]) * inv_l);
+              v.z = pack_bf16x2(__uint_as_float(o[q * 8 + 4]) * inv_l, __uint_as_float(o[q * 8 + 5]) * inv_l);
+              v.w = pack_bf16x2(__uint_as_float(o[q * 8 + 6]) * inv_l, __uint_as_float(o[q * 8 + 7]) * inv_l);
+              *reinterpret_cast<uint4*>(dst + 32 * c + 8 * q) = v;
+            }
+          }
+        }
+        if (kLse && mine && h == 0)
+          p.lse[tok * p.Hq + head] = lf_tot > 0.0f ? (m_run + log2f(lf_tot)) * kLn2 : -INFINITY;
+      } else {
+        // a segment: (O, m, l) to this CTA's slot, 16 bytes of 32 rows side by side
+        const int slot = 2 * blockIdx.x + (k0 == 0 ? 1 : 0);
+        const int row = t * 128 + r;
+        float4* dst = p.part_o + (static_cast<size_t>(slot) * 32 + 16 * h) * p.part_rows + row;
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+          uint32_t o[32];
+          tmem_ld32(tO + 32 * c, o);
+          tmem_wait_ld_dep(o);
+          if (mine) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              dst[static_cast<size_t>(8 * c + q) * p.part_rows] =
+                  make_float4(__uint_as_float(o[4 * q]), __uint_as_float(o[4 * q + 1]), __uint_as_float(o[4 * q + 2]),
+                              __uint_as_float(o[4 * q + 3]));
+          }
+        }
+        if (mine && h == 0) {
+          float* ml = p.part_ml + static_cast<size_t>(slot) * 3 * p.part_rows + row;
+          ml[0] = m_run;
+          ml[p.part_rows] = l_tot;
+          ml[2 * p.part_rows] = lf_tot;
+        }
+      }
+      tc_fence_before();  // O_t may be overwritten by the next segment's first PV
+    }
+    Gb += n;
+  }
+}
+
+// ------------------------------------------------------------------ few rows
+// TMEM: S^T buffers at columns 0 and 32, O^T at 64; N = 16 or 32 columns of each in use.
+constexpr uint32_t kColOt = 64;
+__device__ __forceinline__ int few_cols(const Params& p, const Seg& s) { return s.n_tok * p.G <= 16 ? 16 : 32; }
+
+__device__ __forceinline__ void issue_few(const Params& p, uint32_t sbase, uint32_t tmem, Walk walk) {
+  using C = Few;
+  constexpr int kStages = C::kStages;
+  auto bar = [&](int i) -> uint32_t { return sbase + kOffBar + 8 * i; };
+  constexpr uint32_t kHi = sdesc_hi_sw128(1024);
+  const uint32_t kv_lo = sdesc_lo(sbase + C::kOffKV, 16);
+  const uint32_t vt_lo = sdesc_lo(sbase + C::kOffKV, kHalf);
+  const uint32_t q_lo = sdesc_lo(sbase + C::kOffQ, 16);
+  const uint32_t p_lo = sdesc_lo(sbase + C::kOffP, 16);
+  constexpr uint32_t kTile16 = kTileBytes / 16;
+  uint32_t id_qk = 0, id_pv = 0;
+  auto issue_qk = [&](int st, int bb) {  // S^T = K Q^T
+    const uint32_t a0 = kv_lo + st * kTile16;
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk)
+      umma_ss_lohi(tmem + 32u * bb, a0 + ((kk >> 2) * kHalf + (kk & 3) * 32) / 16,
+                   q_lo + ((kk >> 2) * C::kSmall + (kk & 3) * 32) / 16, kHi, id_qk, kk > 0 ? 1u : 0u);
+  };
+  auto issue_pv = [&](int st, int bb, uint32_t acc) {  // O^T (+)= V^T P^T
+    const uint32_t a0 = vt_lo + st * kTile16;
+    const uint32_t b0 = p_lo + bb * (2 * C::kSmall / 16);
+    umma_ss_lohi(tmem + kColOt, a0, b0, kHi, id_pv, acc);
+#pragma unroll
+    for (int kk = 1; kk < 8; ++kk)
+      umma_ss_lohi(tmem + kColOt, a0 + kk * (2048 / 16), b0 + ((kk >> 2) * C::kSmall + (kk & 3) * 32) / 16, kHi, id_pv,
+                   1u);
+  };
+  bool ok = true;
+  uint32_t L = 0, Gb = 0, Z = 0, uc = 0;
+  auto wait_kv = [&](uint32_t ii) -> bool {
+    return mbar_wait_spin(bar(B_KVFULL + ii % kStages), (ii / kStages) & 1u, SITE_MMA);
+  };
+  auto release = [&](int i) {  // the barriers count two issuers
+    umma_commit(bar(i));
+    umma_commit(bar(i));
+  };
+  auto qk = [&](uint32_t ik, uint32_t g, bool last) -> bool {
+    if (!wait_kv(ik)) return false;
+    if (g >= 2 && !mbar_wait_spin(bar(B_SFREE + (g & 1)), ((g >> 1) - 1) & 1u, SITE_MMA)) return false;
+    tc_fence_after();
+    issue_qk(static_cast<int>(ik % kStages), static_cast<int>(g & 1));
+    umma_commit(bar(B_SFULL + (g & 1)));
+    release(B_KVEMPTY + ik % kStages);
+    if (last) release(B_QEMPTY);
+    return true;
+  };
+  Seg s;
+  while (ok && next_seg(p, walk, s)) {
+    const int n = s.k1 - s.k0;
+    const int cols = few_cols(p, s);
+    id_qk = idesc_bf16_f32(128, cols, false);
+    id_pv = idesc_bf16_f32(128, cols, false) | (1u << 15);  // A (V^T) MN-major
+    ok = mbar_wait_spin(bar(B_QFULL), uc & 1u, SITE_MMA) && qk(L + load_idx_k(0), Gb, n == 1);
+    for (int j = 0; ok && j < n; ++j) {
+      const uint32_t g = Gb + j, iv = L + load_idx_v(j, n);
+      if (j + 1 < n) ok = qk(L + load_idx_k(j + 1), g + 1, j + 1 == n - 1);
+      ok = ok && wait_kv(iv) && mbar_wait_spin(bar(B_PREADY + (g & 1)), (g >> 1) & 1u, SITE_MMA);
+      if (ok && j == n - 1 && s.tail()) ok = mbar_wait_spin(bar(B_VZERO + Z % 8), (Z / 8) & 1u, SITE_MMA);
+      if (!ok) break;
+      tc_fence_after();
+      issue_pv(static_cast<int>(iv % kStages), static_cast<int>(g & 1), j > 0 ? 1u : 0u);
+      umma_commit(bar(B_PVDONE + (g & 1)));
+      release(B_KVEMPTY + iv % kStages);
+    }
+    if (s.tail()) ++Z;
+    L += 2 * n;
+    Gb += n;
+    ++uc;
+  }
+  umma_commit(bar(B_DRAIN));
+  mbar_wait_drain(bar(B_DRAIN), 0, SITE_DRAIN);
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  tmem_wait_ld_dep16(r);
+}
+
+// Whether `v` holds for any of the barrier's threads.
+__device__ __forceinline__ bool named_bar_any(int id, int nthreads, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %1, 0;\n\t"
+      "bar.red.or.pred p, %2, %3, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(v)), "r"(id), "r"(nthreads)
+      : "memory");
+  return r != 0;
+}
+
+// One segment by a softmax warpgroup (two, of 16 rows each): thread i holds slot i of each S^T
+// tile, then dim i of O^T.  The maximum of a row lies across the threads, so it is not taken per
+// tile: a tile only asks whether any score passes its row's running maximum by more than
+// 2^16 (one barrier vote), which after the first tile hardly ever happens.
+template <bool kLse>
+__device__ __forceinline__ void softmax_few(const Params& p, const Seg& s, uint8_t* smem, uint32_t sbase, uint32_t tmem,
+                                            uint32_t& Gb, bool& ok) {
+  using C = Few;
+  constexpr int N = 16;  // columns of a warpgroup
+  auto bar = [&](int i) -> uint32_t { return sbase + kOffBar + 8 * i; };
+  const int i = threadIdx.x & 127, wq = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
+  const int wg = threadIdx.x >> 7;  // rows [16 wg, 16 wg + 16)
+  const uint32_t t_lane = tmem + (static_cast<uint32_t>(wq * 32) << 16) + 16 * wg;
+  const int bar_vote = 1 + wg, bar_red = 3 + wg;
+  float* red = reinterpret_cast<float*>(smem + C::kOffRed) + 64 * wg;  // [4 warps][16]
+  const int* tok = reinterpret_cast<const int*>(smem + C::kOffLim) + 16 * wg;
+  const int n = s.k1 - s.k0;
+  if (s.n_tok * p.G <= 16 * wg) {  // no rows: only keep the hand-offs going
+    for (int j = 0; j < n; ++j) {
+      const uint32_t g = Gb + j;
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_SFULL + (g & 1)), (g >> 1) & 1u, SITE_SOFTMAX));
+      if (ok) {
+        mbar_arrive(bar(B_SFREE + (g & 1)));
+        mbar_arrive(bar(B_PREADY + (g & 1)));
+      }
+    }
+    Gb += n;
+    return;
+  }
+  const float sl2 = p.scale_log2;
+  float m[N], l[N], lf[kLse ? N : 1];
+#pragma unroll
+  for (int c = 0; c < N; ++c) {
+    m[c] = -INFINITY;
+    l[c] = 0.0f;
+    if (kLse) lf[c] = 0.0f;
+  }
+  // x[c] of all 128 threads combined: across a warp by halves (each step exchanges half of
+  // the columns left, so lanes 2c and 2c + 1 end with column c: 16 shuffles, not 80), across
+  // the warps through `red`
+  auto across = [&](float (&x)[N], bool take_max) {
+    float y[N];
+#pragma unroll
+    for (int c = 0; c < N; ++c) y[c] = x[c];
+#pragma unroll
+    for (int o = N; o >= 2; o /= 2) {
+      const bool up = (lane & o) != 0;
+#pragma unroll
+      for (int c = 0; c < o / 2; ++c) {
+        const float give = up ? y[c] : y[c + o / 2], keep = up ? y[c + o / 2] : y[c];
+        const float got = __shfl_xor_sync(0xffffffffu, give, o);
+        y[c] = take_max ? fmaxf(keep, got) : keep + got;
+      }
+    }
+    const float z = __shfl_xor_sync(0xffffffffu, y[0], 1);
+    if ((lane & 1) == 0) red[wq * N + (lane >> 1)] = take_max ? fmaxf(y[0], z) : y[0] + z;
+    named_bar_sync(bar_red, 128);
+#pragma unroll
+    for (int c = 0; c < N; c += 4) {
+      float4 v[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) v[w] = *reinterpret_cast<const float4*>(red + w * N + c);
+      x[c] = take_max ? fmaxf(fmaxf(v[0].x, v[1].x), fmaxf(v[2].x, v[3].x)) : (v[0].x + v[1].x) + (v[2].x + v[3].x);
+      x[c + 1] = take_max ? fmaxf(fmaxf(v[0].y, v[1].y), fmaxf(v[2].y, v[3].y)) : (v[0].y + v[1].y) + (v[2].y + v[3].y);
+      x[c + 2] = take_max ? fmaxf(fmaxf(v[0].z, v[1].z), fmaxf(v[2].z, v[3].z)) : (v[0].z + v[1].z) + (v[2].z + v[3].z);
+      x[c + 3] = take_max ? fmaxf(fmaxf(v[0].w, v[1].w), fmaxf(v[2].w, v[3].w)) : (v[0].w + v[1].w) + (v[2].w + v[3].w);
+    }
+  };
+  for (int j = 0; j < n; ++j) {
+    const uint32_t g = Gb + j;
+    const int bb = static_cast<int>(g & 1);
+    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_SFULL + bb), (g >> 1) & 1u, SITE_SOFTMAX));
+    uint32_t sv[N];
+    if (ok) {
+      tc_fence_after();
+      tmem_ld16(t_lane + 32 * bb, sv);
+      tc_fence_before();
+      mbar_arrive(bar(B_SFREE + bb));
+    } else {
+#pragma unroll
+      for (int c = 0; c < N; ++c) sv[c] = 0xFF800000u;
+    }
+    const int slot0 = (s.k0 + j) * kBN, key = slot0 + i;
+    if (slot0 + kBN - 1 > (p.causal ? s.base : s.s.L - 1)) {  // some row does not see all of the tile
+#pragma unroll
+      for (int c = 0; c < N; ++c)
+        if (key > (p.causal ? min(s.base + tok[c], s.s.L - 1) : s.s.L - 1)) sv[c] = 0xFF800000u;
+    }
+    float big = -INFINITY;  // -m is +inf as long as the row has seen nothing: its first score votes
+#pragma unroll
+    for (int c = 0; c < N; ++c) big = fmaxf(big, fmaf(__uint_as_float(sv[c]), sl2, -m[c]));
+    if (named_bar_any(bar_vote, 128, big > kRescaleLog2)) {
+      float x[N];
+#pragma unroll
+      for (int c = 0; c < N; ++c) x[c] = __uint_as_float(sv[c]);
+      across(x, true);
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        const float m_new = fmaxf(m[c], x[c] * sl2);
+        const bool need = m_new > m[c] + kRescaleLog2;
+        x[c] = need ? ex2_approx(m[c] - m_new) : 1.0f;
+        m[c] = need ? m_new : m[c];
+        l[c] *= x[c];
+        if (kLse) lf[c] *= x[c];
+      }
+      if (j > 0) {
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_PVDONE + (bb ^ 1)), ((g - 1) >> 1) & 1u, SITE_SOFTMAX));
+        if (ok) {
+          uint32_t o[N];
+          tc_fence_after();
+          tmem_ld16(t_lane + kColOt, o);
+#pragma unroll
+          for (int c = 0; c < N; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * x[c]);
+          tmem_st16(t_lane + kColOt, o);
+          tmem_wait_st();
+        }
+      }
+    }
+    // P's buffer is free once the PV of two tiles ago finished
+    if (ok && j >= 2) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_PVDONE + bb), ((g - 2) >> 1) & 1u, SITE_SOFTMAX));
+    if (ok) {
+      uint8_t* dst = smem + C::kOffP + bb * 2 * C::kSmall + (i >> 6) * C::kSmall + wg * 2048 + (i & 7) * 2;
+      const int chunk = (i & 63) >> 3;
+#pragma unroll
+      for (int c = 0; c < N; c += 2) {
+        const float e0 = ex2_approx(fmaf(__uint_as_float(sv[c]), sl2, m[c] == -INFINITY ? 0.0f : -m[c]));
+        const float e1 = ex2_approx(fmaf(__uint_as_float(sv[c + 1]), sl2, m[c + 1] == -INFINITY ? 0.0f : -m[c + 1]));
+        if (kLse) {
+          lf[c] += e0;
+          lf[c + 1] += e1;
+        }
+        const uint32_t w = pack_bf16x2(e0, e1);
+        l[c] += bf16_lo(w);
+        l[c + 1] += bf16_hi(w);
+        *reinterpret_cast<uint16_t*>(dst + c * 128 + ((chunk ^ (c & 7)) << 4)) = static_cast<uint16_t>(w);
+        *reinterpret_cast<uint16_t*>(dst + (c + 1) * 128 + ((chunk ^ ((c + 1) & 7)) << 4)) = static_cast<uint16_t>(w >> 16);
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      mbar_arrive(bar(B_PREADY + bb));
+    }
+  }
+  Gb += n;
+
+  // ---- epilogue.  The last PV needed every thread's P, so `red` has been read.
+  const uint32_t last = Gb - 1;
+  if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_PVDONE + (last & 1)), (last >> 1) & 1u, SITE_EPILOGUE));
+  across(l, false);
+  if constexpr (kLse) {
+    named_bar_sync(bar_vote, 128);
+    across(lf, false);
+  }
+  if (!ok) return;
+  uint32_t o[N];
+  tc_fence_after();
+  tmem_ld16(t_lane + kColOt, o);
+  tc_fence_before();  // O^T may be overwritten by the next segment's first PV
+  const int rows = s.n_tok * p.G - 16 * wg;  // of this warpgroup's columns
+  if (s.whole()) {
+    uint16_t* dst = p.o + static_cast<long long>(s.s.a + s.tok0) * p.o_t + static_cast<long long>(s.h) * p.G * p.o_h + i;
+    int t = 16 * wg / p.G, hd = 16 * wg % p.G;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      if (c < rows) {
+        const float inv = l[c] > 0.0f ? __fdividef(1.0f, l[c]) : 0.0f;
+        dst[t * p.o_t + hd * p.o_h] = static_cast<uint16_t>(pack_bf16x2(__uint_as_float(o[c]) * inv, 0.0f));
+        if (kLse && i == c)
+          p.lse[static_cast<size_t>(s.s.a + s.tok0 + t) * p.Hq + s.h * p.G + hd] =
+              lf[kLse ? c : 0] > 0.0f ? (m[c] + log2f(lf[kLse ? c : 0])) * kLn2 : -INFINITY;
+        if (++hd == p.G) {
+          hd = 0;
+          ++t;
+        }
+      }
+    }
+  } else {
+    const int slot = 2 * blockIdx.x + (s.k0 == 0 ? 1 : 0);
+    float* dst = reinterpret_cast<float*>(p.part_o + (static_cast<size_t>(slot) * 32 + (i >> 2)) * p.part_rows) + (i & 3);
+    float* ml = p.part_ml + static_cast<size_t>(slot) * 3 * p.part_rows;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      if (c < rows) {
+        dst[4 * (16 * wg + c)] = __uint_as_float(o[c]);
+        if (i == c) {
+          ml[16 * wg + c] = m[c];
+          ml[p.part_rows + 16 * wg + c] = l[c];
+          ml[2 * p.part_rows + 16 * wg + c] = kLse ? lf[kLse ? c : 0] : 0.0f;
+        }
+      }
+    }
+  }
+}
+
+template <bool kLse>
+__global__ void __launch_bounds__(kThreads, 1)
+    attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmQfew,
+                  const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Params p) {
   extern __shared__ __align__(1024) uint8_t smem[];
   if (smem_u32(smem) & 1023u) {  // uniform across the CTA: leave before any barrier
     if (threadIdx.x == 0) record_error(SITE_SMEM_ALIGN);
@@ -213,420 +944,93 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
   const uint32_t sbase = smem_u32(smem);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  auto bar = [&](int i) -> uint32_t { return sbase + C::kOffBar + 8 * i; };
+  auto bar = [&](int i) -> uint32_t { return sbase + kOffBar + 8 * i; };
 
-  if (threadIdx.x == 0) {
-    for (int t = 0; t < NT; ++t) {
-      mbar_init(bar(B_QFULL + t), 1);
-      mbar_init(bar(B_SFULL + t), 1);
-      mbar_init(bar(B_PVDONE + t), 1);
-      mbar_init(bar(B_SFREE + t), 256);
-      mbar_init(bar(B_PREADY + t), 256);
-      mbar_init(bar(B_DRAIN + t), 1);
-    }
-    mbar_init(bar(B_QEMPTY), NT);
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(bar(B_KVFULL + s), 1);
-      mbar_init(bar(B_KVEMPTY + s), NT + 1);
-    }
-    for (int k = 0; k < 4; ++k) mbar_init(bar(B_VZERO + k), 32);
-    fence_mbar_init();
-  }
-  if (warp == C::kWarpMma) {
-    tmem_alloc(sbase + C::kOffTmemPtr, 256 * NT);
+  if (warp == kWarpMma) {
+    tmem_alloc(sbase + kOffTmemPtr, 512);
     tmem_relinquish();
   }
-  if (warp == C::kWarpProducer && lane == 0) {
+  if (warp == kWarpHelper) {  // a barrier a lane
+    static_assert(kNumBars <= 64, "two a lane");
+    for (int i = lane; i < kNumBars; i += 32) {
+      int count = 1;
+      if (i == B_QEMPTY) count = 2;                          // issuers
+      if (i >= B_KVEMPTY && i < B_KVEMPTY + 6) count = 3;    // issuers and helper
+      if (i >= B_SFREE && i < B_PVDONE) count = 256;         // softmax threads of a hand-off
+      if (i >= B_VZERO && i < B_DRAIN) count = 32;
+      mbar_init(bar(i), count);
+    }
+    fence_mbar_init();
+  }
+  if (warp == kWarpProducer && lane == 0) {
     tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmQfew);
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
-
-  ragged::plan<C::kThreads>(p.batch, Line(p), reinterpret_cast<long long*>(smem + C::kOffKV),
-                            reinterpret_cast<Walk*>(smem + C::kOffStart), p.desc, SITE_Q_START, SITE_LENGTH);
+  {
+    const Line lines[2] = {Line(p, false), Line(p, true)};
+    const int cost[2] = {kCostFew, kCostMany};
+    ragged::plan<kThreads>(p.batch, lines, cost, reinterpret_cast<uint32_t*>(smem),
+                           reinterpret_cast<Walk*>(smem + kOffStart), p.desc, SITE_Q_START, SITE_LENGTH);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + C::kOffTmemPtr);
-  Walk walk = *reinterpret_cast<const Walk*>(smem + C::kOffStart);
-  auto colS = [](int t) -> uint32_t { return static_cast<uint32_t>(t * 128); };
-  auto colO = [](int t) -> uint32_t { return static_cast<uint32_t>(NT * 128 + t * 128); };
-  // The plan's scratch (generic writes) lies where TMA will write.
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + kOffTmemPtr);
+  const Walk walk = *reinterpret_cast<const Walk*>(smem + kOffStart);
+  const bool many = walk.line != 0;
+  if (!many) {
+    // Q rows that no box fills stay zero; the token of each row
+    for (int i = threadIdx.x; i < 2 * Few::kSmall / 16; i += kThreads)
+      reinterpret_cast<uint4*>(smem + Few::kOffQ)[i] = make_uint4(0, 0, 0, 0);
+    if (threadIdx.x < kFewRows) reinterpret_cast<int*>(smem + Few::kOffLim)[threadIdx.x] = threadIdx.x / p.G;
+  }
+  // Generic writes (the plan's scratch, zeros) lie where TMA will write.
   fence_proxy_async_smem();
   __syncthreads();
 
-  if (warp == C::kWarpProducer) {
-    // ------------------------------------------------------------ TMA producer (whole warp)
-    if constexpr (C::kSplitRegs) regs_dec<C::kRegsHelper>();
-    bool ok = true;
-    uint32_t L = 0;               // K/V loads issued by this CTA (ring position)
-    uint32_t n_q[2] = {0, 0};     // Q tiles loaded
-    uint32_t n_seg = 0;
-    const Boxes boxes(p.box, lane);
+  if (warp >= kWarpProducer) {
+    regs_dec<kRegsHelper>();
+    if (warp == kWarpProducer) {
+      if (many)
+        produce<Many, 2>(p, &tmQ, &tmK, &tmV, sbase, walk, lane);
+      else
+        produce<Few, 1>(p, &tmQfew, &tmK, &tmV, sbase, walk, lane);
+    } else if (warp == kWarpHelper) {
+      if (many)
+        clear_tails<Many>(p, smem, sbase, walk, lane);
+      else
+        clear_tails<Few>(p, smem, sbase, walk, lane);
+    } else {
+      if (lane == 0) {
+        if (many)
+          issue_many(p, sbase, tmem, walk, warp - kWarpMma);
+        else if (warp == kWarpMma)
+          issue_few(p, sbase, tmem, walk);
+      }
+      __syncwarp();
+    }
+  } else if (many) {
+    regs_inc<kRegsMany>();
+    softmax_many<kLse>(p, smem, sbase, tmem, walk, warp);
+  } else if (warp < 8) {
+    regs_inc<kRegsFew>();
+    Walk w = walk;
     Seg s;
-    while (ok && next_seg(p, walk, s)) {
-      // Q tiles are reused once the previous segment's last QK^T is done
-      if (n_seg > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_QEMPTY), (n_seg - 1) & 1, SITE_PRODUCER));
-      if (!ok) break;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        if (t * p.tpt < s.n_tok) {
-          ++n_q[t];
-          if (lane == 0) {
-            const uint32_t dst = sbase + C::kOffQ + t * kTileBytes;
-            mbar_expect_tx(bar(B_QFULL + t), 2 * 128 * p.G * p.tpt);
-            for (int e = 0; e < 2; ++e)
-              tma_load_4d(dst + e * kHalf, &tmQ, bar(B_QFULL + t), 64 * e, s.h * p.G, s.s.a + s.tok0 + t * p.tpt, 0);
-          }
-        }
-      }
-      ++n_seg;
-      const int n = s.k1 - s.k0;
-      const int32_t* table = p.batch.table + static_cast<size_t>(s.b) * p.batch.max_pages;
-      int page_next = boxes.page(p.batch, table, s.k0 * kBN, s.limit);  // read one K tile ahead
-      int row_k = -1, row_v = -1;  // rows of the latest K tile and of the tile whose V comes next
-      for (int li = 0; ok && li < 2 * n; ++li) {
-        const int st = static_cast<int>(L % kStages);
-        const uint32_t r = L / kStages;
-        // li -> (tile, K or V): K one tile ahead of V
-        const bool is_v = (li == 2 * n - 1) || (li >= 2 && (li & 1) == 0);
-        int row;
-        if (is_v) {
-          row = li == 2 * n - 1 ? row_k : row_v;
-        } else {
-          const int slot0 = (s.k0 + (li == 0 ? 0 : (li + 1) >> 1)) * kBN;
-          row_v = row_k;
-          row_k = boxes.row(p.batch, page_next, s.h, slot0, s.limit, SITE_BAD_PAGE);
-          page_next = boxes.page(p.batch, table, slot0 + kBN, s.limit);
-          row = row_k;
-        }
-        if (r > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_KVEMPTY + st), (r - 1) & 1u, SITE_PRODUCER));
-        if (!ok) break;
-        const uint32_t mine = __ballot_sync(0xffffffffu, row >= 0);
-        if (lane == 0) mbar_expect_tx(bar(B_KVFULL + st), __popc(mine) * p.box * 128);
-        __syncwarp();
-        if (row >= 0)
-          tma_load_3d(sbase + C::kOffKV + st * kTileBytes + boxes.offset, is_v ? &tmV : &tmK, bar(B_KVFULL + st),
-                      boxes.half * 64, row, 0);
-        ++L;
-      }
-    }
-    // Drain: every load this warp issued must land before the CTA may exit.
-    for (uint32_t i = L > static_cast<uint32_t>(kStages) ? L - kStages : 0u; i < L; ++i)
-      mbar_wait_drain(bar(B_KVFULL + static_cast<int>(i % kStages)), (i / kStages) & 1u, SITE_DRAIN);
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-      if (n_q[t] > 0) mbar_wait_drain(bar(B_QFULL + t), (n_q[t] - 1) & 1, SITE_DRAIN);
-    __syncwarp();
-  } else if (warp >= C::kWarpMma && warp < C::kWarpMma + NT) {
-    // ------------------------------------------------------------ MMA issuers
-    // One per Q tile: a single thread starts a 128x128x16 MMA only every ~85 cycles, a
-    // third slower than the tensor core runs it.
-    if constexpr (C::kSplitRegs) regs_dec<C::kRegsHelper>();
-    const int tq = warp - C::kWarpMma;
-    if (lane == 0) {
-      constexpr uint32_t kIdQK = idesc_bf16_f32(128, kBN, false);
-      constexpr uint32_t kIdPV = idesc_bf16_f32(128, kD, true);
-      constexpr uint32_t kHi = sdesc_hi_sw128(1024);
-      const uint32_t q_lo = sdesc_lo(sbase + C::kOffQ + tq * kTileBytes, 16);
-      const uint32_t p_lo = sdesc_lo(sbase + C::kOffP + tq * kTileBytes, 16);
-      const uint32_t kv_lo = sdesc_lo(sbase + C::kOffKV, 16);
-      const uint32_t v_lo = sdesc_lo(sbase + C::kOffKV, kHalf);
-      constexpr uint32_t kTile16 = kTileBytes / 16;
-      const uint32_t dS = tmem + colS(tq), dO = tmem + colO(tq);
-      auto issue_qk = [&](int st) {  // S_t = Q_t K^T over d = 128
-        const uint32_t b0 = kv_lo + st * kTile16;
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          const uint32_t off = ((kk >> 2) * kHalf + (kk & 3) * 32) / 16;
-          umma_ss_lohi(dS, q_lo + off, b0 + off, kHi, kIdQK, kk > 0 ? 1u : 0u);
-        }
-      };
-      auto issue_pv = [&](int st, uint32_t acc) {  // O_t (+)= P_t V over 128 slots
-        const uint32_t b0 = v_lo + st * kTile16;
-        umma_ss_lohi(dO, p_lo, b0, kHi, kIdPV, acc);
-#pragma unroll
-        for (int kk = 1; kk < 8; ++kk) {
-          const uint32_t off = ((kk >> 2) * kHalf + (kk & 3) * 32) / 16;
-          umma_ss_lohi(dO, p_lo + off, b0 + kk * (2048 / 16), kHi, kIdPV, 1u);
-        }
-      };
-      bool ok = true;
-      uint32_t L = 0, Gb = 0, Z = 0;  // ring position, iterations of this tile, clearing events
-      uint32_t uc = 0;                // segments with this tile
-      Seg s;
-      while (ok && next_seg(p, walk, s)) {
-        const int n = s.k1 - s.k0;
-        auto wait_kv = [&](uint32_t ii) -> bool {
-          return mbar_wait_spin(bar(B_KVFULL + ii % kStages), (ii / kStages) & 1u, SITE_MMA);
-        };
-        if (tq * p.tpt >= s.n_tok) {
-          // no rows in this tile: pass the stages on, in step with the ring
-          for (int li = 0; ok && li < 2 * n; ++li) {
-            ok = wait_kv(L + li);
-            if (ok) mbar_arrive(bar(B_KVEMPTY + (L + li) % kStages));
-          }
-          if (ok) mbar_arrive(bar(B_QEMPTY));
-        } else {
-          ok = mbar_wait_spin(bar(B_QFULL + tq), uc & 1u, SITE_MMA) && wait_kv(L + load_idx_k(0)) &&
-               (Gb == 0 || mbar_wait_spin(bar(B_SFREE + tq), (Gb - 1) & 1u, SITE_MMA));
-          if (!ok) break;
-          {
-            const int sk = static_cast<int>((L + load_idx_k(0)) % kStages);
-            tc_fence_after();
-            issue_qk(sk);
-            umma_commit(bar(B_SFULL + tq));
-            umma_commit(bar(B_KVEMPTY + sk));
-            if (n == 1) umma_commit(bar(B_QEMPTY));
-          }
-          for (int j = 0; ok && j < n; ++j) {
-            const uint32_t g = Gb + j;
-            const uint32_t iv = L + load_idx_v(j, n);
-            const int sv = static_cast<int>(iv % kStages);
-            if (j + 1 < n) {
-              // next S as soon as this tile's softmax holds S(j) in registers
-              const uint32_t ik = L + load_idx_k(j + 1);
-              ok = wait_kv(ik) && mbar_wait_spin(bar(B_SFREE + tq), g & 1u, SITE_MMA);
-              if (!ok) break;
-              tc_fence_after();
-              issue_qk(static_cast<int>(ik % kStages));
-              umma_commit(bar(B_SFULL + tq));
-              umma_commit(bar(B_KVEMPTY + ik % kStages));
-              if (j + 1 == n - 1) umma_commit(bar(B_QEMPTY));
-            }
-            ok = wait_kv(iv) && mbar_wait_spin(bar(B_PREADY + tq), g & 1u, SITE_MMA);
-            if (ok && j == n - 1 && s.tail()) ok = mbar_wait_spin(bar(B_VZERO + Z % 4), (Z / 4) & 1u, SITE_MMA);
-            if (!ok) break;
-            tc_fence_after();
-            issue_pv(sv, j > 0 ? 1u : 0u);
-            umma_commit(bar(B_PVDONE + tq));
-            umma_commit(bar(B_KVEMPTY + sv));
-          }
-          Gb += n;
-          ++uc;
-        }
-        if (s.tail()) ++Z;
-        L += 2 * n;
-      }
-      umma_commit(bar(B_DRAIN + tq));
-      mbar_wait_drain(bar(B_DRAIN + tq), 0, SITE_DRAIN);
-    }
-    __syncwarp();
-  } else if (warp == C::kWarpHelper) {
-    // ------------------------------------------------------------ V rows past the last slot
-    if constexpr (C::kSplitRegs) regs_dec<C::kRegsHelper>();
-    bool ok = true;
-    uint32_t L = 0, Z = 0;
-    Seg s;
-    while (ok && next_seg(p, walk, s)) {
-      const int n = s.k1 - s.k0;
-      for (int li = 0; ok && li < 2 * n; ++li) {  // a reader like the issuers, in step with the ring
-        const int st = static_cast<int>((L + li) % kStages);
-        ok = __all_sync(0xffffffffu, mbar_wait(bar(B_KVFULL + st), ((L + li) / kStages) & 1u, SITE_HELPER));
-        if (!ok) break;
-        if (li == 2 * n - 1 && s.tail()) {
-          const int first = s.limit - (s.count - 1) * kBN;  // rows [first, 128) of the V tile
-          uint8_t* v = smem + C::kOffKV + st * kTileBytes;
-          for (int i = first * 8 + lane; i < kBN * 8; i += 32) {
-            *reinterpret_cast<uint4*>(v + i * 16) = make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4*>(v + kHalf + i * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-          mbar_arrive(bar(B_VZERO + Z % 4));
-          __syncwarp();
-        }
-        if (lane == 0) mbar_arrive(bar(B_KVEMPTY + st));
-      }
-      if (s.tail()) ++Z;
-      L += 2 * n;
-    }
-  } else if (warp < C::kSoftmaxWarps) {
-    // ------------------------------------------------------------ softmax warpgroups
-    if constexpr (C::kSplitRegs) regs_inc<C::kRegsSoftmax>();
-    const int g = warp >> 2;
-    const int t = g >> 1;             // Q tile
-    const int h = g & 1;              // slots [64h, 64h+64) of each K tile; O dims [64h, 64h+64)
-    const int r = threadIdx.x & 127;  // row in tile == TMEM lane
-    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + lane_off + colS(t) + 64 * h;
-    const uint32_t tO = tmem + lane_off + colO(t) + 64 * h;
-    uint8_t* ptile = smem + C::kOffP + t * kTileBytes;
-    float* xchg = reinterpret_cast<float*>(smem + C::kOffX) + t * 256;  // [half][row]
-    const int bar_x = 1 + t;     // named barrier: both halves of tile t (256 threads)
-    const int bar_free = 3 + t;  // named barrier: exchange slots may be rewritten
-    const float sl2 = p.scale_log2;
-    const int my_tok = r < p.tpt * p.G ? t * p.tpt + r / p.G : 0x3FFFFFFF;  // token in the unit
     bool ok = true;
     uint32_t Gb = 0;
-    Seg s;
-    // Every warp of the tile runs every iteration of every segment and meets every named
-    // barrier, even after a bounded wait failed (ok == false only skips the work), so
-    // the two halves of a tile can never wait on each other forever.
-    while (next_seg(p, walk, s)) {
-      if (t * p.tpt >= s.n_tok) continue;  // no rows in this tile
-      const int n = s.k1 - s.k0;
-      // last slot this row sees (a row without a token computes what nobody reads, unmasked,
-      // so that its warp takes the masked path only where a real row needs it)
-      const int lim = my_tok < s.n_tok ? (p.causal ? s.base + s.tok0 + my_tok : s.s.L - 1) : 0x3FFFFFFF;
-      // warps without any token's row only keep the hand-offs going
-      const bool work = __any_sync(0xffffffffu, my_tok < s.n_tok);
-      float m_run = -INFINITY, l_run = 0.0f, lf_run = 0.0f;
-      for (int j = 0; j < n; ++j) {
-        const uint32_t gi = Gb + j;
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_SFULL + t), gi & 1u, SITE_SOFTMAX));
-        uint32_t s0[32], s1[32];
-        float mx0 = -INFINITY, mx1 = -INFINITY;
-        const int rel = lim - (s.k0 + j) * kBN - 64 * h;  // columns (of this half) > rel are masked
-        if (ok && work) {
-          tc_fence_after();
-          tmem_ld32(tS + 0, s0);
-          tmem_ld32(tS + 32, s1);
-          tmem_wait_ld_dep(s0);
-          reg_dep(s1);
-          tc_fence_before();
-        }
-        if (ok) mbar_arrive(bar(B_SFREE + t));  // S_t may now be overwritten by the next QK^T
-        if (ok && work) {
-          if (rel < 63) {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              if (k > rel) s0[k] = 0xFF800000u;
-              if (k + 32 > rel) s1[k] = 0xFF800000u;
-            }
-          }
-#pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            mx0 = fmax3(mx0, __uint_as_float(s0[k]), __uint_as_float(s0[k + 1]));
-            mx1 = fmax3(mx1, __uint_as_float(s1[k]), __uint_as_float(s1[k + 1]));
-          }
-        }
-        // row max over both halves: slot [h][r] <-> [1-h][r]
-        named_bar_sync(bar_free, 256);  // everyone has read the previous exchange's slots
-        xchg[h * 128 + r] = fmaxf(mx0, mx1);
-        named_bar_sync(bar_x, 256);
-        const float m_tile = fmaxf(fmaxf(mx0, mx1), xchg[(1 - h) * 128 + r]) * sl2;
-        const float m_new = fmaxf(m_run, m_tile);
-        const bool need = m_new > m_run + kRescaleLog2;
-        const float m_use = need ? m_new : m_run;
-        const float alpha = need ? ex2_approx(m_run - m_new) : 1.0f;
-        const float moff = (m_use == -INFINITY) ? 0.0f : m_use;
-        // P_t's buffer (and O_t) are free once the previous PV finished
-        if (ok && j > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_PVDONE + t), (gi - 1) & 1u, SITE_SOFTMAX));
-        float2 sum = make_float2(0.f, 0.f), sumf = make_float2(0.f, 0.f);
-        if (ok && work) {
-          const float2 sc2 = make_float2(sl2, sl2), nm2 = make_float2(-moff, -moff);
-          // Chunks with no masked entry may evaluate part of the exponentials on the FMA
-          // pipe; its cubic is good to 7.5e-5, enough for a weight that is rounded to
-          // bf16 but not for the log-sum-exp.
-          if (rel >= 63) {
-            exp_chunk_store<!kLse, kLse>(s0, ptile, r, 8 * h, sc2, nm2, sum, sumf);
-            exp_chunk_store<!kLse, kLse>(s1, ptile, r, 8 * h + 4, sc2, nm2, sum, sumf);
-          } else {
-            exp_chunk_store<false, kLse>(s0, ptile, r, 8 * h, sc2, nm2, sum, sumf);
-            exp_chunk_store<false, kLse>(s1, ptile, r, 8 * h + 4, sc2, nm2, sum, sumf);
-          }
-          fence_proxy_async_smem();
-          if (j > 0 && __any_sync(0xffffffffu, need)) {
-            tc_fence_after();
-#pragma unroll 1
-            for (int c = 0; c < 2; ++c) {
-              uint32_t o[32];
-              tmem_ld32(tO + 32 * c, o);
-              tmem_wait_ld_dep(o);
-#pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-              tmem_st32(tO + 32 * c, o);
-            }
-            tmem_wait_st();
-          }
-          tc_fence_before();
-        }
-        if (ok) mbar_arrive(bar(B_PREADY + t));
-        l_run = l_run * alpha + (sum.x + sum.y);
-        if (kLse) lf_run = lf_run * alpha + (sumf.x + sumf.y);
-        m_run = m_use;
-      }
-
-      // ---- epilogue
-      const uint32_t last = Gb + n - 1;
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_PVDONE + t), last & 1u, SITE_EPILOGUE));
-      named_bar_sync(bar_free, 256);
-      xchg[h * 128 + r] = l_run;
-      named_bar_sync(bar_x, 256);
-      const float l_tot = l_run + xchg[(1 - h) * 128 + r];
-      float lf_tot = 0.0f;
-      if (kLse) {
-        named_bar_sync(bar_free, 256);
-        xchg[h * 128 + r] = lf_run;
-        named_bar_sync(bar_x, 256);
-        lf_tot = lf_run + xchg[(1 - h) * 128 + r];
-      }
-      if (ok && work) {
-        tc_fence_after();
-        const bool mine = my_tok < s.n_tok;
-        const bool whole = s.whole();
-        const int hd = r % p.G;
-        if (whole) {
-          const float inv_l = l_tot > 0.0f ? 1.0f / l_tot : 0.0f;
-          const long long tok = s.s.a + s.tok0 + my_tok;
-          const int head = s.h * p.G + hd;
-          uint16_t* dst = p.o + tok * p.o_t + head * p.o_h + 64 * h;
-#pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
-            uint32_t o[32];
-            tmem_ld32(tO + 32 * c, o);
-            tmem_wait_ld_dep(o);
-            if (mine) {
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                uint4 v;
-                v.x = pack_bf16x2(__uint_as_float(o[q * 8 + 0]) * inv_l, __uint_as_float(o[q * 8 + 1]) * inv_l);
-                v.y = pack_bf16x2(__uint_as_float(o[q * 8 + 2]) * inv_l, __uint_as_float(o[q * 8 + 3]) * inv_l);
-                v.z = pack_bf16x2(__uint_as_float(o[q * 8 + 4]) * inv_l, __uint_as_float(o[q * 8 + 5]) * inv_l);
-                v.w = pack_bf16x2(__uint_as_float(o[q * 8 + 6]) * inv_l, __uint_as_float(o[q * 8 + 7]) * inv_l);
-                *reinterpret_cast<uint4*>(dst + 32 * c + 8 * q) = v;
-              }
-            }
-          }
-          if (kLse && mine && h == 0)
-            p.lse[tok * p.Hq + head] = lf_tot > 0.0f ? (m_run + log2f(lf_tot)) * kLn2 : -INFINITY;
-        } else {
-          // a segment: (O, m, l) to this CTA's slot, 16 bytes of 32 rows side by side
-          const int slot = 2 * blockIdx.x + (s.k0 == 0 ? 1 : 0);
-          const int row = t * 128 + r;
-          float4* dst = p.part_o + (static_cast<size_t>(slot) * 32 + 16 * h) * p.part_rows + row;
-#pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
-            uint32_t o[32];
-            tmem_ld32(tO + 32 * c, o);
-            tmem_wait_ld_dep(o);
-            if (mine) {
-#pragma unroll
-              for (int q = 0; q < 8; ++q)
-                dst[static_cast<size_t>(8 * c + q) * p.part_rows] =
-                    make_float4(__uint_as_float(o[4 * q]), __uint_as_float(o[4 * q + 1]), __uint_as_float(o[4 * q + 2]),
-                                __uint_as_float(o[4 * q + 3]));
-            }
-          }
-          if (mine && h == 0) {
-            float* ml = p.part_ml + static_cast<size_t>(slot) * 3 * p.part_rows + row;
-            ml[0] = m_run;
-            ml[p.part_rows] = l_tot;
-            ml[2 * p.part_rows] = lf_tot;
-          }
-        }
-        tc_fence_before();  // O_t may be overwritten by the next segment's first PV
-      }
-      Gb += n;
-    }
+    while (next_seg(p, w, s)) softmax_few<kLse>(p, s, smem, sbase, tmem, Gb, ok);
+  } else {
+    regs_dec<kRegsHelper>();
   }
 
   // ---- teardown: everyone done with TMEM and shared memory
   tc_fence_before();
   __syncthreads();
-  if (warp == C::kWarpMma) {
+  if (warp == kWarpMma) {
     tc_fence_after();
-    tmem_dealloc(tmem, 256 * NT);
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -634,13 +1038,15 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
 // O = sum_i O_i 2^(m_i - M) / sum_i l_i 2^(m_i - M), segments in order.  A thread holds
 // eight dims of one row: 32 lanes read 32 rows' 16 bytes side by side.
 constexpr int kMergeThreads = 128;
-__global__ void __launch_bounds__(kMergeThreads) merge_kernel(const Params p, int nt) {
+constexpr int kBatch = 4;
+__global__ void __launch_bounds__(kMergeThreads) merge_kernel(const Params p) {
   cudaGridDependencySynchronize();
   const int c0 = blockIdx.x;
   const Desc d = p.desc[c0];
   if (!d.valid) return;
-  const Seq s = seq_of(p.batch, d.b);
-  const int n_tok = min(p.tu, s.n - d.u * p.tu);
+  const Seq& s = d.s;
+  const int tu = s.n <= p.few ? p.few : p.tu;
+  const int n_tok = min(tu, s.n - d.u * tu);
   const int rows_tile = p.tpt * p.G;
   const int rows = n_tok > p.tpt ? 128 + (n_tok - p.tpt) * p.G : n_tok * p.G;
   const int lane = threadIdx.x & 31;
@@ -650,27 +1056,46 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const Params p, in
     const int row = (it >> 4) * 32 + lane, d8 = it & 15;
     const int t = row >> 7, r = row & 127;
     if (row >= rows || r >= rows_tile) continue;
-    auto ml_of = [&](int c, int k) {
-      const size_t slot = 2 * static_cast<size_t>(c) + (c == c0 ? 1 : 0);
-      return p.part_ml[(slot * 3 + k) * p.part_rows + row];
-    };
-    float M = -INFINITY;
-    for (int c = c0; c <= d.last; ++c) M = fmaxf(M, ml_of(c, 0));
-    float l = 0.0f, lf = 0.0f, acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll 2
-    for (int c = c0; c <= d.last; ++c) {
-      const float m = ml_of(c, 0);
-      const float w = m == -INFINITY ? 0.0f : ex2_approx(m - M);
-      l += ml_of(c, 1) * w;
-      if (p.lse) lf += ml_of(c, 2) * w;
-      const size_t slot = 2 * static_cast<size_t>(c) + (c == c0 ? 1 : 0);
-      const float4* o = p.part_o + (slot * 32 + 2 * d8) * p.part_rows + row;
-      const float4 a = o[0], b = o[p.part_rows];
-      acc[0] += a.x * w, acc[1] += a.y * w, acc[2] += a.z * w, acc[3] += a.w * w;
-      acc[4] += b.x * w, acc[5] += b.y * w, acc[6] += b.z * w, acc[7] += b.w * w;
+    float M = -INFINITY, l = 0.0f, lf = 0.0f, acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    // kBatch segments at a time, so that their loads' latencies overlap
+    for (int c = c0; c <= d.last; c += kBatch) {
+      float m[kBatch], li[kBatch], lfi[kBatch];
+      float4 a[kBatch], b[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        m[i] = -INFINITY, li[i] = lfi[i] = 0.0f;
+        a[i] = b[i] = make_float4(0, 0, 0, 0);
+        if (c + i <= d.last) {
+          const size_t slot = 2 * static_cast<size_t>(c + i) + (c + i == c0 ? 1 : 0);
+          const float* ml = p.part_ml + slot * 3 * p.part_rows + row;
+          const float4* o = p.part_o + (slot * 32 + 2 * d8) * p.part_rows + row;
+          m[i] = ml[0];
+          li[i] = ml[p.part_rows];
+          if (p.lse) lfi[i] = ml[2 * p.part_rows];
+          a[i] = o[0];
+          b[i] = o[p.part_rows];
+        }
+      }
+      float top = M;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) top = fmaxf(top, m[i]);
+      const float keep = M == -INFINITY ? 0.0f : ex2_approx(M - top);
+      l *= keep;
+      lf *= keep;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) acc[k] *= keep;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const float w = m[i] == -INFINITY ? 0.0f : ex2_approx(m[i] - top);
+        l += li[i] * w;
+        lf += lfi[i] * w;
+        acc[0] += a[i].x * w, acc[1] += a[i].y * w, acc[2] += a[i].z * w, acc[3] += a[i].w * w;
+        acc[4] += b[i].x * w, acc[5] += b[i].y * w, acc[6] += b[i].z * w, acc[7] += b[i].w * w;
+      }
+      M = top;
     }
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    const long long tok = s.a + d.u * p.tu + t * p.tpt + r / p.G;
+    const long long tok = s.a + d.u * tu + t * p.tpt + r / p.G;
     const int head = d.h * p.G + r % p.G;
     *reinterpret_cast<uint4*>(p.o + tok * p.o_t + head * p.o_h + 8 * d8) =
         make_uint4(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv),
@@ -697,24 +1122,21 @@ inline Layout layout_of(int T, int G) {
   return w;
 }
 
-template <int NT, bool kLse>
-int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const Params& p, int grid,
-           cudaStream_t stream) {
-  using C = Cfg<NT>;
-  auto* kernel = attend_kernel<NT, kLse>;
+template <bool kLse>
+int launch(const CUtensorMap& q, const CUtensorMap& q_few, const CUtensorMap& k, const CUtensorMap& v, const Params& p,
+           int grid, cudaStream_t stream) {
+  auto* kernel = attend_kernel<kLse>;
   static std::atomic<uint64_t> attr_done{0};
   int rc;
-  if ((rc = ensure_smem_attr(kernel, C::kSmemBytes, attr_done)) != GQA_OK) return rc;
-  if constexpr (C::kSplitRegs) {  // the register split assumes the compiled count
-    static std::atomic<int> regs_ok{0};
-    if (regs_ok.load(std::memory_order_acquire) == 0) {
-      cudaFuncAttributes fa;
-      if (cudaFuncGetAttributes(&fa, kernel) != cudaSuccess) return GQA_ERR_CUDA;
-      regs_ok.store(fa.numRegs == C::kRegsLaunch ? 1 : -1, std::memory_order_release);
-    }
-    if (regs_ok.load(std::memory_order_acquire) < 0) return GQA_ERR_UNSUPPORTED;
+  if ((rc = ensure_smem_attr(kernel, kSmemBytes, attr_done)) != GQA_OK) return rc;
+  static std::atomic<int> regs_ok{0};  // the register split assumes the compiled count
+  if (regs_ok.load(std::memory_order_acquire) == 0) {
+    cudaFuncAttributes fa;
+    if (cudaFuncGetAttributes(&fa, kernel) != cudaSuccess) return GQA_ERR_CUDA;
+    regs_ok.store(fa.numRegs == kRegsLaunch ? 1 : -1, std::memory_order_release);
   }
-  kernel<<<grid, C::kThreads, C::kSmemBytes, stream>>>(q, k, v, p);
+  if (regs_ok.load(std::memory_order_acquire) < 0) return GQA_ERR_UNSUPPORTED;
+  kernel<<<grid, kThreads, kSmemBytes, stream>>>(q, q_few, k, v, p);
   return cudaGetLastError() == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }
 
@@ -756,6 +1178,9 @@ extern "C" int gqa_attend_chunk_bf16(const void* q, long long q_token_stride, lo
   const long long capacity = static_cast<long long>(max_pages_per_seq) * page_size;
   const long long pool_rows = static_cast<long long>(num_pages) * Hkv * page_size;
   if (G > 128 || B > kMaxB || capacity > 0x7FFFFF00LL || pool_rows > 0x7FFFFFFFLL) return GQA_ERR_UNSUPPORTED;
+  // K/V tiles over all units: counted in 32 bits
+  const long long units = (T + 2 * (128 / G) - 1) / (2 * (128 / G)) + std::min(B, T);
+  if (static_cast<double>(units) * Hkv * (capacity / kBN + 1 + kExtraMany) >= 2147483648.0) return GQA_ERR_UNSUPPORTED;
   // a TMA dimension needs a stride: heads or tokens that share one row are the caller's to expand
   if ((T > 1 && q_token_stride == 0) || (Hq > 1 && q_head_stride == 0)) return GQA_ERR_UNSUPPORTED;
   const Layout w = layout_of(T, G);
@@ -777,16 +1202,16 @@ extern "C" int gqa_attend_chunk_bf16(const void* q, long long q_token_stride, lo
   p.scale_log2 = scale * 1.4426950408889634f;
   p.box = std::min(128, page_size & -page_size);
   p.tpt = 128 / G;
-  const int longest = max_q_len > 0 ? std::min(max_q_len, T) : T;
-  const int nt = longest <= p.tpt ? 1 : 2;
-  p.tu = nt * p.tpt;
+  p.tu = 2 * p.tpt;
+  p.few = kFewRows / G;
 
-  CUtensorMap tmQ, tmK, tmV;
+  CUtensorMap tmQ, tmQfew, tmK, tmV;
   int rc;
   const long long ht = Hq > 1 ? q_head_stride : kD, tt = T > 1 ? q_token_stride : static_cast<long long>(Hq) * kD;
   const long long qd[4] = {kD, Hq, T, 1}, qs[3] = {ht * 2, tt * 2, tt * 2};
-  const int qb[4] = {64, G, p.tpt, 1};
+  const int qb[4] = {64, G, p.tpt, 1}, qf[4] = {64, G, std::max(p.few, 1), 1};
   if ((rc = make_tmap_4d(&tmQ, q, 2, qd, qs, qb)) != GQA_OK) return rc;
+  if ((rc = make_tmap_4d(&tmQfew, q, 2, qd, qs, qf)) != GQA_OK) return rc;
   if ((rc = make_tmap_3d_bf16(&tmK, kpages, kD, pool_rows, 1, 64, p.box, 1)) != GQA_OK) return rc;
   if ((rc = make_tmap_3d_bf16(&tmV, vpages, kD, pool_rows, 1, 64, p.box, 1)) != GQA_OK) return rc;
 
@@ -794,13 +1219,11 @@ extern "C" int gqa_attend_chunk_bf16(const void* q, long long q_token_stride, lo
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   const int grid = std::min(sms, kMaxCtas);
-  if (nt == 1)
-    rc = lse ? launch<1, true>(tmQ, tmK, tmV, p, grid, stream) : launch<1, false>(tmQ, tmK, tmV, p, grid, stream);
-  else
-    rc = lse ? launch<2, true>(tmQ, tmK, tmV, p, grid, stream) : launch<2, false>(tmQ, tmK, tmV, p, grid, stream);
+  rc = lse ? launch<true>(tmQ, tmQfew, tmK, tmV, p, grid, stream) : launch<false>(tmQ, tmQfew, tmK, tmV, p, grid, stream);
   if (rc != GQA_OK) return rc;
   // The merge starts while the first kernel drains and waits for it on the device.
-  const int rows = std::min(nt * 128, (longest * G + 31) / 32 * 32);
+  const int longest = max_q_len > 0 ? std::min(max_q_len, T) : T;  // a grid for so many rows; any number is merged
+  const int rows = static_cast<int>(std::min(256LL, (static_cast<long long>(longest) * G + 31) / 32 * 32));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid, std::max(1, rows / 32 * 16 / (kMergeThreads / 32)));
   cfg.blockDim = dim3(kMergeThreads);
@@ -810,5 +1233,5 @@ extern "C" int gqa_attend_chunk_bf16(const void* q, long long q_token_stride, lo
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, merge_kernel, static_cast<const Params>(p), nt) == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, merge_kernel, static_cast<const Params>(p)) == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }

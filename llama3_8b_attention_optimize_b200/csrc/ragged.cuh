@@ -3,14 +3,19 @@
 // Every (sequence, kv head) has units, and a unit has steps (for attention: blocks of
 // query tokens and K/V tiles; for the weight sums: blocks of slots and query tiles).  All steps of
 // all units form one line, sequence by sequence, head by head, unit by unit; CTA c of N takes
-// the steps [c W / N, (c + 1) W / N) of its W.  A unit that lies across a cut is
+// an equal part of its W steps.  A unit that lies across a cut is
 // finished by a merge kernel from the parts that its CTAs leave: the first part in slot
 // 2c + 1 of the CTA where the unit begins, the others in slot 2c of theirs.  So the SMs
 // finish together whatever the lengths, nothing is planned on the host, and two
 // slots a CTA are enough.
 //
-// A Line gives, for a sequence: units(s), count(s, u) steps of unit u, and before(s, k), the
-// steps of the first k units in closed form.
+// A Line gives, for a sequence: has(s), whether it has units; units(s); count(s, u) steps of
+// unit u; ends(s, u), whether u is the last; and before(s, k), the steps of the first k units in
+// closed form, with line.extra steps for each unit: what beginning and ending one costs.  They lie
+// in front of the unit's own and hold no work.  All steps together are fewer than 2^31 (the host's
+// bound).  There may be two lines with a step cost each:
+// the CTAs are dealt out in proportion to what the lines cost, and a sequence has units in
+// one of them.
 #pragma once
 
 #include <cstdint>
@@ -42,18 +47,21 @@ __device__ __forceinline__ Seq seq_of(const Batch& p, int b) {
   return s;
 }
 
-// sum_{i < n} floor((a i + b) / m), by Euclid's steps on (a, m); a, b >= 0, m > 0.
-__device__ __forceinline__ long long floor_sum(long long n, long long m, long long a, long long b) {
-  long long sum = 0;
+// sum_{i < n} floor((a i + b) / m), by Euclid's steps on (a, m).  The caller knows that the
+// sum is below 2^31; what wraps on the way is multiplied by zero.
+__device__ __forceinline__ uint32_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
+  uint32_t sum = 0;
+#pragma unroll 1
   while (n > 0) {
-    sum += (a / m) * (n * (n - 1) / 2) + (b / m) * n;
-    a %= m;
-    b %= m;
-    const long long top = a * n + b;
+    const uint32_t qa = a / m, qb = b / m;
+    sum += qa * (n * (n - 1) / 2) + qb * n;
+    a -= qa * m;
+    b -= qb * m;
+    const uint32_t top = a * n + b;
     if (top < m) break;
     n = top / m;  // count lattice points the other way round
-    b = top % m;
-    const long long x = m;
+    b = top - n * m;
+    const uint32_t x = m;
     m = a;
     a = x;
   }
@@ -62,6 +70,7 @@ __device__ __forceinline__ long long floor_sum(long long n, long long m, long lo
 
 struct Walk {
   int b, h, u, k, left;  // place on the line, and the steps left to this CTA
+  int line;
 };
 
 struct Part {
@@ -73,127 +82,161 @@ struct Part {
 // The CTA's next part of a unit; false when its steps are done.
 template <class Line>
 __device__ __forceinline__ bool next_part(const Batch& p, const Line& line, Walk& w, Part& x) {
-  if (w.left <= 0 || w.b >= p.B) return false;
-  x.s = seq_of(p, w.b);
-  while (line.units(x.s) == 0) {
-    if (++w.b >= p.B) return false;
+  for (;;) {
+    if (w.left <= 0 || w.b >= p.B) return false;
     x.s = seq_of(p, w.b);
-  }
-  x.b = w.b;
-  x.h = w.h;
-  x.u = w.u;
-  x.count = line.count(x.s, w.u);
-  x.k0 = w.k;
-  x.k1 = min(x.count, w.k + w.left);
-  w.left -= x.k1 - x.k0;
-  w.k = 0;
-  if (++w.u >= line.units(x.s)) {
-    w.u = 0;
-    if (++w.h == p.Hkv) {
-      w.h = 0;
-      ++w.b;
+    while (!line.has(x.s)) {
+      if (++w.b >= p.B) return false;
+      x.s = seq_of(p, w.b);
     }
+    x.b = w.b;
+    x.h = w.h;
+    x.u = w.u;
+    x.count = line.count(x.s, w.u);
+    const int end = min(x.count + line.extra, w.k + w.left);
+    w.left -= end - w.k;
+    x.k0 = max(0, w.k - line.extra);
+    x.k1 = end - line.extra;
+    w.k = 0;
+    if (line.ends(x.s, w.u++)) {
+      w.u = 0;
+      if (++w.h == p.Hkv) {
+        w.h = 0;
+        ++w.b;
+      }
+    }
+    if (x.k1 > x.k0) return true;  // else the cut lies in the extra steps: all work is the next CTA's
   }
-  return true;
 }
 
 struct Desc {  // a unit split over CTAs c .. last, written by CTA c (valid = 0: none)
-  int valid, b, h, u, last, pad[3];
+  int valid, b, h, u, last;
+  Seq s;
 };
+static_assert(sizeof(Desc) == 32, "two 16-byte loads");
 
-// By the whole block: this CTA's place on the line (`start`, shared) and the unit that it
-// begins but does not finish (desc[blockIdx.x]).  `scratch`: shared, 8 (kMaxB + 64) bytes.
-// Ends before a barrier that the caller gives.
-template <int kThreads, class Line>
-__device__ __forceinline__ void plan(const Batch& p, const Line& line, long long* scratch, Walk* start, Desc* desc,
-                                     int site_q_start, int site_length) {
+// By the whole block: this CTA's place on its line (`start`, shared) and the unit that it
+// begins but does not finish (desc[blockIdx.x]).  `scratch`: shared, kPlanBytes.  Ends
+// before a barrier that the caller gives.
+constexpr int kPlanBytes = (2 * kMaxB + 64) * 4;
+template <int kThreads, int kLines, class Line>
+__device__ __forceinline__ void plan(const Batch& p, const Line (&lines)[kLines], const int (&cost)[kLines],
+                                     uint32_t* scratch, Walk* start, Desc* desc, int site_q_start, int site_length) {
+  static_assert(kLines == 1 || kLines == 2, "one line or two");
+  constexpr int kWarps = kThreads / 32;
+  static_assert(kWarps <= 32 && kLines * kWarps <= 64, "room for the warps' sums");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  long long* prefix = scratch;          // [B] steps in front of each sequence
-  long long* wsum = scratch + kMaxB;    // [warps]
-  long long carry = 0;
+  uint32_t* wsum = scratch + 2 * kMaxB;  // [kLines][warps]
+  // warps 0 and 1 need the totals; the others work only where there are sequences for them
+  const int warps = max(2, min(kWarps, (p.B + 31) / 32));
+  // ---- steps in front of each sequence, per line: scratch[i * kMaxB + b]
+  uint32_t total[kLines] = {};
+#pragma unroll 1
   for (int b0 = 0; b0 < p.B; b0 += kThreads) {
     const int b = b0 + threadIdx.x;
-    long long mine = 0;
-    if (b < p.B) {
-      const Seq s = seq_of(p, b);
-      const int units = line.units(s);
-      if (units > 0) mine = line.before(s, units) * p.Hkv;
-      if (blockIdx.x == 0) {
-        const int z = __ldg(p.q_start + b + 1), L = __ldg(p.lens + b);
-        if (s.a < 0 || z < s.a || z > p.T) record_input_error(site_q_start);
-        if (L < 0 || L > p.capacity) record_input_error(site_length);
+    uint32_t mine[kLines] = {}, scan[kLines] = {};
+    if (warp < warps) {
+      Seq s = {0, 0, 0};
+      if (b < p.B) {
+        s = seq_of(p, b);
+        if (blockIdx.x == 0) {
+          const int z = __ldg(p.q_start + b + 1), L = __ldg(p.lens + b);
+          if (s.a < 0 || z < s.a || z > p.T) record_input_error(site_q_start);
+          if (L < 0 || L > p.capacity) record_input_error(site_length);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kLines; ++i) {
+        mine[i] = b < p.B && lines[i].has(s) ? lines[i].before(s, lines[i].units(s)) * p.Hkv : 0u;
+        scan[i] = mine[i];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t x = __shfl_up_sync(0xffffffffu, scan[i], o);
+          if (lane >= o) scan[i] += x;
+        }
+        if (lane == 31) wsum[i * kWarps + warp] = scan[i];
       }
     }
-    long long scan = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, scan, o);
-      if (lane >= o) scan += x;
-    }
-    if (lane == 31) wsum[warp] = scan;
     __syncthreads();
-    long long before = carry, all = 0;
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) before += wsum[w];
-      all += wsum[w];
+    if (warp < warps) {
+#pragma unroll
+      for (int i = 0; i < kLines; ++i) {
+        const uint32_t x = lane < warps ? wsum[i * kWarps + lane] : 0u;
+        const uint32_t front = __reduce_add_sync(0xffffffffu, lane < warp ? x : 0u);
+        if (b < p.B) scratch[i * kMaxB + b] = total[i] + front + scan[i] - mine[i];
+        total[i] += __reduce_add_sync(0xffffffffu, x);
+      }
     }
-    if (b < p.B) prefix[b] = before + scan - mine;
-    carry += all;
     __syncthreads();
   }
-  const long long W = carry;
-  const long long ctas = min(static_cast<long long>(gridDim.x), W);
-  const long long c = blockIdx.x;
-  auto locate = [&](long long x) -> Walk {  // the unit and step at place x < W of the line
-    int lo = 0, hi = p.B;                   // the last b with prefix[b] <= x
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (prefix[mid] <= x) lo = mid;
-      else hi = mid;
+  if (warp >= 2) return;
+  // ---- this CTA's line, its first CTA and number of CTAs
+  const int n = static_cast<int>(gridDim.x);
+  int on = 0, c0 = 0, nc = n;
+  if constexpr (kLines == 2) {
+    if (total[1] > 0) {
+      const float w0 = static_cast<float>(total[0]) * cost[0], w1 = static_cast<float>(total[1]) * cost[1];
+      const int n0 = total[0] == 0 ? 0 : min(max(static_cast<int>(n * (w0 / (w0 + w1)) + 0.5f), 1), n - 1);
+      on = static_cast<int>(blockIdx.x) < n0 ? 0 : 1;
+      c0 = on ? n0 : 0;
+      nc = on ? n - n0 : n0;
     }
-    const Seq s = seq_of(p, lo);
+  }
+  const Line line = lines[on];
+  const uint32_t* prefix = scratch + on * kMaxB;
+  const uint32_t W = kLines == 2 && on ? total[kLines - 1] : total[0];
+  const uint32_t ctas = min(static_cast<uint32_t>(nc), W);
+  const uint32_t c = blockIdx.x - c0;
+  // parts: W / ctas steps, the first W % ctas of them one more
+  const uint32_t q = ctas > 0 ? W / ctas : 0u, more = W - q * ctas;
+  auto begin = [&](uint32_t i) -> uint32_t { return i * q + min(i, more); };
+  // Warp 0 finds where the part begins, warp 1 the unit that its end cuts, both by 32-way
+  // searches.
+  const uint32_t x = begin(warp == 0 ? c : c + 1);
+  const bool wanted = warp == 0 ? c < ctas : c + 1 < ctas;
+  Walk w = {0, 0, 0, 0, 0, on};
+  Seq s = {0, 0, 0};
+  if (wanted) {
+    int lo = 0, hi = p.B;  // the last b with prefix[b] <= x
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+      const int below = __popc(__ballot_sync(0xffffffffu, at < hi && prefix[at] <= x));
+      lo += (below - 1) * step;
+      hi = min(hi, lo + step);
+    }
+    s = seq_of(p, lo);
     const int units = line.units(s);
-    const long long head = line.before(s, units);
-    const long long rem = x - prefix[lo];
-    Walk w;
+    const uint32_t head = line.before(s, units), rem = x - prefix[lo];
     w.b = lo;
     w.h = static_cast<int>(rem / head);
-    const long long r = rem - w.h * head;
+    const uint32_t r = rem - w.h * head;
     int u0 = 0, u1 = units;  // the last unit with before(u) <= r
     while (u1 - u0 > 1) {
-      const int mid = (u0 + u1) >> 1;
-      if (line.before(s, mid) <= r) u0 = mid;
-      else u1 = mid;
+      const int step = (u1 - u0 + 31) / 32, at = u0 + lane * step;
+      const int below = __popc(__ballot_sync(0xffffffffu, at < u1 && line.before(s, at) <= r));
+      u0 += (below - 1) * step;
+      u1 = min(u1, u0 + step);
     }
     w.u = u0;
     w.k = static_cast<int>(r - line.before(s, u0));
-    w.left = 0;
-    return w;
-  };
-  if (threadIdx.x == 0) {
-    Walk w = {0, 0, 0, 0, 0};
-    if (c < ctas) {
-      const long long r0 = c * W / ctas, r1 = (c + 1) * W / ctas;
-      w = locate(r0);
-      w.left = static_cast<int>(r1 - r0);
-    }
-    *start = w;
   }
-  if (threadIdx.x == 32) {
+  if (lane != 0) return;
+  if (warp == 0) {
+    if (wanted) w.left = static_cast<int>(begin(c + 1) - x);
+    *start = w;
+  } else {
     Desc d = {0, 0, 0, 0, 0, {0, 0, 0}};
-    if (c + 1 < ctas) {
-      const long long r0 = c * W / ctas, r1 = (c + 1) * W / ctas;
-      const Walk w = locate(r1);
-      if (w.k > 0 && r1 - w.k >= r0) {
-        d.valid = 1;
-        d.b = w.b;
-        d.h = w.h;
-        d.u = w.u;
-        const long long end = r1 - w.k + line.count(seq_of(p, w.b), w.u);
-        d.last = static_cast<int>((end * ctas - 1) / W);  // the CTA of step end - 1
-      }
+    // cut behind a step with work, the first of which is this CTA's
+    if (wanted && w.k > line.extra && x - w.k + line.extra >= begin(c)) {
+      d.valid = 1;
+      d.b = w.b;
+      d.h = w.h;
+      d.u = w.u;
+      d.s = s;
+      const uint32_t last = x - w.k + line.extra + line.count(s, w.u) - 1;  // the unit's last step, and its CTA
+      d.last = c0 + static_cast<int>(last < more * (q + 1) ? last / (q + 1) : more + (last - more * (q + 1)) / q);
     }
-    desc[c] = d;
+    desc[blockIdx.x] = d;
   }
 }
 

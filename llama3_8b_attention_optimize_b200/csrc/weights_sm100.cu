@@ -40,7 +40,6 @@ using ragged::kMaxB;
 using ragged::kMaxCtas;
 using ragged::Part;
 using ragged::Seq;
-using ragged::seq_of;
 using ragged::Walk;
 
 constexpr int kD = 128;
@@ -67,7 +66,7 @@ constexpr int kOffTmemPtr = kOffTok + 128;
 constexpr int kOffStart = kOffTmemPtr + 16;
 constexpr int kSmemBytes = kOffStart + 32;
 static_assert(kSmemBytes <= 232448, "shared memory over the per-block limit");
-static_assert(kMaxB * 8 + 64 * 8 <= 4 * kTileBytes, "the plan's scratch lies in the K tiles");
+static_assert(ragged::kPlanBytes <= kOffBar, "the plan's scratch lies in the tiles");
 static_assert(sizeof(Walk) <= 32, "room for the start");
 
 enum : int {
@@ -107,22 +106,25 @@ struct Params {
 // Units: blocks of 256 slots.  Steps: the query tiles of which some row sees the block; one
 // (empty) step where the sequence brings no tokens, to pass its sums on.
 struct Line {
+  static constexpr int extra = 1;  // a unit's beginning and end cost about a query tile
   int tpt, causal;
   __device__ __forceinline__ Line(const Params& p) : tpt(p.tpt), causal(p.causal) {}
+  __device__ __forceinline__ bool has(const Seq& s) const { return s.L > 0; }
   __device__ __forceinline__ int units(const Seq& s) const { return (s.L + kBlock - 1) / kBlock; }
+  __device__ __forceinline__ bool ends(const Seq& s, int u) const { return (u + 1) * kBlock >= s.L; }
   __device__ __forceinline__ int tiles(const Seq& s) const { return (s.n + tpt - 1) / tpt; }
   // first query tile that sees slot kBlock * u: floor((kBlock u - (L - n)) / tpt), at least 0
   __device__ __forceinline__ int first(const Seq& s, int u) const {
-    const long long x = static_cast<long long>(u) * kBlock - (s.L - s.n);
-    return !causal || x <= 0 ? 0 : static_cast<int>(x / tpt);
+    const int x = u * kBlock - (s.L - s.n);
+    return !causal || x <= 0 ? 0 : x / tpt;
   }
   __device__ __forceinline__ int count(const Seq& s, int u) const { return s.n == 0 ? 1 : tiles(s) - first(s, u); }
-  __device__ __forceinline__ long long before(const Seq& s, int k) const {
-    if (s.n == 0) return k;
-    long long sum = static_cast<long long>(k) * tiles(s);
-    const long long base = s.L - s.n;
-    const int u1 = base > 0 ? static_cast<int>((base + kBlock - 1) / kBlock) : 0;  // first unit past the old slots
-    if (causal && k > u1) sum -= ragged::floor_sum(k - u1, tpt, kBlock, static_cast<long long>(u1) * kBlock - base);
+  __device__ __forceinline__ uint32_t before(const Seq& s, int k) const {
+    if (s.n == 0) return k * (1 + extra);
+    uint32_t sum = static_cast<uint32_t>(k) * (tiles(s) + extra);
+    const int base = s.L - s.n;
+    const int u1 = base > 0 ? (base + kBlock - 1) / kBlock : 0;  // first unit past the old slots
+    if (causal && k > u1) sum -= ragged::floor_sum(k - u1, tpt, kBlock, u1 * kBlock - base);
     return sum;
   }
 };
@@ -163,22 +165,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int lane = threadIdx.x & 31;
   auto bar = [&](int i) -> uint32_t { return sbase + kOffBar + 8 * i; };
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kQStages; ++i) {
-      mbar_init(bar(B_QFULL + i), 1);
-      mbar_init(bar(B_QEMPTY + i), 2);
-    }
-    for (int i = 0; i < 4; ++i) {
-      mbar_init(bar(B_KFULL + i), 1);
-      mbar_init(bar(B_KEMPTY + i), 1);
-      mbar_init(bar(B_SFULL + i), 1);
-      mbar_init(bar(B_SFREE + i), 8);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(bar(B_LFULL + i), 32);
-      mbar_init(bar(B_LEMPTY + i), kSoftmaxWarps);
-      mbar_init(bar(B_DRAIN + i), 1);
-    }
+  if (warp == kWarpHelper) {  // a barrier a lane
+    int count = 1;
+    if (lane >= B_QEMPTY && lane < B_KFULL) count = 2;
+    if (lane >= B_SFREE && lane < B_LFULL) count = 8;
+    if (lane >= B_LFULL && lane < B_LEMPTY) count = 32;
+    if (lane >= B_LEMPTY && lane < B_DRAIN) count = kSoftmaxWarps;
+    if (lane < B_DRAIN + 2) mbar_init(bar(lane), count);
     fence_mbar_init();
   }
   if (threadIdx.x < 128) smem[kOffTok + threadIdx.x] = static_cast<uint8_t>(threadIdx.x / p.G);
@@ -191,7 +184,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tmK);
   }
   const Line line(p);
-  ragged::plan<kThreads>(p.batch, line, reinterpret_cast<long long*>(smem + kOffK),
+  const Line lines[1] = {line};
+  const int cost[1] = {1};
+  ragged::plan<kThreads>(p.batch, lines, cost, reinterpret_cast<uint32_t*>(smem),
                          reinterpret_cast<Walk*>(smem + kOffStart), p.desc, SITE_Q_START, SITE_LENGTH);
   tc_fence_before();
   __syncthreads();
@@ -338,6 +333,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (ragged::next_part(p.batch, line, walk, s)) {
       const int slot = s.u * kBlock + 128 * kt + r;
       const int warp_last = min(s.s.L, s.u * kBlock + 128 * kt + (warp & 3) * 32 + 32) - 1;
+      const size_t at = (static_cast<size_t>(s.b) * p.batch.Hkv + s.h) * p.batch.capacity + slot;
+      // read now: a load's latency is as long as a unit of a single-token batch
+      const float old = ch == 0 && slot < s.s.L - s.s.n && s.whole() ? p.acc[at] : 0.0f;
       float sum = 0.0f;
       if (s.s.n > 0) {
         const int first = line.first(s.s, s.u);
@@ -386,8 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok && ch == 0 && slot < s.s.L) {
         sum += xsum[r];
         if (s.whole()) {
-          const size_t at = (static_cast<size_t>(s.b) * p.batch.Hkv + s.h) * p.batch.capacity + slot;
-          p.acc_out[at] = (slot < s.s.L - s.s.n ? p.acc[at] : 0.0f) + sum;
+          p.acc_out[at] = old + sum;
         } else {
           p.part[static_cast<size_t>(2 * blockIdx.x + (s.k0 == 0 ? 1 : 0)) * kBlock + 128 * kt + r] = sum;
         }
@@ -409,7 +406,7 @@ __global__ void __launch_bounds__(kBlock) merge_kernel(const Params p) {
   cudaGridDependencySynchronize();
   const Desc d = p.desc[blockIdx.x];
   if (!d.valid) return;
-  const Seq s = seq_of(p.batch, d.b);
+  const Seq& s = d.s;
   const int slot = d.u * kBlock + threadIdx.x;
   if (slot >= s.L) return;
   float sum = 0.0f;
@@ -456,6 +453,9 @@ extern "C" int gqa_attn_weight_sums_f32(const void* q, long long q_token_stride,
   const long long capacity = static_cast<long long>(max_pages_per_seq) * page_size;
   const long long pool_rows = static_cast<long long>(num_pages) * Hkv * page_size;
   if (G > 128 || B > kMaxB || capacity > 0x7FFFFE00LL || pool_rows > 0x7FFFFFFFLL) return GQA_ERR_UNSUPPORTED;
+  // query tiles over all blocks of slots: counted in 32 bits
+  const long long steps = (T + 128 / G - 1) / (128 / G) + 2 * B;
+  if (static_cast<double>(steps) * Hkv * (capacity / kBlock + 1) >= 2147483648.0) return GQA_ERR_UNSUPPORTED;
   // a TMA dimension needs a stride: heads or tokens that share one row are the caller's to expand
   if ((T > 1 && q_token_stride == 0) || (Hq > 1 && q_head_stride == 0)) return GQA_ERR_UNSUPPORTED;
   if (!workspace || workspace_bytes < gqa_attn_weight_sums_workspace_size()) return GQA_ERR_WORKSPACE;
