@@ -50,7 +50,6 @@ using attn::exp2_poly2;
 using attn::fmax3;
 using attn::load_idx_k;
 using attn::load_idx_v;
-using attn::sw128_chunk;
 using ragged::Boxes;
 using ragged::Desc;
 using ragged::kMaxB;
@@ -81,7 +80,7 @@ constexpr int kThreads = 640;
 // Register split (setmaxnreg): the launch gives every thread kRegsLaunch registers; the sum
 // of each form's shares must stay within the launch allocation, or setmaxnreg.inc would
 // wait forever; the host checks the compiled count before the first launch.
-constexpr int kRegsLaunch = 96, kRegsHelper = 64, kRegsMany = 104, kRegsFew = 128;
+constexpr int kRegsLaunch = 96, kRegsHelper = 64, kRegsMany = 104, kRegsFew = 144;
 static_assert(4 * 128 * kRegsMany + 128 * kRegsHelper <= kThreads * kRegsLaunch, "register split over budget");
 static_assert(2 * 128 * kRegsFew + 3 * 128 * kRegsHelper <= kThreads * kRegsLaunch, "register split over budget");
 
@@ -101,17 +100,17 @@ struct Few {
   static constexpr int kOffRed = kOffP + 4 * kSmall;  // [2 warpgroups][4 warps][16] floats
   static constexpr int kOffLim = kOffRed + 512;       // [32] token of a row
 };
-constexpr int kOffBar = 7 * kTileBytes;
+constexpr int kOffX = 7 * kTileBytes;  // row exchange [tile][half][128]: halves differ in one address bit
+constexpr int kOffBar = kOffX + 2 * 2 * 128 * 4;
 constexpr int kNumBars = 33;
-constexpr int kOffX = kOffBar + 40 * 8;  // row exchange [tile][half][128]
-constexpr int kOffTmemPtr = kOffX + 2 * 2 * 128 * 4;
+constexpr int kOffTmemPtr = kOffBar + 34 * 8;
 constexpr int kOffStart = kOffTmemPtr + 16;  // this CTA's place on its line
-constexpr int kOffCold = kOffStart + 32;  // [tile] what the many form's softmax needs only between segments
-constexpr int kSmemBytes = kOffCold + 2 * 64;
-static_assert(Few::kOffLim + 128 <= kOffBar, "the few form's buffers");
-static_assert(sizeof(Walk) <= 32, "room for the start");
+constexpr int kOffCold = kOffStart + 48;  // [tile] what the many form's softmax needs only between segments
+constexpr int kSmemBytes = kOffCold + 2 * 96;
+static_assert(Few::kOffLim + 128 <= kOffX, "the few form's buffers");
+static_assert(sizeof(Walk) <= 48, "room for the start");
 static_assert(kSmemBytes <= 232448, "shared memory over the per-block limit");
-static_assert(ragged::kPlanBytes <= kOffBar, "the plan's scratch lies in the tiles");
+static_assert(ragged::kPlanBytes <= kOffX, "the plan's scratch lies in the tiles");
 
 enum : int {
   // [2]: by Q tile in the many form, by parity of the K/V tile in the few form
@@ -204,13 +203,47 @@ __device__ __forceinline__ bool next_seg(const Params& p, Walk& w, Seg& x) {
 }
 
 // ------------------------------------------------------------------ exponentials
+// The softmax loop of the many form holds 64 scores a thread in the 104 registers that 512
+// of them get, so its shared-memory operands are one 32-bit base each with the rest in the
+// instruction.
+template <int kOff>
+__device__ __forceinline__ bool mbar_try_at(uint32_t base, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1 + %3], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(base), "r"(parity), "n"(kOff)
+      : "memory");
+  return ok != 0;
+}
+template <int kOff>
+__device__ __forceinline__ bool mbar_wait_at(uint32_t base, uint32_t parity, int site) {
+  if (mbar_try_at<kOff>(base, parity)) return true;
+  return mbar_wait(base + kOff, parity, site);
+}
+template <int kOff>
+__device__ __forceinline__ void mbar_arrive_at(uint32_t base) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0 + %1];" ::"r"(base), "n"(kOff) : "memory");
+}
+__device__ __forceinline__ void st_shared(uint32_t addr, float x) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(x) : "memory");
+}
+__device__ __forceinline__ float ld_shared(uint32_t addr) {
+  float x;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(addr) : "memory");
+  return x;
+}
+
 // One 32-column chunk of S -> p = 2^(s*scale_log2 - m) as bf16, stored straight into the
-// K-major SW128 P tile (row r, 16-byte chunks c0..c0+3).  acc sums the rounded p that P V
+// K-major SW128 P tile: 16-byte chunk c of the row lies at row ^ 16 c (the swizzle flips address bits
+// 4-6 by the row, which `row` holds already).  acc sums the rounded p that P V
 // multiplies, so that O / l is a mean whose weights add up to one; accf sums them
 // unrounded, for the log-sum-exp.
 template <bool kEmulate, bool kLse>
-__device__ __forceinline__ void exp_chunk_store(const uint32_t (&s)[32], uint8_t* ptile, int r, int c0, float2 sc2,
-                                                float2 nm2, float2& acc, float2& accf) {
+__device__ __forceinline__ void exp_chunk_store(const uint32_t (&s)[32], uint32_t row, int c0, float2 sc2, float2 nm2,
+                                                float2& acc, float2& accf) {
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     uint32_t w[4];
@@ -229,7 +262,9 @@ __device__ __forceinline__ void exp_chunk_store(const uint32_t (&s)[32], uint8_t
       w[e] = pack_bf16x2(y.x, y.y);
       add_bf16x2_to_f32(acc, w[e]);
     }
-    *reinterpret_cast<uint4*>(ptile + sw128_chunk(r, c0 + c)) = make_uint4(w[0], w[1], w[2], w[3]);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row ^ (16u * (c0 + c))), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3])
+                 : "memory");
   }
 }
 
@@ -433,65 +468,80 @@ __device__ __forceinline__ void issue_many(const Params& p, uint32_t sbase, uint
   mbar_wait_drain(bar(B_DRAIN + tq), 0, SITE_DRAIN);
 }
 
-struct Cold {
+// The many form's softmax threads hold two rows of 32 scores each, so what they need only
+// between segments lies in shared memory: one warp per Q tile walks the line for its
+// eight and writes the segment here.
+struct Shared {
   Walk walk;
-  int a, tok0, n_tok, h, k0, whole;
+  int n, k0, whole;               // tiles of the segment (0: no more), its first, whether it is the unit
+  int a, h, tok0, n_tok, base, L;
 };
-static_assert(sizeof(Cold) <= 64, "room for it");
+static_assert(sizeof(Shared) <= 96, "room for it");
 
 // Softmax warps of the many form: four warpgroups, two per Q tile.
 template <bool kLse>
 __device__ __forceinline__ void softmax_many(const Params& p, uint8_t* smem, uint32_t sbase, uint32_t tmem, Walk walk,
                                              int warp) {
   using C = Many;
-  auto bar = [&](int i) -> uint32_t { return sbase + kOffBar + 8 * i; };
   const int g = warp >> 2;
   const int t = g >> 1;             // Q tile
   const int h = g & 1;              // slots [64h, 64h+64) of each K tile; O dims [64h, 64h+64)
   const int r = threadIdx.x & 127;  // row in tile == TMEM lane
   const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
   const uint32_t tS = tmem + lane_off + 128 * t + 64 * h;
-  const uint32_t tO = tmem + lane_off + 256 + 128 * t + 64 * h;
-  uint8_t* ptile = smem + C::kOffP + t * kTileBytes;
-  float* xchg = reinterpret_cast<float*>(smem + kOffX) + t * 256;  // [half][row]
+  constexpr uint32_t kToO = 256;  // from S_t's columns to O_t's
+  // row r of P_t's half h; its 16-byte chunks lie at prow ^ 16 c
+  const uint32_t prow = sbase + C::kOffP + t * kTileBytes + h * kHalf + r * 128 + ((r & 7) << 4);
+  const uint32_t hot = sbase + kOffBar + 8 * t;                     // this tile's barriers
+  const uint32_t own = sbase + kOffX + 1024 * t + 512 * h + 4 * r;  // exchange; the other half's at own ^ 512
   const int bar_x = 1 + t;     // named barrier: both halves of tile t (256 threads)
   const int bar_free = 3 + t;  // named barrier: exchange slots may be rewritten
-  const float sl2 = p.scale_log2;
   constexpr int kNoToken = 0x3FFFFFFF;
-  volatile Cold* cold = reinterpret_cast<volatile Cold*>(smem + kOffCold + 64 * t);
+  volatile Shared* seg = reinterpret_cast<volatile Shared*>(smem + kOffCold + 96 * t);
+  if (h == 0 && (warp & 3) == 0 && (threadIdx.x & 31) == 0) const_cast<Shared*>(seg)->walk = walk;
   bool ok = true;
-  uint32_t Gb = 0;
+  uint32_t phase = 0;  // parity of this tile's iterations
   // Every warp of the tile runs every iteration of every segment and meets every named
   // barrier, even after a bounded wait failed (ok == false only skips the work), so
   // the two halves of a tile can never wait on each other forever.
   for (;;) {
-    int n, slot0, lim;
-    {
+    named_bar_sync(bar_free, 256);  // the previous segment has been read
+    if (h == 0 && (warp & 3) == 0) {
+      __syncwarp();
+      Walk w = const_cast<Shared*>(seg)->walk;
       Seg s;
-      if (!next_seg(p, walk, s)) break;
-      if (t * p.tpt >= s.n_tok) continue;  // no rows in this tile
-      n = s.k1 - s.k0;
-      slot0 = s.k0 * kBN + 64 * h;
+      bool more;
+      do more = next_seg(p, w, s);
+      while (more && t * p.tpt >= s.n_tok);  // no rows in this tile
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) {
+        Shared& x = *const_cast<Shared*>(seg);
+        x.walk = w;
+        x.n = more ? s.k1 - s.k0 : 0;
+        x.k0 = s.k0, x.whole = s.whole();
+        x.a = s.s.a, x.h = s.h, x.tok0 = s.tok0, x.n_tok = s.n_tok, x.base = s.base, x.L = s.s.L;
+      }
+    }
+    named_bar_sync(bar_x, 256);
+    const int n = seg->n;
+    if (n == 0) break;
+    int rel;  // the last column of this half of the next tile that this row sees
+    bool mine;
+    {
+      // A row without a token computes what nobody reads, unmasked, so that its warp takes
+      // the masked path only where a real row needs it.
       const int my_tok = r < p.tpt * p.G ? t * p.tpt + r / p.G : kNoToken;  // token in the unit
-      // last slot this row sees (a row without a token computes what nobody reads, unmasked,
-      // so that its warp takes the masked path only where a real row needs it)
-      lim = my_tok < s.n_tok ? (p.causal ? s.base + s.tok0 + my_tok : s.s.L - 1) : kNoToken;
-      // every warp of the tile writes the same values; all have read them before the
-      // first barrier of the epilogue
-      cold->walk.b = walk.b, cold->walk.h = walk.h, cold->walk.u = walk.u, cold->walk.k = walk.k;
-      cold->walk.left = walk.left;
-      cold->a = s.s.a, cold->tok0 = s.tok0, cold->n_tok = s.n_tok, cold->h = s.h, cold->k0 = s.k0;
-      cold->whole = s.whole();
+      mine = my_tok < seg->n_tok;
+      rel = mine ? (p.causal ? seg->base + seg->tok0 + my_tok : seg->L - 1) - seg->k0 * kBN - 64 * h : kNoToken;
     }
     // warps without any token's row only keep the hand-offs going
-    const bool work = __any_sync(0xffffffffu, lim != kNoToken);
+    const bool work = __any_sync(0xffffffffu, mine);
     float m_run = -INFINITY, l_run = 0.0f, lf_run = 0.0f;
+#pragma unroll 1
     for (int j = 0; j < n; ++j) {
-      const uint32_t gi = Gb + j;
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_SFULL + t), gi & 1u, SITE_SOFTMAX));
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait_at<8 * B_SFULL>(hot, phase, SITE_SOFTMAX));
       uint32_t s0[32], s1[32];
       float mx0 = -INFINITY, mx1 = -INFINITY;
-      const int rel = lim - slot0 - j * kBN;  // columns (of this half) > rel are masked
       if (ok && work) {
         tc_fence_after();
         tmem_ld32(tS + 0, s0);
@@ -500,9 +550,9 @@ __device__ __forceinline__ void softmax_many(const Params& p, uint8_t* smem, uin
         reg_dep(s1);
         tc_fence_before();
       }
-      if (ok) mbar_arrive(bar(B_SFREE + t));  // S_t may now be overwritten by the next QK^T
+      if (ok) mbar_arrive_at<8 * B_SFREE>(hot);  // S_t may now be overwritten by the next QK^T
       if (ok && work) {
-        if (rel < 63) {
+        if (rel < 63) {  // columns of this half > rel are masked
 #pragma unroll
           for (int k = 0; k < 32; ++k) {
             if (k > rel) s0[k] = 0xFF800000u;
@@ -515,83 +565,82 @@ __device__ __forceinline__ void softmax_many(const Params& p, uint8_t* smem, uin
           mx1 = fmax3(mx1, __uint_as_float(s1[k]), __uint_as_float(s1[k + 1]));
         }
       }
-      // row max over both halves: slot [h][r] <-> [1-h][r]
+      mx0 = fmaxf(mx0, mx1);
+      // row max over both halves
       named_bar_sync(bar_free, 256);  // everyone has read the previous exchange's slots
-      xchg[h * 128 + r] = fmaxf(mx0, mx1);
+      st_shared(own, mx0);
       named_bar_sync(bar_x, 256);
-      const float m_tile = fmaxf(fmaxf(mx0, mx1), xchg[(1 - h) * 128 + r]) * sl2;
-      const float m_new = fmaxf(m_run, m_tile);
+      const float m_new = fmaxf(m_run, fmaxf(mx0, ld_shared(own ^ 512u)) * p.scale_log2);
       const bool need = m_new > m_run + kRescaleLog2;
-      const float m_use = need ? m_new : m_run;
       const float alpha = need ? ex2_approx(m_run - m_new) : 1.0f;
-      const float moff = (m_use == -INFINITY) ? 0.0f : m_use;
+      m_run = need ? m_new : m_run;
       // P_t's buffer (and O_t) are free once the previous PV finished
-      if (ok && j > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_PVDONE + t), (gi - 1) & 1u, SITE_SOFTMAX));
-      float2 sum = make_float2(0.f, 0.f), sumf = make_float2(0.f, 0.f);
+      if (ok && j > 0) ok = __all_sync(0xffffffffu, mbar_wait_at<8 * B_PVDONE>(hot, phase ^ 1u, SITE_SOFTMAX));
+      l_run *= alpha;
+      if (kLse) lf_run *= alpha;
       if (ok && work) {
-        const float2 sc2 = make_float2(sl2, sl2), nm2 = make_float2(-moff, -moff);
+        const float moff = (m_run == -INFINITY) ? 0.0f : -m_run;
+        const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), nm2 = make_float2(moff, moff);
+        float2 sum = make_float2(0.f, 0.f), sumf = make_float2(0.f, 0.f);
+        uint32_t row = prow;
+        asm volatile("" : "+r"(row));  // keeps the chunks' addresses from living across the loop
         // Chunks with no masked entry may evaluate part of the exponentials on the FMA
         // pipe; its cubic is good to 7.5e-5, enough for a weight that is rounded to
         // bf16 but not for the log-sum-exp.
         if (rel >= 63) {
-          exp_chunk_store<!kLse, kLse>(s0, ptile, r, 8 * h, sc2, nm2, sum, sumf);
-          exp_chunk_store<!kLse, kLse>(s1, ptile, r, 8 * h + 4, sc2, nm2, sum, sumf);
+          exp_chunk_store<!kLse, kLse>(s0, row, 0, sc2, nm2, sum, sumf);
+          exp_chunk_store<!kLse, kLse>(s1, row, 4, sc2, nm2, sum, sumf);
         } else {
-          exp_chunk_store<false, kLse>(s0, ptile, r, 8 * h, sc2, nm2, sum, sumf);
-          exp_chunk_store<false, kLse>(s1, ptile, r, 8 * h + 4, sc2, nm2, sum, sumf);
+          exp_chunk_store<false, kLse>(s0, row, 0, sc2, nm2, sum, sumf);
+          exp_chunk_store<false, kLse>(s1, row, 4, sc2, nm2, sum, sumf);
         }
+        l_run += sum.x + sum.y;
+        if (kLse) lf_run += sumf.x + sumf.y;
         fence_proxy_async_smem();
         if (j > 0 && __any_sync(0xffffffffu, need)) {
           tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < 2; ++c) {
             uint32_t o[32];
-            tmem_ld32(tO + 32 * c, o);
+            tmem_ld32(tS + kToO + 32 * c, o);
             tmem_wait_ld_dep(o);
 #pragma unroll
             for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-            tmem_st32(tO + 32 * c, o);
+            tmem_st32(tS + kToO + 32 * c, o);
           }
           tmem_wait_st();
         }
         tc_fence_before();
       }
-      if (ok) mbar_arrive(bar(B_PREADY + t));
-      l_run = l_run * alpha + (sum.x + sum.y);
-      if (kLse) lf_run = lf_run * alpha + (sumf.x + sumf.y);
-      m_run = m_use;
+      if (ok) mbar_arrive_at<8 * B_PREADY>(hot);
+      phase ^= 1u;
+      if (mine) rel -= kBN;
     }
 
     // ---- epilogue
-    const uint32_t last = Gb + n - 1;
-    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_PVDONE + t), last & 1u, SITE_EPILOGUE));
-    walk.b = cold->walk.b, walk.h = cold->walk.h, walk.u = cold->walk.u, walk.k = cold->walk.k;
-    walk.left = cold->walk.left;
-    const int tok0 = cold->tok0, seq_a = cold->a, kv_head = cold->h, k0 = cold->k0;
-    const bool whole = cold->whole != 0;
+    if (ok) ok = __all_sync(0xffffffffu, mbar_wait_at<8 * B_PVDONE>(hot, phase ^ 1u, SITE_EPILOGUE));
     named_bar_sync(bar_free, 256);
-    xchg[h * 128 + r] = l_run;
+    st_shared(own, l_run);
     named_bar_sync(bar_x, 256);
-    const float l_tot = l_run + xchg[(1 - h) * 128 + r];
+    const float l_tot = l_run + ld_shared(own ^ 512u);
     float lf_tot = 0.0f;
     if (kLse) {
       named_bar_sync(bar_free, 256);
-      xchg[h * 128 + r] = lf_run;
+      st_shared(own, lf_run);
       named_bar_sync(bar_x, 256);
-      lf_tot = lf_run + xchg[(1 - h) * 128 + r];
+      lf_tot = lf_run + ld_shared(own ^ 512u);
     }
     if (ok && work) {
       tc_fence_after();
-      const bool mine = lim != kNoToken;
-      if (whole) {
+      if (seg->whole) {
         const float inv_l = l_tot > 0.0f ? 1.0f / l_tot : 0.0f;
-        const long long tok = seq_a + tok0 + t * p.tpt + r / p.G;
-        const int head = kv_head * p.G + r % p.G;
+        const long long tok = seg->a + seg->tok0 + t * p.tpt + r / p.G;
+        const int head = seg->h * p.G + r % p.G;
         uint16_t* dst = p.o + tok * p.o_t + head * p.o_h + 64 * h;
 #pragma unroll 1
         for (int c = 0; c < 2; ++c) {
           uint32_t o[32];
-          tmem_ld32(tO + 32 * c, o);
+          tmem_ld32(tS + kToO + 32 * c, o);
           tmem_wait_ld_dep(o);
           if (mine) {
 #pragma unroll
@@ -609,13 +658,13 @@ __device__ __forceinline__ void softmax_many(const Params& p, uint8_t* smem, uin
           p.lse[tok * p.Hq + head] = lf_tot > 0.0f ? (m_run + log2f(lf_tot)) * kLn2 : -INFINITY;
       } else {
         // a segment: (O, m, l) to this CTA's slot, 16 bytes of 32 rows side by side
-        const int slot = 2 * blockIdx.x + (k0 == 0 ? 1 : 0);
+        const int slot = 2 * blockIdx.x + (seg->k0 == 0 ? 1 : 0);
         const int row = t * 128 + r;
         float4* dst = p.part_o + (static_cast<size_t>(slot) * 32 + 16 * h) * p.part_rows + row;
 #pragma unroll 1
         for (int c = 0; c < 2; ++c) {
           uint32_t o[32];
-          tmem_ld32(tO + 32 * c, o);
+          tmem_ld32(tS + kToO + 32 * c, o);
           tmem_wait_ld_dep(o);
           if (mine) {
 #pragma unroll
@@ -634,7 +683,6 @@ __device__ __forceinline__ void softmax_many(const Params& p, uint8_t* smem, uin
       }
       tc_fence_before();  // O_t may be overwritten by the next segment's first PV
     }
-    Gb += n;
   }
 }
 
@@ -1187,7 +1235,8 @@ extern "C" int gqa_attend_chunk_bf16(const void* q, long long q_token_stride, lo
   if (!workspace || workspace_bytes < w.bytes) return GQA_ERR_WORKSPACE;
 
   Params p;
-  p.batch = {block_table, q_start, lens, B, T, Hkv, static_cast<int>(capacity), max_pages_per_seq, page_size, num_pages};
+  p.batch = {block_table, q_start, lens, B, T, Hkv, static_cast<int>(capacity), max_pages_per_seq, page_size, num_pages,
+             ragged::whole_log2(page_size)};
   p.o = static_cast<uint16_t*>(o);
   p.lse = lse;
   char* ws = static_cast<char*>(workspace);

@@ -31,6 +31,8 @@ constexpr int kMaxB = 8192;    // sequences (prefix of their steps in shared mem
 struct Batch {
   const int32_t *table, *q_start, *lens;
   int B, T, Hkv, capacity, max_pages, page_size, num_pages;
+  int page_shift;  // log2(page_size) where that is whole, else -1
+  __device__ __forceinline__ int page_of(int slot) const { return page_shift >= 0 ? slot >> page_shift : slot / page_size; }
 };
 
 struct Seq {
@@ -71,6 +73,7 @@ __device__ __forceinline__ uint32_t floor_sum(uint32_t n, uint32_t m, uint32_t a
 struct Walk {
   int b, h, u, k, left;  // place on the line, and the steps left to this CTA
   int line;
+  Seq s;                 // sequence b
 };
 
 struct Part {
@@ -83,12 +86,8 @@ struct Part {
 template <class Line>
 __device__ __forceinline__ bool next_part(const Batch& p, const Line& line, Walk& w, Part& x) {
   for (;;) {
-    if (w.left <= 0 || w.b >= p.B) return false;
-    x.s = seq_of(p, w.b);
-    while (!line.has(x.s)) {
-      if (++w.b >= p.B) return false;
-      x.s = seq_of(p, w.b);
-    }
+    if (w.left <= 0) return false;
+    x.s = w.s;
     x.b = w.b;
     x.h = w.h;
     x.u = w.u;
@@ -102,7 +101,13 @@ __device__ __forceinline__ bool next_part(const Batch& p, const Line& line, Walk
       w.u = 0;
       if (++w.h == p.Hkv) {
         w.h = 0;
-        ++w.b;
+        do {  // the next sequence of this line, read once
+          if (++w.b >= p.B) {
+            w.left = 0;
+            break;
+          }
+          w.s = seq_of(p, w.b);
+        } while (!line.has(w.s));
       }
     }
     if (x.k1 > x.k0) return true;  // else the cut lies in the extra steps: all work is the next CTA's
@@ -194,8 +199,7 @@ __device__ __forceinline__ void plan(const Batch& p, const Line (&lines)[kLines]
   // searches.
   const uint32_t x = begin(warp == 0 ? c : c + 1);
   const bool wanted = warp == 0 ? c < ctas : c + 1 < ctas;
-  Walk w = {0, 0, 0, 0, 0, on};
-  Seq s = {0, 0, 0};
+  Walk w = {0, 0, 0, 0, 0, on, {0, 0, 0}};
   if (wanted) {
     int lo = 0, hi = p.B;  // the last b with prefix[b] <= x
     while (hi - lo > 1) {
@@ -204,7 +208,8 @@ __device__ __forceinline__ void plan(const Batch& p, const Line (&lines)[kLines]
       lo += (below - 1) * step;
       hi = min(hi, lo + step);
     }
-    s = seq_of(p, lo);
+    const Seq s = seq_of(p, lo);
+    w.s = s;
     const int units = line.units(s);
     const uint32_t head = line.before(s, units), rem = x - prefix[lo];
     w.b = lo;
@@ -232,8 +237,8 @@ __device__ __forceinline__ void plan(const Batch& p, const Line (&lines)[kLines]
       d.b = w.b;
       d.h = w.h;
       d.u = w.u;
-      d.s = s;
-      const uint32_t last = x - w.k + line.extra + line.count(s, w.u) - 1;  // the unit's last step, and its CTA
+      d.s = w.s;
+      const uint32_t last = x - w.k + line.extra + line.count(w.s, w.u) - 1;  // the unit's last step, and its CTA
       d.last = c0 + static_cast<int>(last < more * (q + 1) ? last / (q + 1) : more + (last - more * (q + 1)) / q);
     }
     desc[blockIdx.x] = d;
@@ -256,7 +261,7 @@ struct Boxes {
   // The page of this lane's box of the tile at slot0 (-1: it begins at `limit` or above).
   __device__ __forceinline__ int page(const Batch& p, const int32_t* table, int slot0, int limit) const {
     const int at = slot0 + slot;
-    return loads && at < limit ? __ldg(table + at / p.page_size) : -1;
+    return loads && at < limit ? __ldg(table + p.page_of(at)) : -1;
   }
   // Its first row of the pool, -1 for none; a page outside the pool is reported and
   // replaced by page 0, to keep the pipeline flowing.
@@ -267,9 +272,17 @@ struct Boxes {
       record_input_error(site);
       page = 0;
     }
-    return (page * p.Hkv + h) * p.page_size + at % p.page_size;
+    return (page * p.Hkv + h) * p.page_size + at - p.page_of(at) * p.page_size;
   }
 };
+
+// log2 of a power of two, else -1.
+inline int whole_log2(int x) {
+  if (x <= 0 || (x & (x - 1))) return -1;
+  int n = 0;
+  while (x >>= 1) ++n;
+  return n;
+}
 
 }  // namespace ragged
 }  // namespace gqa

@@ -18,7 +18,7 @@
 // steps of all units are cut into equal parts, one per CTA and SM (ragged.cuh).  Parts of
 // one unit leave 256 sums each, which a second kernel adds in order.
 //
-// Pipeline: a producer warp (K tiles two units ahead, query tiles in a ring of 3), one
+// Pipeline: a producer warp (K tiles in a ring of 5, query tiles in one of 2), one
 // MMA-issuing warp per K tile (two S^T buffers each: all 512 TMEM columns), a helper warp
 // that stages each query tile's lse, and eight softmax warps per K tile (a thread: one
 // slot, 64 of the 128 rows).
@@ -46,7 +46,8 @@ constexpr int kD = 128;
 constexpr int kBlock = 256;                // slots of a unit: two K tiles
 constexpr int kTileBytes = 128 * 128 * 2;  // K and Q tiles: 32 KB
 constexpr int kHalf = kTileBytes / 2;
-constexpr int kQStages = 3;
+constexpr int kQStages = 2;
+constexpr int kKStages = 5;  // K tiles in flight; tile i of the CTA (two a unit) lies in stage i % 5
 constexpr float kLog2e = 1.4426950408889634f;
 
 constexpr int kSoftmaxWarps = 16;
@@ -56,24 +57,24 @@ constexpr int kWarpHelper = 19;
 constexpr int kThreads = 640;
 
 constexpr int kOffQ = 0;
-constexpr int kOffK = kOffQ + kQStages * kTileBytes;  // [unit % 2][K tile]
-constexpr int kOffBar = kOffK + 4 * kTileBytes;
+constexpr int kOffK = kOffQ + kQStages * kTileBytes;
+constexpr int kOffBar = kOffK + kKStages * kTileBytes;
 constexpr int kNumBars = 32;
 constexpr int kOffLse = kOffBar + kNumBars * 8;     // [2][128] -lse * log2(e)
 constexpr int kOffSum = kOffLse + 2 * 128 * 4;      // [K tile][128] sums of the rows' second half
 constexpr int kOffTok = kOffSum + 2 * 128 * 4;      // [128] token of a row in its tile
 constexpr int kOffTmemPtr = kOffTok + 128;
 constexpr int kOffStart = kOffTmemPtr + 16;
-constexpr int kSmemBytes = kOffStart + 32;
+constexpr int kSmemBytes = kOffStart + 48;
 static_assert(kSmemBytes <= 232448, "shared memory over the per-block limit");
 static_assert(ragged::kPlanBytes <= kOffBar, "the plan's scratch lies in the tiles");
-static_assert(sizeof(Walk) <= 32, "room for the start");
+static_assert(sizeof(Walk) <= 48, "room for the start");
 
 enum : int {
-  B_QFULL = 0,    // [3]
-  B_QEMPTY = 3,   // [3] one arrival per issuer
-  B_KFULL = 6,    // [4]
-  B_KEMPTY = 10,  // [4]
+  B_QFULL = 0,    // [2]
+  B_QEMPTY = 2,   // [2] one arrival per issuer
+  B_KFULL = 4,    // [5]
+  B_KEMPTY = 9,   // [5]
   B_SFULL = 14,   // [K tile][2]
   B_SFREE = 18,   // [K tile][2] one arrival per softmax warp
   B_LFULL = 22,   // [2] lse of a query tile staged
@@ -112,11 +113,11 @@ struct Line {
   __device__ __forceinline__ bool has(const Seq& s) const { return s.L > 0; }
   __device__ __forceinline__ int units(const Seq& s) const { return (s.L + kBlock - 1) / kBlock; }
   __device__ __forceinline__ bool ends(const Seq& s, int u) const { return (u + 1) * kBlock >= s.L; }
-  __device__ __forceinline__ int tiles(const Seq& s) const { return (s.n + tpt - 1) / tpt; }
+  __device__ __forceinline__ int tiles(const Seq& s) const { return s.n <= tpt ? 1 : (s.n + tpt - 1) / tpt; }  // n > 0
   // first query tile that sees slot kBlock * u: floor((kBlock u - (L - n)) / tpt), at least 0
   __device__ __forceinline__ int first(const Seq& s, int u) const {
     const int x = u * kBlock - (s.L - s.n);
-    return !causal || x <= 0 ? 0 : x / tpt;
+    return !causal || x < tpt ? 0 : x / tpt;
   }
   __device__ __forceinline__ int count(const Seq& s, int u) const { return s.n == 0 ? 1 : tiles(s) - first(s, u); }
   __device__ __forceinline__ uint32_t before(const Seq& s, int k) const {
@@ -129,7 +130,9 @@ struct Line {
   }
 };
 
-// p = 2^(s * sl2 + nl) of 32 rows that all see the slot
+// p = 2^(s * sl2 + nl) of 32 rows that all see the slot.  The exponentials bound a chunk of
+// many tokens, so kPoly of every 8 pairs go to the FMA pipe.
+constexpr int kPoly = 2;
 __device__ __forceinline__ void add_all(const uint32_t (&s)[32], const float* nl, float2 sl2, float2& a0, float2& a1) {
 #pragma unroll
   for (int c = 0; c < 32; c += 4) {
@@ -138,18 +141,50 @@ __device__ __forceinline__ void add_all(const uint32_t (&s)[32], const float* nl
     const float2 y =
         __ffma2_rn(make_float2(__uint_as_float(s[c + 2]), __uint_as_float(s[c + 3])), sl2, make_float2(l.z, l.w));
     a0 = __fadd2_rn(a0, make_float2(ex2_approx(x.x), ex2_approx(x.y)));
-    a1 = __fadd2_rn(a1, make_float2(ex2_approx(y.x), ex2_approx(y.y)));
+    if ((c / 4) % 4 < kPoly)
+      a1 = __fadd2_rn(a1, attn::exp2_poly2_f32(y));
+    else
+      a1 = __fadd2_rn(a1, make_float2(ex2_approx(y.x), ex2_approx(y.y)));
   }
 }
 
-// the same where rows end (nv of them) or see only some slots: row c sees the slot if
-// its token is at least `from` within the tile
-__device__ __forceinline__ void add_some(const uint32_t (&s)[32], const float* nl, const uint8_t* tok, int nv, int from,
-                                         float sl2, float2& a0) {
+// The same where not all of the 32 rows see the slot: only the first nv, and of those the
+// ones whose token is at least `from` within the tile.
+__device__ __forceinline__ void add_masked(const uint32_t (&s)[32], const float* nl, const uint8_t* tok, int nv, int from,
+                                           float sl2, float2& a0) {
 #pragma unroll
-  for (int c = 0; c < 32; ++c) {
-    const float e = ex2_approx(fmaf(__uint_as_float(s[c]), sl2, nl[c]));
-    if (c < nv && static_cast<int>(tok[c]) >= from) a0.x += e;  // anything else may be NaN
+  for (int c = 0; c < 32; c += 4) {
+    const float4 l = *reinterpret_cast<const float4*>(nl + c);
+    const uchar4 t = *reinterpret_cast<const uchar4*>(tok + c);
+    const float e[4] = {ex2_approx(fmaf(__uint_as_float(s[c]), sl2, l.x)), ex2_approx(fmaf(__uint_as_float(s[c + 1]), sl2, l.y)),
+                        ex2_approx(fmaf(__uint_as_float(s[c + 2]), sl2, l.z)),
+                        ex2_approx(fmaf(__uint_as_float(s[c + 3]), sl2, l.w))};
+    const int k[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i < nv && k[i] >= from) a0.x += e[i];  // anything else may be NaN
+  }
+}
+
+// The same for a few rows, eight at a time: units of single tokens are so short that the
+// fetching of more code would bound them (213 -> 115 us for 64 tokens).
+__device__ __forceinline__ void add_some(uint32_t taddr, const float* nl, const uint8_t* tok, int nv, int from, float sl2,
+                                         float2& a0) {
+#pragma unroll 1
+  for (int c0 = 0; c0 < nv; c0 += 8) {
+    uint32_t v[8];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(taddr + c0));
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7])
+                 :
+                 : "memory");
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const float e = ex2_approx(fmaf(__uint_as_float(v[c]), sl2, nl[c0 + c]));
+      if (c0 + c < nv && static_cast<int>(tok[c0 + c]) >= from) a0.x += e;  // anything else may be NaN
+    }
   }
 }
 
@@ -201,31 +236,40 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kWarpProducer) {
     // ------------------------------------------------------------ TMA producer (whole warp)
     bool ok = true;
-    uint32_t g = 0, m = 0;  // query tiles and units loaded
+    uint32_t g = 0, m = 0;  // query tiles and K tiles loaded
     const Boxes boxes(p.box, lane);
-    while (ok && ragged::next_part(p.batch, line, walk, s)) {
-      if (s.s.n == 0) continue;
+    // the next unit with tokens and its pages, looked up a unit ahead
+    int page[2] = {-1, -1};
+    auto advance = [&]() -> bool {
+      do {
+        if (!ragged::next_part(p.batch, line, walk, s)) return false;
+      } while (s.s.n == 0);
       const int32_t* table = p.batch.table + static_cast<size_t>(s.b) * p.batch.max_pages;
-      const int slot0 = s.u * kBlock;
-      int page[2];
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) page[kt] = boxes.page(p.batch, table, slot0 + 128 * kt, s.s.L);
-      for (int kt = 0; ok && kt < 2 && m >= 2; ++kt)
-        ok = __all_sync(0xffffffffu, mbar_wait(bar(B_KEMPTY + 2 * (m & 1) + kt), (m / 2 - 1) & 1u, SITE_PRODUCER));
-      if (!ok) break;
+      for (int kt = 0; kt < 2; ++kt) page[kt] = boxes.page(p.batch, table, s.u * kBlock + 128 * kt, s.s.L);
+      return true;
+    };
+    bool more = advance();
+    while (ok && more) {
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        const int st = 2 * (m & 1) + kt;
-        const int row = boxes.row(p.batch, page[kt], s.h, slot0 + 128 * kt, s.s.L, SITE_BAD_PAGE);
+        const int st = static_cast<int>(m % kKStages);
+        const int row = boxes.row(p.batch, page[kt], s.h, s.u * kBlock + 128 * kt, s.s.L, SITE_BAD_PAGE);
+        if (ok && m >= kKStages)
+          ok = __all_sync(0xffffffffu, mbar_wait(bar(B_KEMPTY + st), (m / kKStages - 1) & 1u, SITE_PRODUCER));
+        if (!ok) break;
         const uint32_t mine = __ballot_sync(0xffffffffu, row >= 0);
         if (lane == 0) mbar_expect_tx(bar(B_KFULL + st), __popc(mine) * p.box * 128);
         __syncwarp();
         if (row >= 0)
           tma_load_3d(sbase + kOffK + st * kTileBytes + boxes.offset, &tmK, bar(B_KFULL + st), boxes.half * 64, row, 0);
+        ++m;
       }
-      ++m;
-      const int first = line.first(s.s, s.u);
-      for (int k = s.k0; k < s.k1; ++k, ++g) {
+      if (!ok) break;
+      const int steps = s.k1 - s.k0, head = s.h * p.G;
+      int tok = s.s.a + (line.first(s.s, s.u) + s.k0) * p.tpt;
+      more = advance();
+      for (int k = 0; k < steps; ++k, ++g, tok += p.tpt) {
         const int st = static_cast<int>(g % kQStages);
         if (g >= kQStages)
           ok = __all_sync(0xffffffffu, mbar_wait(bar(B_QEMPTY + st), (g / kQStages - 1) & 1u, SITE_PRODUCER));
@@ -233,32 +277,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) {
           mbar_expect_tx(bar(B_QFULL + st), 2 * 128 * p.G * p.tpt);
           for (int e = 0; e < 2; ++e)
-            tma_load_4d(sbase + kOffQ + st * kTileBytes + e * kHalf, &tmQ, bar(B_QFULL + st), 64 * e, s.h * p.G,
-                        s.s.a + (first + k) * p.tpt, 0);
+            tma_load_4d(sbase + kOffQ + st * kTileBytes + e * kHalf, &tmQ, bar(B_QFULL + st), 64 * e, head, tok, 0);
         }
       }
     }
     // Drain: every load this warp issued must land before the CTA may exit.
     for (uint32_t i = g > kQStages ? g - kQStages : 0u; i < g; ++i)
       mbar_wait_drain(bar(B_QFULL + static_cast<int>(i % kQStages)), (i / kQStages) & 1u, SITE_DRAIN);
-    for (uint32_t i = m > 2 ? m - 2 : 0u; i < m; ++i)
-      for (int kt = 0; kt < 2; ++kt) mbar_wait_drain(bar(B_KFULL + 2 * (i & 1) + kt), (i / 2) & 1u, SITE_DRAIN);
+    for (uint32_t i = m > kKStages ? m - kKStages : 0u; i < m; ++i)
+      mbar_wait_drain(bar(B_KFULL + static_cast<int>(i % kKStages)), (i / kKStages) & 1u, SITE_DRAIN);
     __syncwarp();
   } else if (warp == kWarpMma || warp == kWarpMma + 1) {
     // ------------------------------------------------------------ MMA issuers, one per K tile
     const int kt = warp - kWarpMma;
     if (lane == 0) {
       constexpr uint32_t kHi = sdesc_hi_sw128(1024);
-      const uint32_t k_lo = sdesc_lo(sbase + kOffK + kt * kTileBytes, 16);
+      const uint32_t k_lo = sdesc_lo(sbase + kOffK, 16);
       const uint32_t q_lo = sdesc_lo(sbase + kOffQ, 16);
       constexpr uint32_t kTile16 = kTileBytes / 16;
       bool ok = true;
-      uint32_t g = 0, m = 0;
+      uint32_t g = 0, m = kt;  // query tiles, and the K tile
       while (ok && ragged::next_part(p.batch, line, walk, s)) {
         if (s.s.n == 0) continue;
-        const int ks = 2 * (m & 1) + kt;
-        const uint32_t a0 = k_lo + 2 * (m & 1) * kTile16;
-        ok = mbar_wait_spin(bar(B_KFULL + ks), (m / 2) & 1u, SITE_MMA);
+        const int ks = static_cast<int>(m % kKStages);
+        const uint32_t a0 = k_lo + ks * kTile16;
+        ok = mbar_wait_spin(bar(B_KFULL + ks), (m / kKStages) & 1u, SITE_MMA);
         const int first = line.first(s.s, s.u);
         for (int k = s.k0; ok && k < s.k1; ++k, ++g) {
           const int st = static_cast<int>(g % kQStages), bb = static_cast<int>(g & 1);
@@ -279,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           umma_commit(bar(B_QEMPTY + st));
           if (k + 1 == s.k1) umma_commit(bar(B_KEMPTY + ks));
         }
-        ++m;
+        m += 2;
       }
       umma_commit(bar(B_DRAIN + kt));
       mbar_wait_drain(bar(B_DRAIN + kt), 0, SITE_DRAIN);
@@ -329,51 +372,67 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
     bool ok = true;
     uint32_t g = 0;
+    // A slot's old sum, read a unit ahead: its latency is as long as a unit of a
+    // single-token batch.
+    auto slot_of = [&](const Part& x) -> int { return x.u * kBlock + 128 * kt + r; };
+    auto old_of = [&](const Part& x) -> float {
+      const int slot = slot_of(x);
+      if (ch != 0 || slot >= x.s.L - x.s.n || !x.whole()) return 0.0f;
+      return __ldg(p.acc + (static_cast<size_t>(x.b) * p.batch.Hkv + x.h) * p.batch.capacity + slot);
+    };
+    Part ahead;
+    bool more = ragged::next_part(p.batch, line, walk, s);
+    float old = more ? old_of(s) : 0.0f;
     // Every warp meets the named barriers of every unit, even after a failed wait.
-    while (ragged::next_part(p.batch, line, walk, s)) {
-      const int slot = s.u * kBlock + 128 * kt + r;
+    while (more) {
+      more = ragged::next_part(p.batch, line, walk, ahead);
+      const float old_ahead = more ? old_of(ahead) : 0.0f;
+      const int slot = slot_of(s);
       const int warp_last = min(s.s.L, s.u * kBlock + 128 * kt + (warp & 3) * 32 + 32) - 1;
-      const size_t at = (static_cast<size_t>(s.b) * p.batch.Hkv + s.h) * p.batch.capacity + slot;
-      // read now: a load's latency is as long as a unit of a single-token batch
-      const float old = ch == 0 && slot < s.s.L - s.s.n && s.whole() ? p.acc[at] : 0.0f;
       float sum = 0.0f;
       if (s.s.n > 0) {
         const int first = line.first(s.s, s.u);
         for (int k = s.k0; k < s.k1; ++k, ++g) {
           const int bb = static_cast<int>(g & 1);
           const int t0 = (first + k) * p.tpt;
-          const int nv = min(p.tpt, s.s.n - t0) * p.G - 64 * ch;  // rows of this half
+          const int nv = min(64, min(p.tpt, s.s.n - t0) * p.G - 64 * ch);  // rows of this half
           // the tile's first token sees slots up to see0, each next token one more
           const int see0 = p.causal ? s.s.L - s.s.n + t0 : s.s.L - 1;
           if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_SFULL + 2 * kt + bb), (g / 2) & 1u, SITE_SOFTMAX));
           if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_LFULL + bb), (g / 2) & 1u, SITE_SOFTMAX));
           if (!ok) continue;
-          uint32_t s0[32], s1[32];
-          if (nv > 0) {
-            tc_fence_after();
-            tmem_ld32(tS + 128 * bb, s0);
-            if (nv > 32) tmem_ld32(tS + 128 * bb + 32, s1);
-            tmem_wait_ld_dep(s0);
-            reg_dep(s1);
+          const bool all = see0 >= warp_last;
+          const int from = p.causal ? slot - see0 : 0;  // a row of a token below this does not see the slot
+          float2 a0 = make_float2(0.f, 0.f), a1 = make_float2(0.f, 0.f);
+          const uint32_t tv = tS + 128 * bb;
+          const float* nl = lse + 128 * bb + 64 * ch;
+          tc_fence_after();
+          if (nv > 8) {
+            uint32_t v[32];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const int left = nv - 32 * half;
+              if (left > 0) {
+                tmem_ld32(tv + 32 * half, v);
+                tmem_wait_ld_dep(v);
+              }
+              if (half == 1) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(B_SFREE + 2 * kt + bb));
+              }
+              if (all && left >= 32)
+                add_all(v, nl + 32 * half, sl2, a0, a1);
+              else if (left > 0)
+                add_masked(v, nl + 32 * half, tok + 64 * ch + 32 * half, left, from, p.scale_log2, a0);
+            }
+          } else {
+            add_some(tv, nl, tok + 64 * ch, nv, from, p.scale_log2, a0);
             tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(B_SFREE + 2 * kt + bb));
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(B_SFREE + 2 * kt + bb));
-          if (nv > 0) {
-            const float* nl = lse + 128 * bb + 64 * ch;
-            float2 a0 = make_float2(0.f, 0.f), a1 = make_float2(0.f, 0.f);
-            const bool all = see0 >= warp_last;
-            const int from = slot - see0;  // a row of a token below this does not see the slot
-            if (all && nv >= 32)
-              add_all(s0, nl, sl2, a0, a1);
-            else
-              add_some(s0, nl, tok + 64 * ch, nv, p.causal ? from : 0, p.scale_log2, a0);
-            if (all && nv >= 64)
-              add_all(s1, nl + 32, sl2, a0, a1);
-            else if (nv > 32)
-              add_some(s1, nl + 32, tok + 64 * ch + 32, nv - 32, p.causal ? from : 0, p.scale_log2, a0);
-            sum += (a0.x + a0.y) + (a1.x + a1.y);
-          }
+          sum += (a0.x + a0.y) + (a1.x + a1.y);
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(B_LEMPTY + bb));
         }
@@ -383,12 +442,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       named_bar_sync(1 + kt, 256);
       if (ok && ch == 0 && slot < s.s.L) {
         sum += xsum[r];
-        if (s.whole()) {
-          p.acc_out[at] = old + sum;
-        } else {
+        if (s.whole())
+          p.acc_out[(static_cast<size_t>(s.b) * p.batch.Hkv + s.h) * p.batch.capacity + slot] = old + sum;
+        else
           p.part[static_cast<size_t>(2 * blockIdx.x + (s.k0 == 0 ? 1 : 0)) * kBlock + 128 * kt + r] = sum;
-        }
       }
+      s = ahead;
+      old = old_ahead;
     }
   }
 
@@ -461,7 +521,8 @@ extern "C" int gqa_attn_weight_sums_f32(const void* q, long long q_token_stride,
   if (!workspace || workspace_bytes < gqa_attn_weight_sums_workspace_size()) return GQA_ERR_WORKSPACE;
 
   Params p;
-  p.batch = {block_table, q_start, lens, B, T, Hkv, static_cast<int>(capacity), max_pages_per_seq, page_size, num_pages};
+  p.batch = {block_table, q_start, lens, B, T, Hkv, static_cast<int>(capacity), max_pages_per_seq, page_size, num_pages,
+             ragged::whole_log2(page_size)};
   p.lse = lse;
   p.acc = acc;
   p.acc_out = acc_out;

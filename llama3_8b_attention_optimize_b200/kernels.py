@@ -302,6 +302,11 @@ def decode_paged(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, bl
 # [q_start[b], q_start[b + 1]) and lens[b] counts its cached slots with those tokens
 # included, so its token i of n sits in slot lens[b] - n + i.
 
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
+_SCALE = default_scale()
+_raw_stream = torch._C._cuda_getCurrentRawStream  # (device index) -> cudaStream_t, without a Stream object
+
+
 def _rows3(t: torch.Tensor, name: str, dtype=torch.bfloat16) -> None:
     """A CUDA [T, H, d] tensor whose last dim is contiguous; any token and head strides."""
     if not isinstance(t, torch.Tensor):
@@ -320,20 +325,61 @@ def _no_broadcast(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous() if (T > 1 and t.stride(0) == 0) or (H > 1 and t.stride(1) == 0) else t
 
 
-def _same_device(first: torch.Tensor, *rest: torch.Tensor | None) -> None:
-    for t in rest:
-        if t is not None and t.device != first.device:
-            raise ValueError("all tensors must be on one device")
+def _check(dev: int, rows: tuple, flat: tuple) -> None:
+    """Checks of one call's tensors: rows = (tensor or None, name, dtype) of [T, H, d] tensors with
+    a contiguous last dim, flat = the same of contiguous ones, all on device index `dev`.  A
+    call's checks cost the host as much as a short kernel takes, so the usual case is one
+    pass of cheap tests; what fails one is looked at again for its message."""
+    for t, name, dtype in rows:
+        if t is not None and not (t.__class__ is torch.Tensor and t.dtype is dtype and t.get_device() == dev and
+                                  t.dim() == 3 and t.stride(2) == 1):
+            _rows3(t, name, dtype)
+            if t.get_device() != dev:
+                raise ValueError("all tensors must be on one device")
+    for t, name, dtype in flat:
+        if t is not None and not (t.__class__ is torch.Tensor and t.dtype is dtype and t.get_device() == dev and
+                                  t.is_contiguous()):
+            _need(t, name, dtype)
+            if t.get_device() != dev:
+                raise ValueError("all tensors must be on one device")
 
 
-def _call(device: torch.device, name: str, *args) -> None:
-    """Enqueue one C entry point on the device's current torch stream."""
+def _index(t: torch.Tensor, name: str) -> int:
+    """The CUDA device index of a call's first tensor."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (the kernels have no CPU path)")
+    return t.get_device()
+
+
+def _call(dev: int, name: str, *args) -> None:
+    """Enqueue one C entry point on the current torch stream of device index `dev`."""
     fn = getattr(_lib.load(), name)
-    if torch.cuda.current_device() == device.index:
-        check(fn(*args, torch.cuda.current_stream(device).cuda_stream), name)
+    if torch._C._cuda_getDevice() == dev:
+        rc = fn(*args, _raw_stream(dev))
     else:
-        with torch.cuda.device(device):
-            check(fn(*args, torch.cuda.current_stream(device).cuda_stream), name)
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc != 0:
+        check(rc, name)
+
+
+def _workspace(workspace: torch.Tensor | None, need: int, dev: int) -> torch.Tensor:
+    """The caller's workspace, or one of `need` bytes from torch's allocator (whose streams it follows)."""
+    if workspace is None:
+        return torch.empty(max(need, 16), dtype=torch.uint8, device=_devices[dev])
+    if not isinstance(workspace, torch.Tensor) or workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous tensor on the same device")
+    return workspace
+
+
+class _Devices(dict):
+    def __missing__(self, index: int) -> torch.device:
+        return self.setdefault(index, torch.device("cuda", index))
+
+
+_devices = _Devices()
 
 
 def rope_inv_freq(rot_dim: int, theta: float = ROPE_THETA, *, scaling: str = "none", factor: float = 1.0,
@@ -387,7 +433,7 @@ def rope_table(rows: int, rot_dim: int = HEAD_DIM, theta: float = ROPE_THETA, po
     inv = inv.to(device)
     cos = torch.empty(rows, rot_dim // 2, dtype=torch.float32, device=device)
     sin = torch.empty_like(cos)
-    _call(cos.device, "gqa_rope_table_f32", _ptr(inv), _ptr(cos), _ptr(sin), rows, rot_dim // 2, pos0, mscale)
+    _call(cos.get_device(), "gqa_rope_table_f32", _ptr(inv), _ptr(cos), _ptr(sin), rows, rot_dim // 2, pos0, mscale)
     return cos, sin
 
 
@@ -399,47 +445,38 @@ def rope_positions(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, 
     cos, sin: ``rope_table``.  Pairs are (i, i + rot/2), or (2i, 2i + 1) when ``interleaved``.
     ``inverse`` rotates backwards, which is the gradient's way through this operator.
     ``out`` may be x."""
-    if isinstance(x, torch.Tensor) and x.dtype not in (torch.bfloat16, torch.float32):
+    dev = _index(x, "x")
+    if x.dtype is not _BF16 and x.dtype is not _F32:
         raise TypeError(f"x must be bfloat16 or float32, got {x.dtype}")
-    _rows3(x, "x", x.dtype if isinstance(x, torch.Tensor) else None)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    _check(dev, ((x, "x", x.dtype), (out, "out", x.dtype)),
+           ((positions, "positions", _I32), (cos, "cos", _F32), (sin, "sin", _F32)))
     T, H, d = x.shape
-    _need(positions, "positions", torch.int32)
-    _need(cos, "cos", torch.float32)
-    _need(sin, "sin", torch.float32)
     if positions.shape != (T,):
         raise ValueError("positions must be [T]")
     if cos.dim() != 2 or sin.shape != cos.shape or 2 * cos.shape[1] > d:
         raise ValueError("cos and sin must be [rows, rot/2] with rot <= d")
-    out = torch.empty(T, H, d, dtype=x.dtype, device=x.device) if out is None else out
-    _rows3(out, "out", x.dtype)
     if out.shape != x.shape:
         raise ValueError("out must have x's shape")
-    _same_device(x, positions, cos, sin, out)
-    _call(x.device, "gqa_rope_positions_bf16" if x.dtype == torch.bfloat16 else "gqa_rope_positions_f32", _ptr(x),
-          _ptr(out), _ptr(positions), _ptr(cos), _ptr(sin), T, H, d, 2 * cos.shape[1], cos.shape[0], x.stride(0),
-          x.stride(1), out.stride(0), out.stride(1),
-          (GQA_FLAG_INTERLEAVED if interleaved else 0) | (GQA_FLAG_INVERSE if inverse else 0))
+    rows, half = cos.shape
+    _call(dev, "gqa_rope_positions_bf16" if x.dtype is _BF16 else "gqa_rope_positions_f32", x.data_ptr(), out.data_ptr(),
+          positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), T, H, d, 2 * half, rows, x.stride(0), x.stride(1),
+          out.stride(0), out.stride(1), (GQA_FLAG_INTERLEAVED if interleaved else 0) | (GQA_FLAG_INVERSE if inverse else 0))
     return out
 
 
 def _paged(kpages: torch.Tensor, vpages: torch.Tensor | None, block_table: torch.Tensor, q_start: torch.Tensor | None,
            lens: torch.Tensor) -> tuple[int, int, int, int, int]:
-    """(B, max_pages, page_size, num_pages, Hkv) of checked page pools and tables."""
-    _need(kpages, "kpages")
-    if vpages is not None:
-        _need(vpages, "vpages")
-    _need(block_table, "block_table", torch.int32)
-    _need(lens, "lens", torch.int32)
-    if kpages.dim() != 4 or kpages.shape[3] != HEAD_DIM or (vpages is not None and vpages.shape != kpages.shape):
+    """(B, max_pages, page_size, num_pages, Hkv) of page pools and tables with fitting shapes."""
+    shape = kpages.shape
+    if len(shape) != 4 or shape[3] != HEAD_DIM or (vpages is not None and vpages.shape != shape):
         raise ValueError("kpages and vpages must be [num_pages, Hkv, page_size, 128]")
-    num_pages, Hkv, page_size, _ = kpages.shape
+    num_pages, Hkv, page_size, _ = shape
     if block_table.dim() != 2 or lens.shape != (block_table.shape[0],):
         raise ValueError("block_table must be [B, max_pages] and lens [B]")
     B, max_pages = block_table.shape
-    if q_start is not None:
-        _need(q_start, "q_start", torch.int32)
-        if q_start.shape != (B + 1,):
-            raise ValueError("q_start must be [B + 1]")
+    if q_start is not None and q_start.shape != (B + 1,):
+        raise ValueError("q_start must be [B + 1]")
     return B, max_pages, page_size, num_pages, Hkv
 
 
@@ -453,48 +490,43 @@ def kv_extend(k: torch.Tensor, v: torch.Tensor, kpages: torch.Tensor, vpages: to
     are given.  With ``q`` [T, Hq, 128], rotates the queries too and returns them
     (``q_out``, which may be q).  ``slot_pos`` (int32 [B, Hkv, capacity]) receives the
     position held by each slot written, for ``kv_evict``."""
-    _rows3(k, "k")
-    _rows3(v, "v")
+    dev = _index(k, "k")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin come together")
+    if q is not None and q_out is None:
+        q_out = torch.empty(q.shape, dtype=_BF16, device=k.device)
+    elif q is None and q_out is not None:
+        raise ValueError("q_out needs q")
+    _check(dev, ((k, "k", _BF16), (v, "v", _BF16), (q, "q", _BF16), (q_out, "q_out", _BF16)),
+           ((kpages, "kpages", _BF16), (vpages, "vpages", _BF16), (block_table, "block_table", _I32),
+            (q_start, "q_start", _I32), (lens, "lens", _I32), (positions, "positions", _I32), (cos, "cos", _F32),
+            (sin, "sin", _F32), (slot_pos, "slot_pos", _I32)))
     B, max_pages, page_size, num_pages, Hkv = _paged(kpages, vpages, block_table, q_start, lens)
     T = k.shape[0]
     if k.shape != (T, Hkv, HEAD_DIM) or v.shape != k.shape:
         raise ValueError("k and v must be [T, Hkv, 128]")
-    if (cos is None) != (sin is None):
-        raise ValueError("cos and sin come together")
-    rows = rot = 0
+    rows = half = 0
     if cos is not None:
-        _need(cos, "cos", torch.float32)
-        _need(sin, "sin", torch.float32)
         if cos.dim() != 2 or sin.shape != cos.shape or 2 * cos.shape[1] > HEAD_DIM:
             raise ValueError("cos and sin must be [rows, rot/2] with rot <= 128")
-        rows, rot = cos.shape[0], 2 * cos.shape[1]
-    if positions is not None:
-        _need(positions, "positions", torch.int32)
-        if positions.shape != (T,):
-            raise ValueError("positions must be [T]")
+        rows, half = cos.shape
+    if positions is not None and positions.shape != (T,):
+        raise ValueError("positions must be [T]")
     Hq = q_t = q_h = o_t = o_h = 0
     if q is not None:
-        _rows3(q, "q")
         if q.shape[0] != T or q.shape[2] != HEAD_DIM:
             raise ValueError("q must be [T, Hq, 128]")
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
-        _rows3(q_out, "q_out")
         if q_out.shape != q.shape:
             raise ValueError("q_out must have q's shape")
         Hq, q_t, q_h, o_t, o_h = q.shape[1], q.stride(0), q.stride(1), q_out.stride(0), q_out.stride(1)
-    elif q_out is not None:
-        raise ValueError("q_out needs q")
-    if slot_pos is not None:
-        _need(slot_pos, "slot_pos", torch.int32)
-        if slot_pos.shape != (B, Hkv, max_pages * page_size):
-            raise ValueError("slot_pos must be [B, Hkv, max_pages * page_size]")
-    _same_device(k, v, kpages, vpages, block_table, q_start, lens, positions, cos, sin, q, q_out, slot_pos)
-    _call(k.device, "gqa_kv_extend_bf16", _ptr(k), _ptr(v), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-          _ptr(kpages), _ptr(vpages), _ptr(block_table), max_pages, page_size, num_pages, _ptr(q_start), _ptr(lens),
-          None if positions is None else _ptr(positions), None if cos is None else _ptr(cos),
-          None if sin is None else _ptr(sin), rows, rot, None if q is None else _ptr(q), q_t, q_h,
-          None if q_out is None else _ptr(q_out), o_t, o_h, None if slot_pos is None else _ptr(slot_pos), B, T, Hq, Hkv,
-          HEAD_DIM, GQA_FLAG_INTERLEAVED if interleaved else 0)
+    if slot_pos is not None and slot_pos.shape != (B, Hkv, max_pages * page_size):
+        raise ValueError("slot_pos must be [B, Hkv, max_pages * page_size]")
+    _call(dev, "gqa_kv_extend_bf16", k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+          kpages.data_ptr(), vpages.data_ptr(), block_table.data_ptr(), max_pages, page_size, num_pages, q_start.data_ptr(),
+          lens.data_ptr(), None if positions is None else positions.data_ptr(), None if cos is None else cos.data_ptr(),
+          None if sin is None else sin.data_ptr(), rows, 2 * half, None if q is None else q.data_ptr(), q_t, q_h,
+          None if q is None else q_out.data_ptr(), o_t, o_h, None if slot_pos is None else slot_pos.data_ptr(), B, T, Hq,
+          Hkv, HEAD_DIM, GQA_FLAG_INTERLEAVED if interleaved else 0)
     return q_out
 
 
@@ -512,29 +544,26 @@ def attend_chunk(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, bl
     log of the softmax's sum.  ``max_q_len``: the longest sequence's number of new tokens
     where the caller knows it (a hint that picks the tiling).  Tokens that see no slot give
     zeros and -inf."""
-    _rows3(q, "q")
+    dev = _index(q, "q")
+    out = torch.empty(q.shape, dtype=_BF16, device=q.device) if out is None else out
+    _check(dev, ((q, "q", _BF16), (out, "out", _BF16)),
+           ((kpages, "kpages", _BF16), (vpages, "vpages", _BF16), (block_table, "block_table", _I32),
+            (q_start, "q_start", _I32), (lens, "lens", _I32), (lse, "lse", _F32)))
     B, max_pages, page_size, num_pages, Hkv = _paged(kpages, vpages, block_table, q_start, lens)
     T, Hq, d = q.shape
     if d != HEAD_DIM:
         raise ValueError("q must be [T, Hq, 128]")
-    q = _no_broadcast(q)
-    out = torch.empty(T, Hq, d, dtype=q.dtype, device=q.device) if out is None else out
-    _rows3(out, "out")
     if out.shape != q.shape:
         raise ValueError("out must have q's shape")
-    if lse is not None:
-        _need(lse, "lse", torch.float32)
-        if lse.shape != (T, Hq):
-            raise ValueError("lse must be [T, Hq]")
-    if workspace is None:
-        workspace = torch.empty(max(attend_chunk_workspace_bytes(T, Hq, Hkv), 16), dtype=torch.uint8, device=q.device)
-    _need(workspace, "workspace", workspace.dtype)
-    _same_device(q, kpages, vpages, block_table, q_start, lens, out, lse, workspace)
-    _call(q.device, "gqa_attend_chunk_bf16", _ptr(q), q.stride(0), q.stride(1), _ptr(kpages), _ptr(vpages),
-          _ptr(block_table), max_pages, page_size, num_pages, _ptr(q_start), _ptr(lens), _ptr(out), out.stride(0),
-          out.stride(1), None if lse is None else _ptr(lse), _ptr(workspace),
-          workspace.numel() * workspace.element_size(), B, T, Hq, Hkv, d, max_q_len,
-          default_scale(d) if scale is None else float(scale), GQA_FLAG_CAUSAL if causal else 0)
+    if lse is not None and lse.shape != (T, Hq):
+        raise ValueError("lse must be [T, Hq]")
+    q = _no_broadcast(q)
+    workspace = _workspace(workspace, attend_chunk_workspace_bytes(T, Hq, Hkv), dev)
+    _call(dev, "gqa_attend_chunk_bf16", q.data_ptr(), q.stride(0), q.stride(1), kpages.data_ptr(), vpages.data_ptr(),
+          block_table.data_ptr(), max_pages, page_size, num_pages, q_start.data_ptr(), lens.data_ptr(), out.data_ptr(),
+          out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(), workspace.data_ptr(),
+          workspace.numel() * workspace.element_size(), B, T, Hq, Hkv, d, max_q_len, _SCALE if scale is None else scale,
+          GQA_FLAG_CAUSAL if causal else 0)
     return out
 
 
@@ -554,27 +583,25 @@ def attn_weight_sums(q: torch.Tensor, kpages: torch.Tensor, block_table: torch.T
     ``max_q_len`` is accepted too (this kernel has one tiling)."""
     if max_q_len < 0:
         raise ValueError("max_q_len must not be negative")
-    _rows3(q, "q")
+    dev = _index(q, "q")
+    acc_out = acc if acc_out is None else acc_out
+    _check(dev, ((q, "q", _BF16),),
+           ((kpages, "kpages", _BF16), (block_table, "block_table", _I32), (q_start, "q_start", _I32), (lens, "lens", _I32),
+            (lse, "lse", _F32), (acc, "acc", _F32), (acc_out, "acc_out", _F32)))
     B, max_pages, page_size, num_pages, Hkv = _paged(kpages, None, block_table, q_start, lens)
     T, Hq, d = q.shape
     if d != HEAD_DIM:
         raise ValueError("q must be [T, Hq, 128]")
-    _need(lse, "lse", torch.float32)
     if lse.shape != (T, Hq):
         raise ValueError("lse must be [T, Hq]")
-    acc_out = acc if acc_out is None else acc_out
-    for t, n in ((acc, "acc"), (acc_out, "acc_out")):
-        _need(t, n, torch.float32)
-        if t.shape != (B, Hkv, max_pages * page_size):
-            raise ValueError(f"{n} must be [B, Hkv, max_pages * page_size]")
-    if workspace is None:
-        workspace = torch.empty(attn_weight_sums_workspace_bytes(), dtype=torch.uint8, device=q.device)
-    _need(workspace, "workspace", workspace.dtype)
-    _same_device(q, kpages, block_table, q_start, lens, lse, acc, acc_out, workspace)
+    if acc.shape != (B, Hkv, max_pages * page_size) or acc_out.shape != acc.shape:
+        raise ValueError("acc and acc_out must be [B, Hkv, max_pages * page_size]")
     q = _no_broadcast(q)
-    _call(q.device, "gqa_attn_weight_sums_f32", _ptr(q), q.stride(0), q.stride(1), _ptr(kpages), _ptr(block_table),
-          max_pages, page_size, num_pages, _ptr(q_start), _ptr(lens), _ptr(lse), _ptr(acc), _ptr(acc_out), _ptr(workspace),
-          workspace.numel() * workspace.element_size(), B, T, Hq, Hkv, d, default_scale(d) if scale is None else float(scale), GQA_FLAG_CAUSAL if causal else 0)
+    workspace = _workspace(workspace, attn_weight_sums_workspace_bytes(), dev)
+    _call(dev, "gqa_attn_weight_sums_f32", q.data_ptr(), q.stride(0), q.stride(1), kpages.data_ptr(), block_table.data_ptr(),
+          max_pages, page_size, num_pages, q_start.data_ptr(), lens.data_ptr(), lse.data_ptr(), acc.data_ptr(),
+          acc_out.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(), B, T, Hq, Hkv, d,
+          _SCALE if scale is None else scale, GQA_FLAG_CAUSAL if causal else 0)
     return acc_out
 
 
@@ -592,28 +619,24 @@ def kv_evict(kpages: torch.Tensor, vpages: torch.Tensor, block_table: torch.Tens
     below the new length that goes receives the i-th kept one above it; K and V rows move
     in place.  acc, slot_pos [B, Hkv, capacity] (float32, int32) follow into acc_out,
     slot_pos_out, the lengths into lens_out; each defaults to its input."""
-    B, max_pages, page_size, num_pages, Hkv = _paged(kpages, vpages, block_table, None, lens)
+    dev = _index(kpages, "kpages")
     acc_out = acc if acc_out is None else acc_out
     slot_pos_out = slot_pos if slot_pos_out is None else slot_pos_out
     lens_out = lens if lens_out is None else lens_out
-    for t, n, dt in ((acc, "acc", torch.float32), (acc_out, "acc_out", torch.float32),
-                     (slot_pos, "slot_pos", torch.int32), (slot_pos_out, "slot_pos_out", torch.int32)):
-        _need(t, n, dt)
-        if t.shape != (B, Hkv, max_pages * page_size):
-            raise ValueError(f"{n} must be [B, Hkv, max_pages * page_size]")
-    for t, n in ((next_pos, "next_pos"), (lens_out, "lens_out")):
-        _need(t, n, torch.int32)
-        if t.shape != (B,):
-            raise ValueError(f"{n} must be [B]")
-    if workspace is None:
-        workspace = torch.empty(max(kv_evict_workspace_bytes(B, Hkv, budget), 16), dtype=torch.uint8,
-                                device=kpages.device)
-    _need(workspace, "workspace", workspace.dtype)
-    _same_device(kpages, vpages, block_table, lens, acc, slot_pos, next_pos, acc_out, slot_pos_out, lens_out, workspace)
-    _call(kpages.device, "gqa_kv_evict_bf16", _ptr(kpages), _ptr(vpages), _ptr(block_table), max_pages, page_size,
-          num_pages, _ptr(lens), _ptr(lens_out), _ptr(acc), _ptr(acc_out), _ptr(slot_pos), _ptr(slot_pos_out),
-          _ptr(next_pos), _ptr(workspace), workspace.numel() * workspace.element_size(), B, Hkv, HEAD_DIM, budget,
-          recent, sink)
+    _check(dev, (), ((kpages, "kpages", _BF16), (vpages, "vpages", _BF16), (block_table, "block_table", _I32),
+                     (lens, "lens", _I32), (acc, "acc", _F32), (acc_out, "acc_out", _F32), (slot_pos, "slot_pos", _I32),
+                     (slot_pos_out, "slot_pos_out", _I32), (next_pos, "next_pos", _I32), (lens_out, "lens_out", _I32)))
+    B, max_pages, page_size, num_pages, Hkv = _paged(kpages, vpages, block_table, None, lens)
+    shape = (B, Hkv, max_pages * page_size)
+    if acc.shape != shape or acc_out.shape != shape or slot_pos.shape != shape or slot_pos_out.shape != shape:
+        raise ValueError("acc, acc_out, slot_pos and slot_pos_out must be [B, Hkv, max_pages * page_size]")
+    if next_pos.shape != (B,) or lens_out.shape != (B,):
+        raise ValueError("next_pos and lens_out must be [B]")
+    workspace = _workspace(workspace, kv_evict_workspace_bytes(B, Hkv, budget), dev)
+    _call(dev, "gqa_kv_evict_bf16", kpages.data_ptr(), vpages.data_ptr(), block_table.data_ptr(), max_pages, page_size,
+          num_pages, lens.data_ptr(), lens_out.data_ptr(), acc.data_ptr(), acc_out.data_ptr(), slot_pos.data_ptr(),
+          slot_pos_out.data_ptr(), next_pos.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+          B, Hkv, HEAD_DIM, budget, recent, sink)
 
 
 def linear(x: torch.Tensor, w: torch.Tensor, *, out_f32: bool = False,
