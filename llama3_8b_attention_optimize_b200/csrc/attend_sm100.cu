@@ -66,7 +66,7 @@ constexpr int kHalf = kTileBytes / 2;      // one 64-column swizzle block of 128
 constexpr float kRescaleLog2 = 16.0f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-constexpr int kFewRows = 32;               // rows of a unit of the few-row form
+constexpr int kBlockRows = 16;             // rows of a block of the few-row form; a unit has one or two
 // What one K/V tile costs in each form, for dealing out the CTAs: a tile of the few form is
 // 64 KB from memory, one of the many form two tiles' softmax.
 constexpr int kCostFew = 3, kCostMany = 5;
@@ -87,43 +87,49 @@ static_assert(2 * 128 * kRegsFew + 3 * 128 * kRegsHelper <= kThreads * kRegsLaun
 // Shared memory; the 1024-byte-aligned tiles come first.
 struct Many {
   static constexpr int kStages = 3;
-  static constexpr int kOffQ = 0, kQHalf = kHalf;  // [2 tiles][2 halves of 64 dims]
+  static constexpr int kOffQ = 0, kQHalf = kHalf, kQTile = kTileBytes;  // [2 tiles][2 halves of 64 dims]
   static constexpr int kOffP = 2 * kTileBytes;
   static constexpr int kOffKV = 4 * kTileBytes;
 };
 struct Few {
   static constexpr int kStages = 6;
   static constexpr int kOffKV = 0;
-  static constexpr int kSmall = kFewRows * 128;  // one 64-column block of 32 rows: 4 KB
-  static constexpr int kOffQ = 6 * kTileBytes, kQHalf = kSmall;
-  static constexpr int kOffP = kOffQ + 2 * kSmall;    // [2 buffers][2 halves of 64 slots]
-  static constexpr int kOffRed = kOffP + 4 * kSmall;  // [2 warpgroups][4 warps][16] floats
-  static constexpr int kOffLim = kOffRed + 512;       // [32] token of a row
+  static constexpr int kSmall = kBlockRows * 128;  // 64 columns of a block: 2 KB
+  static constexpr int kQHalf = kSmall, kQTile = 2 * kSmall;
+  static constexpr int kOffQ = 6 * kTileBytes;        // [block][2 halves of 64 dims]
+  static constexpr int kOffP = kOffQ + 2 * kQTile;    // [block][2 buffers][2 halves of 64 slots]
+  static constexpr int kOffRed = kOffP + 8 * kSmall;  // [block][4 warps][16] floats
+  static constexpr int kOffTok = kOffRed + 512;       // [16] token of a row in its block
 };
 constexpr int kOffX = 7 * kTileBytes;  // row exchange [tile][half][128]: halves differ in one address bit
 constexpr int kOffBar = kOffX + 2 * 2 * 128 * 4;
-constexpr int kNumBars = 33;
-constexpr int kOffTmemPtr = kOffBar + 34 * 8;
+constexpr int kNumBars = 50;
+constexpr int kOffTmemPtr = kOffBar + kNumBars * 8;
 constexpr int kOffStart = kOffTmemPtr + 16;  // this CTA's place on its line
 constexpr int kOffCold = kOffStart + 48;  // [tile] what the many form's softmax needs only between segments
 constexpr int kSmemBytes = kOffCold + 2 * 96;
-static_assert(Few::kOffLim + 128 <= kOffX, "the few form's buffers");
+static_assert(Few::kOffTok + 64 <= kOffX, "the few form's buffers");
 static_assert(sizeof(Walk) <= 48, "room for the start");
 static_assert(kSmemBytes <= 232448, "shared memory over the per-block limit");
 static_assert(ragged::kPlanBytes <= kOffX, "the plan's scratch lies in the tiles");
 
 enum : int {
-  // [2]: by Q tile in the many form, by parity of the K/V tile in the few form
-  B_QFULL = 0,     // [2] Q tile of the current unit landed (few: [0] alone)
-  B_QEMPTY = 2,    // [1] last QK^T of the segment complete (one arrival per issuer)
-  B_KVFULL = 3,    // [6] K/V stage landed
-  B_KVEMPTY = 9,   // [6] MMAs reading the stage completed (issuers + helper)
-  B_SFULL = 15,    // [2] S = Q K^T complete
-  B_SFREE = 17,    // [2] S copied to registers
-  B_PREADY = 19,   // [2] P in shared memory, O rescaled
-  B_PVDONE = 21,   // [2] O += P V complete
-  B_VZERO = 23,    // [8] rows past the last seen slot cleared (event k in slot k % 8)
-  B_DRAIN = 31,    // [2] every MMA of issuer t complete
+  // [2]: of Q tile t (many) or block t (few)
+  B_QFULL = 0,     // [2] Q landed
+  B_QEMPTY = 2,    // [2] last QK^T of the segment complete
+  B_KVFULL = 4,    // [6] K/V stage landed
+  B_KVEMPTY = 10,  // [6] MMAs reading the stage completed (issuers + helper)
+  B_SFULL = 16,    // [2] S_t = Q_t K^T complete
+  B_SFREE = 18,    // [2] S_t copied to registers
+  B_PREADY = 20,   // [2] P_t in shared memory, O_t rescaled
+  B_PVDONE = 22,   // [2] O_t += P_t V complete
+  B_VZERO = 24,    // [8] rows past the last seen slot cleared (event k in slot k % 8)
+  B_DRAIN = 32,    // [2] every MMA of issuer t complete
+  // the few form's hand-offs, [block][buffer]
+  F_SFULL = 34,
+  F_SFREE = 38,
+  F_PREADY = 42,
+  F_PVDONE = 46,
 };
 
 enum : int {
@@ -149,7 +155,7 @@ struct Params {
   long long o_t, o_h;
   int G, Hq, causal;
   int tpt, tu;     // query tokens per tile and per unit of the many form
-  int few;         // most new tokens of a sequence of the few form, its unit
+  int few;         // query tokens of a block of the few form, for sequences of up to twice so many
   int box;         // rows of one K/V box: the largest power of two dividing page_size, <= 128
   int part_rows;
   float scale_log2;
@@ -161,7 +167,7 @@ struct Line {
   int tu, causal, from, to;  // sequences with from <= n <= to new tokens
   int extra;
   __device__ __forceinline__ Line(const Params& p, bool many)
-      : tu(many ? p.tu : p.few), causal(p.causal), from(many ? p.few + 1 : 1), to(many ? 0x7FFFFFFF : p.few),
+      : tu(many ? p.tu : 2 * p.few), causal(p.causal), from(many ? 2 * p.few + 1 : 1), to(many ? 0x7FFFFFFF : 2 * p.few),
         extra(many ? kExtraMany : kExtraFew) {}
   __device__ __forceinline__ bool has(const Seq& s) const { return s.n >= from && s.n <= to; }
   __device__ __forceinline__ int units(const Seq& s) const { return (s.n + tu - 1) / tu; }
@@ -186,19 +192,36 @@ struct Line {
   }
 };
 
+// A segment: a CTA's part of a unit.  Its rows lie in Q tiles (many) or blocks (few) t = 0, 1.
 struct Seg : Part {
   int tok0, n_tok, base, limit;
+  int tiles;   // bit t: tile t has rows
+  int second;  // first token (of the unit) of tile 1 where both have rows
   // the unit's last slots lie in this segment and do not fill their tile
   __device__ __forceinline__ bool tail() const { return k1 == count && limit < count * kBN; }
+  __device__ __forceinline__ bool has(int t) const { return (tiles >> t) & 1; }
+  __device__ __forceinline__ int from(int t) const { return t == 1 && tiles == 3 ? second : 0; }
 };
 
+// Units of one block go to the two blocks in turn, so that one's end overlaps the next
+// one's beginning.
 __device__ __forceinline__ bool next_seg(const Params& p, Walk& w, Seg& x) {
-  const Line line(p, w.line != 0);
+  const bool many = w.line != 0;
+  const Line line(p, many);
   if (!ragged::next_part(p.batch, line, w, x)) return false;
   x.tok0 = x.u * line.tu;
   x.n_tok = min(line.tu, x.s.n - x.tok0);
   x.base = x.s.L - x.s.n;
   x.limit = line.limit(x.s, x.u);
+  x.second = many ? p.tpt : p.few;
+  if (x.n_tok > x.second) {
+    x.tiles = 3;
+  } else if (many) {
+    x.tiles = 1;
+  } else {
+    x.tiles = 1 << w.turn;
+    w.turn ^= 1;
+  }
   return true;
 }
 
@@ -271,16 +294,14 @@ __device__ __forceinline__ void exp_chunk_store(const uint32_t (&s)[32], uint32_
 // ------------------------------------------------------------------ shared roles
 // Producer warp (all lanes): per segment K0, its Q tile(s), K1 V0 K2 V1 ...; K and V through the
 // ring of C::kStages tiles.
-template <class C, int kQTiles>
-__device__ __forceinline__ void produce(const Params& p, const CUtensorMap* tmQ, const CUtensorMap* tmK,
+template <class C>
+__device__ __forceinline__ void produce(const Params& p, int q_tokens, const CUtensorMap* tmQ, const CUtensorMap* tmK,
                                         const CUtensorMap* tmV, uint32_t sbase, Walk walk, int lane) {
   constexpr int kStages = C::kStages;
   auto bar = [&](int i) -> uint32_t { return sbase + kOffBar + 8 * i; };
-  const int q_tokens = kQTiles == 2 ? p.tpt : p.few;  // tokens of one Q box
   bool ok = true;
   uint32_t L = 0;               // K/V loads issued by this CTA (ring position)
-  uint32_t n_q[kQTiles] = {};   // Q tiles loaded
-  uint32_t n_seg = 0;
+  uint32_t n_q[2] = {0, 0};     // Q tiles loaded
   const Boxes boxes(p.box, lane);
   Seg s;
   while (ok && next_seg(p, walk, s)) {
@@ -313,30 +334,28 @@ __device__ __forceinline__ void produce(const Params& p, const CUtensorMap* tmQ,
                     boxes.half * 64, row, 0);
       ++L;
       if (li > 0) continue;
-      // The first K tile is on its way.  The Q tiles are reused once the previous segment's
-      // last QK^T is done.
-      if (n_seg > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_QEMPTY), (n_seg - 1) & 1, SITE_PRODUCER));
-      if (!ok) break;
+      // The first K tile is on its way.  A Q tile is reused once the last QK^T of its
+      // previous segment is done.
 #pragma unroll
-      for (int t = 0; t < kQTiles; ++t) {
-        if (t * q_tokens < s.n_tok) {
-          ++n_q[t];
-          if (lane == 0) {
-            const uint32_t dst = sbase + C::kOffQ + t * kTileBytes;
-            mbar_expect_tx(bar(B_QFULL + t), 2 * 128 * p.G * q_tokens);
-            for (int e = 0; e < 2; ++e)
-              tma_load_4d(dst + e * C::kQHalf, tmQ, bar(B_QFULL + t), 64 * e, s.h * p.G, s.s.a + s.tok0 + t * q_tokens, 0);
-          }
+      for (int t = 0; t < 2; ++t) {
+        if (!s.has(t)) continue;
+        if (ok && n_q[t] > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_QEMPTY + t), (n_q[t] - 1) & 1, SITE_PRODUCER));
+        if (!ok) break;
+        ++n_q[t];
+        if (lane == 0) {
+          const uint32_t dst = sbase + C::kOffQ + t * C::kQTile;
+          mbar_expect_tx(bar(B_QFULL + t), 2 * 128 * p.G * q_tokens);
+          for (int e = 0; e < 2; ++e)
+            tma_load_4d(dst + e * C::kQHalf, tmQ, bar(B_QFULL + t), 64 * e, s.h * p.G, s.s.a + s.tok0 + s.from(t), 0);
         }
       }
-      ++n_seg;
     }
   }
   // Drain: every load this warp issued must land before the CTA may exit.
   for (uint32_t i = L > static_cast<uint32_t>(kStages) ? L - kStages : 0u; i < L; ++i)
     mbar_wait_drain(bar(B_KVFULL + static_cast<int>(i % kStages)), (i / kStages) & 1u, SITE_DRAIN);
 #pragma unroll
-  for (int t = 0; t < kQTiles; ++t)
+  for (int t = 0; t < 2; ++t)
     if (n_q[t] > 0) mbar_wait_drain(bar(B_QFULL + t), (n_q[t] - 1) & 1, SITE_DRAIN);
   __syncwarp();
 }
@@ -416,13 +435,12 @@ __device__ __forceinline__ void issue_many(const Params& p, uint32_t sbase, uint
   Seg s;
   while (ok && next_seg(p, walk, s)) {
     const int n = s.k1 - s.k0;
-    if (tq * p.tpt >= s.n_tok) {
+    if (!s.has(tq)) {
       // no rows in this tile: pass the stages on, in step with the ring
       for (int li = 0; ok && li < 2 * n; ++li) {
         ok = wait_kv(L + li);
         if (ok) mbar_arrive(bar(B_KVEMPTY + (L + li) % kStages));
       }
-      if (ok) mbar_arrive(bar(B_QEMPTY));
     } else {
       ok = mbar_wait_spin(bar(B_QFULL + tq), uc & 1u, SITE_MMA) && wait_kv(L + load_idx_k(0)) &&
            (Gb == 0 || mbar_wait_spin(bar(B_SFREE + tq), (Gb - 1) & 1u, SITE_MMA));
@@ -433,7 +451,7 @@ __device__ __forceinline__ void issue_many(const Params& p, uint32_t sbase, uint
         issue_qk(sk);
         umma_commit(bar(B_SFULL + tq));
         umma_commit(bar(B_KVEMPTY + sk));
-        if (n == 1) umma_commit(bar(B_QEMPTY));
+        if (n == 1) umma_commit(bar(B_QEMPTY + tq));
       }
       for (int j = 0; ok && j < n; ++j) {
         const uint32_t g = Gb + j;
@@ -448,7 +466,7 @@ __device__ __forceinline__ void issue_many(const Params& p, uint32_t sbase, uint
           issue_qk(static_cast<int>(ik % kStages));
           umma_commit(bar(B_SFULL + tq));
           umma_commit(bar(B_KVEMPTY + ik % kStages));
-          if (j + 1 == n - 1) umma_commit(bar(B_QEMPTY));
+          if (j + 1 == n - 1) umma_commit(bar(B_QEMPTY + tq));
         }
         ok = wait_kv(iv) && mbar_wait_spin(bar(B_PREADY + tq), g & 1u, SITE_MMA);
         if (ok && j == n - 1 && s.tail()) ok = mbar_wait_spin(bar(B_VZERO + Z % 8), (Z / 8) & 1u, SITE_MMA);
@@ -512,7 +530,7 @@ __device__ __forceinline__ void softmax_many(const Params& p, uint8_t* smem, uin
       Seg s;
       bool more;
       do more = next_seg(p, w, s);
-      while (more && t * p.tpt >= s.n_tok);  // no rows in this tile
+      while (more && !s.has(t));
       __syncwarp();
       if ((threadIdx.x & 31) == 0) {
         Shared& x = *const_cast<Shared*>(seg);
@@ -687,81 +705,83 @@ __device__ __forceinline__ void softmax_many(const Params& p, uint8_t* smem, uin
 }
 
 // ------------------------------------------------------------------ few rows
-// TMEM: S^T buffers at columns 0 and 32, O^T at 64; N = 16 or 32 columns of each in use.
-constexpr uint32_t kColOt = 64;
-__device__ __forceinline__ int few_cols(const Params& p, const Seg& s) { return s.n_tok * p.G <= 16 ? 16 : 32; }
-
-__device__ __forceinline__ void issue_few(const Params& p, uint32_t sbase, uint32_t tmem, Walk walk) {
+// Two blocks of 16 rows, each with its issuer, its softmax warpgroup, its Q, its P and S^T
+// double buffers and its O^T; both read the same ring.  TMEM: S^T of block t, buffer b at
+// column 32 t + 16 b, O^T of block t at 64 + 16 t.
+__device__ __forceinline__ void issue_few(const Params& p, uint32_t sbase, uint32_t tmem, Walk walk, int tq) {
   using C = Few;
   constexpr int kStages = C::kStages;
   auto bar = [&](int i) -> uint32_t { return sbase + kOffBar + 8 * i; };
   constexpr uint32_t kHi = sdesc_hi_sw128(1024);
+  constexpr uint32_t kIdQK = idesc_bf16_f32(128, kBlockRows, false);
+  constexpr uint32_t kIdPV = idesc_bf16_f32(128, kBlockRows, false) | (1u << 15);  // A (V^T) MN-major
   const uint32_t kv_lo = sdesc_lo(sbase + C::kOffKV, 16);
   const uint32_t vt_lo = sdesc_lo(sbase + C::kOffKV, kHalf);
-  const uint32_t q_lo = sdesc_lo(sbase + C::kOffQ, 16);
-  const uint32_t p_lo = sdesc_lo(sbase + C::kOffP, 16);
+  const uint32_t q_lo = sdesc_lo(sbase + C::kOffQ + tq * C::kQTile, 16);
+  const uint32_t p_lo = sdesc_lo(sbase + C::kOffP + tq * 4 * C::kSmall, 16);
+  const uint32_t dS = tmem + 32 * tq, dO = tmem + 64 + 16 * tq;
   constexpr uint32_t kTile16 = kTileBytes / 16;
-  uint32_t id_qk = 0, id_pv = 0;
   auto issue_qk = [&](int st, int bb) {  // S^T = K Q^T
     const uint32_t a0 = kv_lo + st * kTile16;
 #pragma unroll
     for (int kk = 0; kk < 8; ++kk)
-      umma_ss_lohi(tmem + 32u * bb, a0 + ((kk >> 2) * kHalf + (kk & 3) * 32) / 16,
-                   q_lo + ((kk >> 2) * C::kSmall + (kk & 3) * 32) / 16, kHi, id_qk, kk > 0 ? 1u : 0u);
+      umma_ss_lohi(dS + 16u * bb, a0 + ((kk >> 2) * kHalf + (kk & 3) * 32) / 16,
+                   q_lo + ((kk >> 2) * C::kSmall + (kk & 3) * 32) / 16, kHi, kIdQK, kk > 0 ? 1u : 0u);
   };
   auto issue_pv = [&](int st, int bb, uint32_t acc) {  // O^T (+)= V^T P^T
     const uint32_t a0 = vt_lo + st * kTile16;
     const uint32_t b0 = p_lo + bb * (2 * C::kSmall / 16);
-    umma_ss_lohi(tmem + kColOt, a0, b0, kHi, id_pv, acc);
+    umma_ss_lohi(dO, a0, b0, kHi, kIdPV, acc);
 #pragma unroll
     for (int kk = 1; kk < 8; ++kk)
-      umma_ss_lohi(tmem + kColOt, a0 + kk * (2048 / 16), b0 + ((kk >> 2) * C::kSmall + (kk & 3) * 32) / 16, kHi, id_pv,
-                   1u);
+      umma_ss_lohi(dO, a0 + kk * (2048 / 16), b0 + ((kk >> 2) * C::kSmall + (kk & 3) * 32) / 16, kHi, kIdPV, 1u);
   };
   bool ok = true;
-  uint32_t L = 0, Gb = 0, Z = 0, uc = 0;
+  uint32_t L = 0, Gb = 0, Z = 0, uc = 0;  // ring position, this block's iterations, clearing events, segments
   auto wait_kv = [&](uint32_t ii) -> bool {
     return mbar_wait_spin(bar(B_KVFULL + ii % kStages), (ii / kStages) & 1u, SITE_MMA);
   };
-  auto release = [&](int i) {  // the barriers count two issuers
-    umma_commit(bar(i));
-    umma_commit(bar(i));
-  };
   auto qk = [&](uint32_t ik, uint32_t g, bool last) -> bool {
+    const int hb = 2 * tq + (g & 1);
     if (!wait_kv(ik)) return false;
-    if (g >= 2 && !mbar_wait_spin(bar(B_SFREE + (g & 1)), ((g >> 1) - 1) & 1u, SITE_MMA)) return false;
+    if (g >= 2 && !mbar_wait_spin(bar(F_SFREE + hb), ((g >> 1) - 1) & 1u, SITE_MMA)) return false;
     tc_fence_after();
     issue_qk(static_cast<int>(ik % kStages), static_cast<int>(g & 1));
-    umma_commit(bar(B_SFULL + (g & 1)));
-    release(B_KVEMPTY + ik % kStages);
-    if (last) release(B_QEMPTY);
+    umma_commit(bar(F_SFULL + hb));
+    umma_commit(bar(B_KVEMPTY + ik % kStages));
+    if (last) umma_commit(bar(B_QEMPTY + tq));
     return true;
   };
   Seg s;
   while (ok && next_seg(p, walk, s)) {
     const int n = s.k1 - s.k0;
-    const int cols = few_cols(p, s);
-    id_qk = idesc_bf16_f32(128, cols, false);
-    id_pv = idesc_bf16_f32(128, cols, false) | (1u << 15);  // A (V^T) MN-major
-    ok = mbar_wait_spin(bar(B_QFULL), uc & 1u, SITE_MMA) && qk(L + load_idx_k(0), Gb, n == 1);
-    for (int j = 0; ok && j < n; ++j) {
-      const uint32_t g = Gb + j, iv = L + load_idx_v(j, n);
-      if (j + 1 < n) ok = qk(L + load_idx_k(j + 1), g + 1, j + 1 == n - 1);
-      ok = ok && wait_kv(iv) && mbar_wait_spin(bar(B_PREADY + (g & 1)), (g >> 1) & 1u, SITE_MMA);
-      if (ok && j == n - 1 && s.tail()) ok = mbar_wait_spin(bar(B_VZERO + Z % 8), (Z / 8) & 1u, SITE_MMA);
-      if (!ok) break;
-      tc_fence_after();
-      issue_pv(static_cast<int>(iv % kStages), static_cast<int>(g & 1), j > 0 ? 1u : 0u);
-      umma_commit(bar(B_PVDONE + (g & 1)));
-      release(B_KVEMPTY + iv % kStages);
+    if (!s.has(tq)) {
+      for (int li = 0; ok && li < 2 * n; ++li) {  // pass the stages on, in step with the ring
+        ok = wait_kv(L + li);
+        if (ok) mbar_arrive(bar(B_KVEMPTY + (L + li) % kStages));
+      }
+    } else {
+      ok = mbar_wait_spin(bar(B_QFULL + tq), uc & 1u, SITE_MMA) && qk(L + load_idx_k(0), Gb, n == 1);
+      for (int j = 0; ok && j < n; ++j) {
+        const uint32_t g = Gb + j, iv = L + load_idx_v(j, n);
+        const int hb = 2 * tq + (g & 1);
+        if (j + 1 < n) ok = qk(L + load_idx_k(j + 1), g + 1, j + 1 == n - 1);
+        ok = ok && wait_kv(iv) && mbar_wait_spin(bar(F_PREADY + hb), (g >> 1) & 1u, SITE_MMA);
+        if (ok && j == n - 1 && s.tail()) ok = mbar_wait_spin(bar(B_VZERO + Z % 8), (Z / 8) & 1u, SITE_MMA);
+        if (!ok) break;
+        tc_fence_after();
+        issue_pv(static_cast<int>(iv % kStages), static_cast<int>(g & 1), j > 0 ? 1u : 0u);
+        umma_commit(bar(F_PVDONE + hb));
+        umma_commit(bar(B_KVEMPTY + iv % kStages));
+      }
+      Gb += n;
+      ++uc;
     }
     if (s.tail()) ++Z;
     L += 2 * n;
-    Gb += n;
-    ++uc;
   }
-  umma_commit(bar(B_DRAIN));
-  mbar_wait_drain(bar(B_DRAIN), 0, SITE_DRAIN);
+  umma_commit(bar(B_DRAIN + tq));
+  mbar_wait_drain(bar(B_DRAIN + tq), 0, SITE_DRAIN);
 }
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -787,35 +807,25 @@ __device__ __forceinline__ bool named_bar_any(int id, int nthreads, bool v) {
   return r != 0;
 }
 
-// One segment by a softmax warpgroup (two, of 16 rows each): thread i holds slot i of each S^T
-// tile, then dim i of O^T.  The maximum of a row lies across the threads, so it is not taken per
+// One segment by block wg's softmax warpgroup: thread i holds slot i of each S^T tile, then
+// dim i of O^T.  The maximum of a row lies across the threads, so it is not taken per
 // tile: a tile only asks whether any score passes its row's running maximum by more than
 // 2^16 (one barrier vote), which after the first tile hardly ever happens.
 template <bool kLse>
 __device__ __forceinline__ void softmax_few(const Params& p, const Seg& s, uint8_t* smem, uint32_t sbase, uint32_t tmem,
                                             uint32_t& Gb, bool& ok) {
   using C = Few;
-  constexpr int N = 16;  // columns of a warpgroup
+  constexpr int N = kBlockRows;
   auto bar = [&](int i) -> uint32_t { return sbase + kOffBar + 8 * i; };
   const int i = threadIdx.x & 127, wq = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
-  const int wg = threadIdx.x >> 7;  // rows [16 wg, 16 wg + 16)
-  const uint32_t t_lane = tmem + (static_cast<uint32_t>(wq * 32) << 16) + 16 * wg;
+  const int wg = threadIdx.x >> 7;
+  const uint32_t t_lane = tmem + (static_cast<uint32_t>(wq * 32) << 16);
+  const uint32_t tS = t_lane + 32 * wg, tO = t_lane + 64 + 16 * wg;
   const int bar_vote = 1 + wg, bar_red = 3 + wg;
   float* red = reinterpret_cast<float*>(smem + C::kOffRed) + 64 * wg;  // [4 warps][16]
-  const int* tok = reinterpret_cast<const int*>(smem + C::kOffLim) + 16 * wg;
+  const int* tok = reinterpret_cast<const int*>(smem + C::kOffTok);
   const int n = s.k1 - s.k0;
-  if (s.n_tok * p.G <= 16 * wg) {  // no rows: only keep the hand-offs going
-    for (int j = 0; j < n; ++j) {
-      const uint32_t g = Gb + j;
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_SFULL + (g & 1)), (g >> 1) & 1u, SITE_SOFTMAX));
-      if (ok) {
-        mbar_arrive(bar(B_SFREE + (g & 1)));
-        mbar_arrive(bar(B_PREADY + (g & 1)));
-      }
-    }
-    Gb += n;
-    return;
-  }
+  const int first_tok = s.from(wg);
   const float sl2 = p.scale_log2;
   float m[N], l[N], lf[kLse ? N : 1];
 #pragma unroll
@@ -857,23 +867,23 @@ __device__ __forceinline__ void softmax_few(const Params& p, const Seg& s, uint8
   };
   for (int j = 0; j < n; ++j) {
     const uint32_t g = Gb + j;
-    const int bb = static_cast<int>(g & 1);
-    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_SFULL + bb), (g >> 1) & 1u, SITE_SOFTMAX));
+    const int bb = static_cast<int>(g & 1), hb = 2 * wg + bb;
+    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(F_SFULL + hb), (g >> 1) & 1u, SITE_SOFTMAX));
     uint32_t sv[N];
     if (ok) {
       tc_fence_after();
-      tmem_ld16(t_lane + 32 * bb, sv);
+      tmem_ld16(tS + 16 * bb, sv);
       tc_fence_before();
-      mbar_arrive(bar(B_SFREE + bb));
+      mbar_arrive(bar(F_SFREE + hb));
     } else {
 #pragma unroll
       for (int c = 0; c < N; ++c) sv[c] = 0xFF800000u;
     }
     const int slot0 = (s.k0 + j) * kBN, key = slot0 + i;
-    if (slot0 + kBN - 1 > (p.causal ? s.base : s.s.L - 1)) {  // some row does not see all of the tile
+    if (slot0 + kBN - 1 > (p.causal ? s.base + first_tok : s.s.L - 1)) {  // some row does not see all of the tile
 #pragma unroll
       for (int c = 0; c < N; ++c)
-        if (key > (p.causal ? min(s.base + tok[c], s.s.L - 1) : s.s.L - 1)) sv[c] = 0xFF800000u;
+        if (key > (p.causal ? min(s.base + first_tok + tok[c], s.s.L - 1) : s.s.L - 1)) sv[c] = 0xFF800000u;
     }
     float big = -INFINITY;  // -m is +inf as long as the row has seen nothing: its first score votes
 #pragma unroll
@@ -893,22 +903,22 @@ __device__ __forceinline__ void softmax_few(const Params& p, const Seg& s, uint8
         if (kLse) lf[c] *= x[c];
       }
       if (j > 0) {
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_PVDONE + (bb ^ 1)), ((g - 1) >> 1) & 1u, SITE_SOFTMAX));
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(F_PVDONE + (hb ^ 1)), ((g - 1) >> 1) & 1u, SITE_SOFTMAX));
         if (ok) {
           uint32_t o[N];
           tc_fence_after();
-          tmem_ld16(t_lane + kColOt, o);
+          tmem_ld16(tO, o);
 #pragma unroll
           for (int c = 0; c < N; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * x[c]);
-          tmem_st16(t_lane + kColOt, o);
+          tmem_st16(tO, o);
           tmem_wait_st();
         }
       }
     }
     // P's buffer is free once the PV of two tiles ago finished
-    if (ok && j >= 2) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_PVDONE + bb), ((g - 2) >> 1) & 1u, SITE_SOFTMAX));
+    if (ok && j >= 2) ok = __all_sync(0xffffffffu, mbar_wait(bar(F_PVDONE + hb), ((g - 2) >> 1) & 1u, SITE_SOFTMAX));
     if (ok) {
-      uint8_t* dst = smem + C::kOffP + bb * 2 * C::kSmall + (i >> 6) * C::kSmall + wg * 2048 + (i & 7) * 2;
+      uint8_t* dst = smem + C::kOffP + hb * 2 * C::kSmall + (i >> 6) * C::kSmall + (i & 7) * 2;
       const int chunk = (i & 63) >> 3;
 #pragma unroll
       for (int c = 0; c < N; c += 2) {
@@ -926,56 +936,60 @@ __device__ __forceinline__ void softmax_few(const Params& p, const Seg& s, uint8
       }
       fence_proxy_async_smem();
       tc_fence_before();
-      mbar_arrive(bar(B_PREADY + bb));
+      mbar_arrive(bar(F_PREADY + hb));
     }
   }
   Gb += n;
 
   // ---- epilogue.  The last PV needed every thread's P, so `red` has been read.
   const uint32_t last = Gb - 1;
-  if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_PVDONE + (last & 1)), (last >> 1) & 1u, SITE_EPILOGUE));
+  if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(F_PVDONE + 2 * wg + (last & 1)), (last >> 1) & 1u, SITE_EPILOGUE));
+  float my_l = 0.0f, my_lf = 0.0f;  // of row i, where this thread is the one that writes it
+  auto mine = [&]() { return i < N ? (red[i] + red[N + i]) + (red[2 * N + i] + red[3 * N + i]) : 0.0f; };
   across(l, false);
+  my_l = mine();
   if constexpr (kLse) {
     named_bar_sync(bar_vote, 128);
     across(lf, false);
+    my_lf = mine();
   }
   if (!ok) return;
   uint32_t o[N];
   tc_fence_after();
-  tmem_ld16(t_lane + kColOt, o);
-  tc_fence_before();  // O^T may be overwritten by the next segment's first PV
-  const int rows = s.n_tok * p.G - 16 * wg;  // of this warpgroup's columns
+  tmem_ld16(tO, o);
+  tc_fence_before();  // O^T may be overwritten by the block's next segment
+  const int rows = min(p.few, s.n_tok - first_tok) * p.G;
+  float my_m = m[0];
+#pragma unroll
+  for (int c = 1; c < N; ++c) my_m = i == c ? m[c] : my_m;
   if (s.whole()) {
-    uint16_t* dst = p.o + static_cast<long long>(s.s.a + s.tok0) * p.o_t + static_cast<long long>(s.h) * p.G * p.o_h + i;
-    int t = 16 * wg / p.G, hd = 16 * wg % p.G;
+    const int tok0 = s.s.a + s.tok0 + first_tok;
+    uint16_t* dst = p.o + static_cast<long long>(tok0) * p.o_t + static_cast<long long>(s.h) * p.G * p.o_h + i;
+    const long long wrap = p.o_t - (p.G - 1) * p.o_h;  // from a token's last head to the next token's first
+    int hd = 0;
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-      if (c < rows) {
-        const float inv = l[c] > 0.0f ? __fdividef(1.0f, l[c]) : 0.0f;
-        dst[t * p.o_t + hd * p.o_h] = static_cast<uint16_t>(pack_bf16x2(__uint_as_float(o[c]) * inv, 0.0f));
-        if (kLse && i == c)
-          p.lse[static_cast<size_t>(s.s.a + s.tok0 + t) * p.Hq + s.h * p.G + hd] =
-              lf[kLse ? c : 0] > 0.0f ? (m[c] + log2f(lf[kLse ? c : 0])) * kLn2 : -INFINITY;
-        if (++hd == p.G) {
-          hd = 0;
-          ++t;
-        }
-      }
+      if (c < rows)
+        *dst = static_cast<uint16_t>(pack_bf16x2(l[c] > 0.0f ? __uint_as_float(o[c]) * __fdividef(1.0f, l[c]) : 0.0f, 0.0f));
+      const bool end = ++hd == p.G;
+      dst += end ? wrap : p.o_h;
+      if (end) hd = 0;
     }
+    if (kLse && i < rows)
+      p.lse[static_cast<size_t>(tok0 + i / p.G) * p.Hq + s.h * p.G + i % p.G] =
+          my_lf > 0.0f ? (my_m + log2f(my_lf)) * kLn2 : -INFINITY;
   } else {
-    const int slot = 2 * blockIdx.x + (s.k0 == 0 ? 1 : 0);
-    float* dst = reinterpret_cast<float*>(p.part_o + (static_cast<size_t>(slot) * 32 + (i >> 2)) * p.part_rows) + (i & 3);
-    float* ml = p.part_ml + static_cast<size_t>(slot) * 3 * p.part_rows;
+    const int slot = 2 * blockIdx.x + (s.k0 == 0 ? 1 : 0), row0 = first_tok * p.G;
+    float* dst =
+        reinterpret_cast<float*>(p.part_o + (static_cast<size_t>(slot) * 32 + (i >> 2)) * p.part_rows + row0) + (i & 3);
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
-      if (c < rows) {
-        dst[4 * (16 * wg + c)] = __uint_as_float(o[c]);
-        if (i == c) {
-          ml[16 * wg + c] = m[c];
-          ml[p.part_rows + 16 * wg + c] = l[c];
-          ml[2 * p.part_rows + 16 * wg + c] = kLse ? lf[kLse ? c : 0] : 0.0f;
-        }
-      }
+    for (int c = 0; c < N; ++c)
+      if (c < rows) dst[4 * c] = __uint_as_float(o[c]);
+    if (i < rows) {
+      float* ml = p.part_ml + static_cast<size_t>(slot) * 3 * p.part_rows + row0 + i;
+      ml[0] = my_m;
+      ml[p.part_rows] = my_l;
+      ml[2 * p.part_rows] = my_lf;
     }
   }
 }
@@ -1002,10 +1016,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     static_assert(kNumBars <= 64, "two a lane");
     for (int i = lane; i < kNumBars; i += 32) {
       int count = 1;
-      if (i == B_QEMPTY) count = 2;                          // issuers
-      if (i >= B_KVEMPTY && i < B_KVEMPTY + 6) count = 3;    // issuers and helper
-      if (i >= B_SFREE && i < B_PVDONE) count = 256;         // softmax threads of a hand-off
+      if (i >= B_KVEMPTY && i < B_SFULL) count = 3;    // issuers and helper
+      if (i >= B_SFREE && i < B_PVDONE) count = 256;   // softmax threads of a hand-off
       if (i >= B_VZERO && i < B_DRAIN) count = 32;
+      if (i >= F_SFREE && i < F_PVDONE) count = 128;
       mbar_init(bar(i), count);
     }
     fence_mbar_init();
@@ -1030,9 +1044,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const bool many = walk.line != 0;
   if (!many) {
     // Q rows that no box fills stay zero; the token of each row
-    for (int i = threadIdx.x; i < 2 * Few::kSmall / 16; i += kThreads)
+    for (int i = threadIdx.x; i < 2 * Few::kQTile / 16; i += kThreads)
       reinterpret_cast<uint4*>(smem + Few::kOffQ)[i] = make_uint4(0, 0, 0, 0);
-    if (threadIdx.x < kFewRows) reinterpret_cast<int*>(smem + Few::kOffLim)[threadIdx.x] = threadIdx.x / p.G;
+    if (threadIdx.x < kBlockRows) reinterpret_cast<int*>(smem + Few::kOffTok)[threadIdx.x] = threadIdx.x / p.G;
   }
   // Generic writes (the plan's scratch, zeros) lie where TMA will write.
   fence_proxy_async_smem();
@@ -1042,9 +1056,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     regs_dec<kRegsHelper>();
     if (warp == kWarpProducer) {
       if (many)
-        produce<Many, 2>(p, &tmQ, &tmK, &tmV, sbase, walk, lane);
+        produce<Many>(p, p.tpt, &tmQ, &tmK, &tmV, sbase, walk, lane);
       else
-        produce<Few, 1>(p, &tmQfew, &tmK, &tmV, sbase, walk, lane);
+        produce<Few>(p, p.few, &tmQfew, &tmK, &tmV, sbase, walk, lane);
     } else if (warp == kWarpHelper) {
       if (many)
         clear_tails<Many>(p, smem, sbase, walk, lane);
@@ -1054,8 +1068,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) {
         if (many)
           issue_many(p, sbase, tmem, walk, warp - kWarpMma);
-        else if (warp == kWarpMma)
-          issue_few(p, sbase, tmem, walk);
+        else
+          issue_few(p, sbase, tmem, walk, warp - kWarpMma);
       }
       __syncwarp();
     }
@@ -1068,7 +1082,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     Seg s;
     bool ok = true;
     uint32_t Gb = 0;
-    while (next_seg(p, w, s)) softmax_few<kLse>(p, s, smem, sbase, tmem, Gb, ok);
+    while (next_seg(p, w, s))
+      if (s.has(threadIdx.x >> 7)) softmax_few<kLse>(p, s, smem, sbase, tmem, Gb, ok);
   } else {
     regs_dec<kRegsHelper>();
   }
@@ -1093,7 +1108,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const Params p) {
   const Desc d = p.desc[c0];
   if (!d.valid) return;
   const Seq& s = d.s;
-  const int tu = s.n <= p.few ? p.few : p.tu;
+  const int tu = s.n <= 2 * p.few ? 2 * p.few : p.tu;
   const int n_tok = min(tu, s.n - d.u * tu);
   const int rows_tile = p.tpt * p.G;
   const int rows = n_tok > p.tpt ? 128 + (n_tok - p.tpt) * p.G : n_tok * p.G;
@@ -1252,7 +1267,7 @@ extern "C" int gqa_attend_chunk_bf16(const void* q, long long q_token_stride, lo
   p.box = std::min(128, page_size & -page_size);
   p.tpt = 128 / G;
   p.tu = 2 * p.tpt;
-  p.few = kFewRows / G;
+  p.few = kBlockRows / G;
 
   CUtensorMap tmQ, tmQfew, tmK, tmV;
   int rc;

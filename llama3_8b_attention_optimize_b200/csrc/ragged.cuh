@@ -73,6 +73,7 @@ __device__ __forceinline__ uint32_t floor_sum(uint32_t n, uint32_t m, uint32_t a
 struct Walk {
   int b, h, u, k, left;  // place on the line, and the steps left to this CTA
   int line;
+  int turn;              // for the kernel's own use
   Seq s;                 // sequence b
 };
 
@@ -199,7 +200,7 @@ __device__ __forceinline__ void plan(const Batch& p, const Line (&lines)[kLines]
   // searches.
   const uint32_t x = begin(warp == 0 ? c : c + 1);
   const bool wanted = warp == 0 ? c < ctas : c + 1 < ctas;
-  Walk w = {0, 0, 0, 0, 0, on, {0, 0, 0}};
+  Walk w = {0, 0, 0, 0, 0, on, 0, {0, 0, 0}};
   if (wanted) {
     int lo = 0, hi = p.B;  // the last b with prefix[b] <= x
     while (hi - lo > 1) {
