@@ -1288,14 +1288,6 @@ extern "C" int gqa_attend_chunk_bf16(const void* q, long long q_token_stride, lo
   // The merge starts while the first kernel drains and waits for it on the device.
   const int longest = max_q_len > 0 ? std::min(max_q_len, T) : T;  // a grid for so many rows; any number is merged
   const int rows = static_cast<int>(std::min(256LL, (static_cast<long long>(longest) * G + 31) / 32 * 32));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid, std::max(1, rows / 32 * 16 / (kMergeThreads / 32)));
-  cfg.blockDim = dim3(kMergeThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, merge_kernel, static_cast<const Params>(p)) == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
+  return launch_after(merge_kernel, dim3(grid, std::max(1, rows / 32 * 16 / (kMergeThreads / 32))), kMergeThreads, stream,
+                      p);
 }

@@ -7,14 +7,17 @@
 // ascending order: rows that can stay do, and no row is both read and written, so all
 // rows move at once and in place.
 //
-// Kernel 1, one block per (b, h): order-preserving 32-bit keys of the weights, the
-// budget-th largest by four 8-bit histogram passes, then the lists of holes and movers
-// by ballots (each warp owns a contiguous run of slots, so three block barriers order
-// everything).  Kernel 2 moves the rows: 512 bytes (K and V) a warp step.
+// Kernel 1, one block per (b, h): order-preserving 32-bit keys of the weights in shared
+// memory, the budget-th largest by three histogram passes (11, 11 and 10 bits), then the
+// lists of holes and movers by ballots (each warp owns a contiguous run of slots, so three
+// block barriers order everything).  Bound by latencies: loads are issued eight at a time.
+// Kernel 2 moves the rows, bound by memory: 16 rows a warp step, their slots turned into
+// addresses by one lane each, K by lanes 0-15 and V by 16-31, 16 bytes a lane.
 #include <algorithm>
 
 #include "common.cuh"
 #include "gqa_internal.h"
+#include "ragged.cuh"
 
 namespace gqa {
 namespace evict {
@@ -23,7 +26,10 @@ constexpr int kD = 128;
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMoveWarps = 8;
-constexpr int kRowsPerWarp = 4;
+constexpr int kRowsPerWarp = 16;           // of a step, in two batches
+constexpr int kBins = 2048;
+static_assert(2 * kThreads == kBins, "two bins a thread");
+constexpr int kUnroll = 8;                  // loads in flight a thread
 constexpr int kCachedKeys = 48 * 1024;      // keys of up to so many slots stay in shared memory
 constexpr int kMaxCapacity = 1 << 20;       // slots of a sequence (kept bits in shared memory)
 
@@ -39,7 +45,7 @@ struct Params {
   float* acc_out;
   int32_t *pos_out, *lens_out;
   int32_t *src, *dst, *count;  // workspace: [B * Hkv][budget] twice, [B * Hkv]
-  int Hkv, capacity, max_pages, page_size, num_pages, budget, recent, sink, cached, max_moves;
+  int Hkv, capacity, max_pages, page_size, num_pages, budget, recent, sink, cached, page_shift;
 };
 
 // Order-preserving key: larger weight, larger key; NaN below every number, -0 equals +0,
@@ -53,7 +59,7 @@ __device__ __forceinline__ uint32_t key_of(float w, bool held) {
 
 __global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
   extern __shared__ uint32_t smem[];
-  __shared__ int hist[256];
+  __shared__ int hist[kBins];
   __shared__ int counts[2][kWarps];
   __shared__ int chosen[2];
   const int bh = blockIdx.x, b = bh / p.Hkv;
@@ -78,59 +84,61 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
       for (int i = tid; i < n; i += kThreads) pos_out[i] = pos[i];
     return;
   }
-  uint32_t* bits = smem;                              // kept slots, [ceil(capacity / 32)]
-  uint32_t* keys = smem + (p.capacity + 31) / 32;     // [capacity] when cached
+  uint32_t* bits = smem;                           // kept slots, [ceil(capacity / 32)]
+  uint32_t* keys = smem + (p.capacity + 31) / 32;  // [capacity] when cached
   const long long recent_from = static_cast<long long>(__ldg(p.next_pos + b)) - p.recent;
-  auto make_key = [&](int i) {
-    const int q = pos[i];
-    return key_of(acc[i], q < p.sink || q >= recent_from);
-  };
+  auto make_key = [&](float w, int q) { return key_of(w, q < p.sink || q >= recent_from); };
   if (p.cached) {
-    for (int i = tid; i < n; i += kThreads) keys[i] = make_key(i);
+    for (int i0 = tid; i0 < n; i0 += kUnroll * kThreads) {
+      float w[kUnroll];
+      int q[kUnroll];
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) {
+        const int i = i0 + k * kThreads;
+        w[k] = i < n ? acc[i] : 0.0f;
+        q[k] = i < n ? pos[i] : 0;
+      }
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k)
+        if (i0 + k * kThreads < n) keys[i0 + k * kThreads] = make_key(w[k], q[k]);
+    }
   }
-  auto key_at = [&](int i) { return p.cached ? keys[i] : make_key(i); };
+  auto key_at = [&](int i) { return p.cached ? keys[i] : make_key(acc[i], pos[i]); };
 
   // ---- the budget-th largest key, and how many of its equals are kept
   uint32_t prefix = 0, mask = 0;
   int need = p.budget;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kThreads) hist[i] = 0;
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t digits = pass == 2 ? 1023u : 2047u;
+    for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
     __syncthreads();
-    for (int i0 = warp * 32; i0 < n; i0 += kThreads) {
-      const int i = i0 + lane;
-      const uint32_t k = i < n ? key_at(i) : 0u;
-      const bool in = i < n && (k & mask) == prefix;
-      // one add per distinct digit of the warp: weights crowd into few exponents
-      const uint32_t digit = in ? (k >> shift) & 255u : 256u;
-      const uint32_t peers = __match_any_sync(0xffffffffu, digit);
-      if (in && lane == __ffs(peers) - 1) atomicAdd(&hist[digit], __popc(peers));
+#pragma unroll 4
+    for (int i = tid; i < n; i += kThreads) {
+      const uint32_t k = key_at(i);
+      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & digits], 1);
     }
     __syncthreads();
-    if (warp == 0) {  // lane l holds digits [255 - 8l - 7, 255 - 8l], largest first
-      int mine[8], sum = 0;
+    // thread t holds bins 2047 - 2t and 2046 - 2t, largest first: a scan over the block
+    const int a = hist[kBins - 1 - 2 * tid], c = hist[kBins - 2 - 2 * tid];
+    int above = a + c;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum += mine[j] = hist[255 - 8 * lane - j];
-      int above = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, above, o);
-        if (lane >= o) above += x;
-      }
-      above -= sum;
-      if (above < need && above + sum >= need) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (above < need && above + mine[j] >= need) {
-            chosen[0] = 255 - 8 * lane - j;
-            chosen[1] = need - above;
-          }
-          above += mine[j];
-        }
-      }
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, above, o);
+      if (lane >= o) above += x;
+    }
+    if (lane == 31) counts[0][warp] = above;
+    __syncthreads();
+    above += __reduce_add_sync(0xffffffffu, lane < warp ? counts[0][lane] : 0) - a - c;
+    if (above < need && above + a + c >= need) {
+      const bool first = above + a >= need;
+      chosen[0] = kBins - 1 - 2 * tid - (first ? 0 : 1);
+      chosen[1] = need - above - (first ? 0 : a);
     }
     __syncthreads();
     prefix |= static_cast<uint32_t>(chosen[0]) << shift;
-    mask |= 255u << shift;
+    mask |= digits << shift;
     need = chosen[1];
   }
 
@@ -179,54 +187,93 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
     if ((is_mover >> lane) & 1u) src[mover + __popc(is_mover & below)] = i;
     hole += __popc(is_hole);
     mover += __popc(is_mover);
-    if (i < left && keep) {
-      if (acc_out != acc) acc_out[i] = acc[i];
-      if (pos_out != pos) pos_out[i] = pos[i];
-    }
   }
   int total = 0;
   for (int w = 0; w < kWarps; ++w) total += counts[0][w];
   if (tid == 0) p.count[bh] = total;
+  // what stays keeps its place
+  if (acc_out != acc || pos_out != pos) {
+    for (int i0 = tid; i0 < left; i0 += kUnroll * kThreads) {
+      float w[kUnroll];
+      int q[kUnroll];
+      bool keep[kUnroll];
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) {
+        const int i = i0 + k * kThreads;
+        keep[k] = i < left && ((bits[i >> 5] >> (i & 31)) & 1u);
+        w[k] = keep[k] ? acc[i] : 0.0f;
+        q[k] = keep[k] ? pos[i] : 0;
+      }
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) {
+        const int i = i0 + k * kThreads;
+        if (keep[k] && acc_out != acc) acc_out[i] = w[k];
+        if (keep[k] && pos_out != pos) pos_out[i] = q[k];
+      }
+    }
+  }
   __syncthreads();  // the lists are complete
-  for (int i = tid; i < total; i += kThreads) {
-    const int s = src[i], d = dst[i];
-    acc_out[d] = acc[s];
-    pos_out[d] = pos[s];
+  for (int i0 = tid; i0 < total; i0 += kUnroll * kThreads) {
+    int from[kUnroll], to[kUnroll], q[kUnroll];
+    float w[kUnroll];
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {
+      const int i = i0 + k * kThreads;
+      from[k] = i < total ? src[i] : -1;
+      to[k] = i < total ? dst[i] : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {
+      w[k] = from[k] >= 0 ? acc[from[k]] : 0.0f;
+      q[k] = from[k] >= 0 ? pos[from[k]] : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k)
+      if (from[k] >= 0) {
+        acc_out[to[k]] = w[k];
+        pos_out[to[k]] = q[k];
+      }
   }
 }
 
 __global__ void __launch_bounds__(kMoveWarps * 32) move_kernel(const Params p) {
+  cudaGridDependencySynchronize();  // launched while the selection drains
   const int bh = blockIdx.y, b = bh / p.Hkv, h = bh % p.Hkv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int count = p.count[bh];
   const int32_t* src = p.src + static_cast<size_t>(bh) * p.budget;
   const int32_t* dst = p.dst + static_cast<size_t>(bh) * p.budget;
-  uint16_t* pool = lane < 16 ? p.kp : p.vp;
-  auto row_of = [&](int slot) -> long long {
-    const int page = __ldg(p.table + static_cast<long long>(b) * p.max_pages + slot / p.page_size);
-    if (page < 0 || page >= p.num_pages) {
-      record_input_error(SITE_BAD_PAGE);
-      return -1;
-    }
-    return ((static_cast<long long>(page) * p.Hkv + h) * p.page_size + slot % p.page_size) * kD + (lane & 15) * 8;
-  };
+  uint16_t* pool = (lane < 16 ? p.kp : p.vp) + (lane & 15) * 8;
+  const int32_t* table = p.table + static_cast<long long>(b) * p.max_pages;
+  const int32_t* list = lane < 16 ? src : dst;
   for (int i0 = (blockIdx.x * kMoveWarps + warp) * kRowsPerWarp; i0 < count;
        i0 += gridDim.x * kMoveWarps * kRowsPerWarp) {
-    uint4 v[kRowsPerWarp];
-    long long to[kRowsPerWarp];
+    // lane j: the pool row that move j reads, lane 16 + j: the one it writes; -1 for none
+    long long row = -1;
+    if (i0 + (lane & 15) < count) {
+      const int slot = list[i0 + (lane & 15)];
+      const int lp = p.page_shift >= 0 ? slot >> p.page_shift : slot / p.page_size;
+      const int page = __ldg(table + lp);
+      if (page < 0 || page >= p.num_pages)
+        record_input_error(SITE_BAD_PAGE);
+      else
+        row = (static_cast<long long>(page) * p.Hkv + h) * p.page_size + (slot - lp * p.page_size);
+    }
+    if (__shfl_xor_sync(0xffffffffu, row < 0 ? 1 : 0, 16)) row = -1;  // both ends or none
 #pragma unroll
-    for (int j = 0; j < kRowsPerWarp; ++j) {
-      to[j] = -1;
-      if (i0 + j < count) {
-        const long long from = row_of(src[i0 + j]);
-        to[j] = row_of(dst[i0 + j]);
-        if (from < 0) to[j] = -1;
-        if (to[j] >= 0) v[j] = *reinterpret_cast<const uint4*>(pool + from);
+    for (int j0 = 0; j0 < kRowsPerWarp; j0 += 8) {
+      uint4 v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const long long from = __shfl_sync(0xffffffffu, row, j0 + j);
+        if (from >= 0) v[j] = *reinterpret_cast<const uint4*>(pool + from * kD);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const long long to = __shfl_sync(0xffffffffu, row, 16 + j0 + j);
+        if (to >= 0) *reinterpret_cast<uint4*>(pool + to * kD) = v[j];
       }
     }
-#pragma unroll
-    for (int j = 0; j < kRowsPerWarp; ++j)
-      if (to[j] >= 0) *reinterpret_cast<uint4*>(pool + to[j]) = v[j];
   }
 }
 
@@ -295,6 +342,7 @@ extern "C" int gqa_kv_evict_bf16(void* kpages, void* vpages, const int32_t* bloc
   p.recent = recent;
   p.sink = sink;
   p.cached = capacity <= kCachedKeys ? 1 : 0;
+  p.page_shift = ragged::whole_log2(page_size);
   const int smem = static_cast<int>((capacity + 31) / 32 + (p.cached ? capacity : 0)) * 4;
   static std::atomic<uint64_t> attr_done{0};
   int rc;
@@ -306,9 +354,10 @@ extern "C" int gqa_kv_evict_bf16(void* kpages, void* vpages, const int32_t* bloc
   if (moves > 0) {
     const long long per_block = kMoveWarps * kRowsPerWarp;
     const long long want = (moves + per_block - 1) / per_block;
-    const long long cap = std::max<long long>(1, 148 * 32 / (static_cast<long long>(B) * Hkv));
-    move_kernel<<<dim3(static_cast<unsigned>(std::min(want, cap)), B * Hkv), kMoveWarps * 32, 0, stream>>>(p);
-    if (cudaGetLastError() != cudaSuccess) return GQA_ERR_CUDA;
+    const long long cap = std::max<long long>(1, 148 * 16 / (static_cast<long long>(B) * Hkv));
+    if ((rc = launch_after(move_kernel, dim3(static_cast<unsigned>(std::min(want, cap)), B * Hkv), kMoveWarps * 32, stream,
+                           p)) != GQA_OK)
+      return rc;
   }
   if (lens_out == lens) {
     shorten_kernel<<<(B + 255) / 256, 256, 0, stream>>>(lens_out, B, p.capacity, budget);

@@ -43,6 +43,22 @@ int ensure_smem_attr(F func, int bytes, std::atomic<uint64_t>& done_mask) {
   return GQA_OK;
 }
 
+// Launch a kernel that may start while the one before it on the stream drains; it waits for
+// that one itself (cudaGridDependencySynchronize).
+template <typename P>
+int launch_after(void (*kernel)(const P), dim3 grid, int threads, cudaStream_t stream, const P& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
+}
+
 // Per-file device error words (see GQA_ERROR_FLAG_ACCESSOR): value, optionally cleared.
 int error_flag_stages(bool clear);
 int error_flag_prefill(bool clear);

@@ -36,13 +36,14 @@ __global__ void __launch_bounds__(256) table_kernel(const double* inv_freq, floa
   sin_t[i] = static_cast<float>(s * mscale);
 }
 
-// E values of type T as 32-bit floats, read and written as one vector (16 bytes) or singly.
+// E values of type T, read and written as one vector (16 bytes) or singly; kept as they
+// were read until they are used.
 template <typename T, int E>
 struct Vec;
 template <>
 struct Vec<uint16_t, 8> {
-  static __device__ __forceinline__ void ld(const uint16_t* p, float (&f)[8]) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
+  using Raw = uint4;
+  static __device__ __forceinline__ void unpack(const Raw& v, float (&f)[8]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -50,83 +51,99 @@ struct Vec<uint16_t, 8> {
       f[2 * i + 1] = bf16_hi(w[i]);
     }
   }
-  static __device__ __forceinline__ void st(uint16_t* p, const float (&f)[8]) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
-                                              pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+  static __device__ __forceinline__ Raw pack(const float (&f)[8]) {
+    return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
   }
 };
 template <>
 struct Vec<float, 4> {
-  static __device__ __forceinline__ void ld(const float* p, float (&f)[4]) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
+  using Raw = float4;
+  static __device__ __forceinline__ void unpack(const Raw& v, float (&f)[4]) {
     f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
   }
-  static __device__ __forceinline__ void st(float* p, const float (&f)[4]) {
-    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-  }
+  static __device__ __forceinline__ Raw pack(const float (&f)[4]) { return make_float4(f[0], f[1], f[2], f[3]); }
 };
 template <>
 struct Vec<uint16_t, 1> {
-  static __device__ __forceinline__ void ld(const uint16_t* p, float (&f)[1]) { f[0] = bf2f_bits(*p); }
-  static __device__ __forceinline__ void st(uint16_t* p, const float (&f)[1]) { *p = f2bf_bits(f[0]); }
+  using Raw = uint16_t;
+  static __device__ __forceinline__ void unpack(const Raw& v, float (&f)[1]) { f[0] = bf2f_bits(v); }
+  static __device__ __forceinline__ Raw pack(const float (&f)[1]) { return f2bf_bits(f[0]); }
 };
 template <>
 struct Vec<float, 1> {
-  static __device__ __forceinline__ void ld(const float* p, float (&f)[1]) { f[0] = *p; }
-  static __device__ __forceinline__ void st(float* p, const float (&f)[1]) { *p = f[0]; }
+  using Raw = float;
+  static __device__ __forceinline__ void unpack(const Raw& v, float (&f)[1]) { f[0] = v; }
+  static __device__ __forceinline__ Raw pack(const float (&f)[1]) { return f[0]; }
+};
+template <typename T, int E>
+__device__ __forceinline__ typename Vec<T, E>::Raw ld(const T* p) {
+  return *reinterpret_cast<const typename Vec<T, E>::Raw*>(p);
+}
+template <typename T, int E>
+__device__ __forceinline__ void st(T* p, const typename Vec<T, E>::Raw& v) {
+  *reinterpret_cast<typename Vec<T, E>::Raw*>(p) = v;
+}
+
+// A head row is cut into chunks of vectors E values long (16 bytes, or single values where
+// sizes or alignment do not allow more): first the rotated ones, then those that pass
+// through.  In the half layout a rotated chunk is two vectors, rot/2 apart, with E table
+// entries; in the interleaved one it is a vector of E/2 pairs with E/2 entries (two single
+// values where E is 1).
+struct Shape {
+  int half, n_pairs, n_chunks;  // rot/2, rotated chunks, all chunks
 };
 
-// Table entries [i0, i0 + E) of one row.
-template <int E>
-__device__ __forceinline__ void ld_table(const float* row, int i0, float (&f)[E]) {
-  if constexpr (E == 1) {
-    f[0] = __ldg(row + i0);
-  } else {
+template <int E, bool IL>
+struct Chunk {
+  static constexpr bool kTwo = !IL || E == 1;   // two vectors
+  static constexpr int kEntries = kTwo ? E : E / 2;
+  int a, b, entry;  // vectors' offsets (b < 0: one), first table entry (-1: passes through)
+  __device__ __forceinline__ Chunk(const Shape& s, int c) {
+    entry = c < s.n_pairs ? c * kEntries : -1;
+    if (entry < 0) {
+      a = 2 * s.half + (c - s.n_pairs) * E;
+      b = -1;
+    } else {
+      a = IL ? (E == 1 ? 2 * c : c * E) : c * E;
+      b = !kTwo ? -1 : IL ? a + 1 : a + s.half;
+    }
+  }
+};
+
+// Table entries [i0, i0 + N) of one row.
+template <int N>
+__device__ __forceinline__ void ld_table(const float* row, int i0, float (&f)[N]) {
+  if constexpr (N % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < E; i += 4) {
+    for (int i = 0; i < N; i += 4) {
       const float4 v = __ldg(reinterpret_cast<const float4*>(row + i0 + i));
       f[i] = v.x, f[i + 1] = v.y, f[i + 2] = v.z, f[i + 3] = v.w;
     }
+  } else if constexpr (N == 2) {
+    const float2 v = __ldg(reinterpret_cast<const float2*>(row + i0));
+    f[0] = v.x, f[1] = v.y;
+  } else {
+    f[0] = __ldg(row + i0);
   }
 }
 
-// A head row is cut into chunks: rot/2/E of E pairs each, then (head_dim - rot)/E of E
-// values that pass through.  Chunk c of pairs holds table entries [cE, cE + E): two
-// vectors E values long, rot/2 apart (half layout) or side by side (interleaved).
-struct Shape {
-  int half, n_pairs, n_chunks;  // rot/2, chunks of pairs, all chunks
-};
-
+// Rotate a chunk: vectors a and (where there are two) b.
 template <typename T, int E, bool IL>
-__device__ __forceinline__ void chunk_addr(const Shape& s, int c, int& a, int& b) {
-  if (c < s.n_pairs) {
-    a = IL ? 2 * c * E : c * E;
-    b = IL ? a + E : a + s.half;
-  } else {
-    a = 2 * s.half + (c - s.n_pairs) * E;
-    b = -1;
-  }
-}
-
-template <int E, bool IL>
-__device__ __forceinline__ void rotate(float (&u)[E], float (&w)[E], const float (&c)[E], const float (&s)[E]) {
-  if constexpr (!IL || E == 1) {
+__device__ __forceinline__ void rotate(typename Vec<T, E>::Raw& ra, typename Vec<T, E>::Raw& rb,
+                                       const float (&c)[Chunk<E, IL>::kEntries], const float (&s)[Chunk<E, IL>::kEntries]) {
+  float u[E], w[E];
+  Vec<T, E>::unpack(ra, u);
+  if constexpr (Chunk<E, IL>::kTwo) Vec<T, E>::unpack(rb, w);
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const float a = u[i], b = w[i];
-      u[i] = fmaf(a, c[i], -(b * s[i]));
-      w[i] = fmaf(b, c[i], a * s[i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      float(&v)[E] = i < E / 2 ? u : w;
-      const int k = 2 * (i % (E / 2));
-      const float a = v[k], b = v[k + 1];
-      v[k] = fmaf(a, c[i], -(b * s[i]));
-      v[k + 1] = fmaf(b, c[i], a * s[i]);
-    }
+  for (int i = 0; i < Chunk<E, IL>::kEntries; ++i) {
+    float& x = Chunk<E, IL>::kTwo ? u[i] : u[(2 * i) % E];
+    float& y = Chunk<E, IL>::kTwo ? w[i] : u[(2 * i + 1) % E];
+    const float a = x, b = y;
+    x = fmaf(a, c[i], -(b * s[i]));
+    y = fmaf(b, c[i], a * s[i]);
   }
+  ra = Vec<T, E>::pack(u);
+  if constexpr (Chunk<E, IL>::kTwo) rb = Vec<T, E>::pack(w);
 }
 
 template <typename T>
@@ -143,45 +160,57 @@ struct Params {
 };
 
 // Block (chunks, heads, tokens); a thread keeps its chunk's table entries over its heads.
+// Bound by memory: the first kAhead heads are on their way before the position is known.
+constexpr int kAhead = 4;
 template <typename T, int E, bool IL>
 __global__ void __launch_bounds__(512) rope_kernel(const Params<T> p) {
-  const int c = threadIdx.x;
+  using C = Chunk<E, IL>;
   const long long t = static_cast<long long>(blockIdx.x) * blockDim.z + threadIdx.z;
   if (t >= p.T_) return;
-  const int pos = __ldg(p.positions + t);
-  if (pos < 0 || pos >= p.rows) {
-    if (c == 0 && threadIdx.y == 0) record_input_error(SITE_POSITION);
-    return;
-  }
-  int a, b;
-  chunk_addr<T, E, IL>(p.s, c, a, b);
-  float cs[E], sn[E];
-  if (b >= 0) {
-    ld_table<E>(p.cos + static_cast<size_t>(pos) * p.s.half, c * E, cs);
-    ld_table<E>(p.sin + static_cast<size_t>(pos) * p.s.half, c * E, sn);
-#pragma unroll
-    for (int i = 0; i < E; ++i) sn[i] *= p.sign;
-  }
+  const C ch(p.s, threadIdx.x);
   const T* x = p.x + t * p.x_t;
   T* y = p.y + t * p.y_t;
-#pragma unroll 4
-  for (int h = threadIdx.y; h < p.H; h += blockDim.y) {
-    const T* xr = x + h * p.x_h;
-    T* yr = y + h * p.y_h;
-    float u[E], w[E];
-    Vec<T, E>::ld(xr + a, u);
-    if (b >= 0) {
-      Vec<T, E>::ld(xr + b, w);
-      rotate<E, IL>(u, w, cs, sn);
-      Vec<T, E>::st(yr + b, w);
+  typename Vec<T, E>::Raw u[kAhead], w[kAhead];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int h = h0 + k * blockDim.y;
+      if (h < p.H) {
+        u[k] = ld<T, E>(x + h * p.x_h + ch.a);
+        if (C::kTwo && ch.b >= 0) w[k] = ld<T, E>(x + h * p.x_h + ch.b);
+      }
     }
-    Vec<T, E>::st(yr + a, u);
+  };
+  load(threadIdx.y);
+  const int pos = __ldg(p.positions + t);
+  if (pos < 0 || pos >= p.rows) {
+    if (threadIdx.x == 0 && threadIdx.y == 0) record_input_error(SITE_POSITION);
+    return;
+  }
+  float cs[C::kEntries], sn[C::kEntries];
+  if (ch.entry >= 0) {
+    ld_table<C::kEntries>(p.cos + static_cast<size_t>(pos) * p.s.half, ch.entry, cs);
+    ld_table<C::kEntries>(p.sin + static_cast<size_t>(pos) * p.s.half, ch.entry, sn);
+#pragma unroll
+    for (int i = 0; i < C::kEntries; ++i) sn[i] *= p.sign;
+  }
+  for (int h0 = threadIdx.y; h0 < p.H; h0 += kAhead * blockDim.y) {
+    if (h0 != static_cast<int>(threadIdx.y)) load(h0);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int h = h0 + k * blockDim.y;
+      if (h < p.H) {
+        if (ch.entry >= 0) rotate<T, E, IL>(u[k], w[k], cs, sn);
+        st<T, E>(y + h * p.y_h + ch.a, u[k]);
+        if (C::kTwo && ch.b >= 0) st<T, E>(y + h * p.y_h + ch.b, w[k]);
+      }
+    }
   }
 }
 
 // ------------------------------------------------------------------ ragged paged append
 constexpr int kD = 128;
-constexpr int kMaxTokens = 16;  // tokens of one block
+constexpr int kMaxTokens = 4;  // tokens of one block
 
 struct ExtendParams {
   const uint16_t *k, *v, *q;
@@ -245,44 +274,56 @@ __global__ void __launch_bounds__(512) extend_kernel(const ExtendParams p) {
     tok[tid] = k;
   }
   __syncthreads();
-  int a, b;
-  chunk_addr<uint16_t, E, IL>(p.s, threadIdx.x, a, b);
+  using C = Chunk<E, IL>;
+  const C ch(p.s, threadIdx.x);
   const int n_rows = p.Hq + 2 * p.Hkv;
   const long long capacity = static_cast<long long>(p.max_pages) * p.page_size;
-#pragma unroll 2
-  for (int w = threadIdx.y; w < n_tok * n_rows; w += blockDim.y) {
-    const int i = w / n_rows, r = w - i * n_rows;
-    const Token k = tok[i];
-    if (k.page_row < 0) continue;
-    const long long t = t0 + i;
-    const uint16_t* src;
-    uint16_t* dst;
-    bool turn = b >= 0;
-    if (r < p.Hq) {
-      src = p.q + t * p.q_t + r * p.q_h;
-      dst = p.q_out + t * p.o_t + r * p.o_h;
-    } else if (r < p.Hq + p.Hkv) {
-      const int h = r - p.Hq;
-      src = p.k + t * p.k_t + h * p.k_h;
-      dst = p.kp + (k.page_row + static_cast<long long>(h) * p.page_size) * kD;
-      if (p.slot_pos && threadIdx.x == 0) p.slot_pos[k.pos_at + h * capacity] = k.pos;
-    } else {
-      const int h = r - p.Hq - p.Hkv;
-      src = p.v + t * p.v_t + h * p.v_h;
-      dst = p.vp + (k.page_row + static_cast<long long>(h) * p.page_size) * kD;
-      turn = false;
+  // kAhead rows at a time, their loads on the way together
+  for (int w0 = threadIdx.y; w0 < n_tok * n_rows; w0 += kAhead * blockDim.y) {
+    typename Vec<uint16_t, E>::Raw u[kAhead], x[kAhead];
+    uint16_t* dst[kAhead];
+    int pos[kAhead];  // -1: not rotated
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      dst[k] = nullptr;
+      pos[k] = -1;
+      const int w = w0 + k * blockDim.y;
+      if (w >= n_tok * n_rows) continue;
+      const int i = w / n_rows, r = w - i * n_rows;
+      const Token tk = tok[i];
+      if (tk.page_row < 0) continue;
+      const long long t = t0 + i;
+      const uint16_t* src;
+      if (r < p.Hq) {
+        src = p.q + t * p.q_t + r * p.q_h;
+        dst[k] = p.q_out + t * p.o_t + r * p.o_h;
+        pos[k] = tk.pos;
+      } else if (r < p.Hq + p.Hkv) {
+        const int h = r - p.Hq;
+        src = p.k + t * p.k_t + h * p.k_h;
+        dst[k] = p.kp + (tk.page_row + static_cast<long long>(h) * p.page_size) * kD;
+        pos[k] = tk.pos;
+        if (p.slot_pos && threadIdx.x == 0) p.slot_pos[tk.pos_at + h * capacity] = tk.pos;
+      } else {
+        const int h = r - p.Hq - p.Hkv;
+        src = p.v + t * p.v_t + h * p.v_h;
+        dst[k] = p.vp + (tk.page_row + static_cast<long long>(h) * p.page_size) * kD;
+      }
+      u[k] = ld<uint16_t, E>(src + ch.a);
+      if (C::kTwo && ch.b >= 0) x[k] = ld<uint16_t, E>(src + ch.b);
     }
-    float u[E], x[E];
-    Vec<uint16_t, E>::ld(src + a, u);
-    if (b >= 0) Vec<uint16_t, E>::ld(src + b, x);
-    if (turn) {
-      float cs[E], sn[E];
-      ld_table<E>(p.cos + static_cast<size_t>(k.pos) * p.s.half, threadIdx.x * E, cs);
-      ld_table<E>(p.sin + static_cast<size_t>(k.pos) * p.s.half, threadIdx.x * E, sn);
-      rotate<E, IL>(u, x, cs, sn);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (!dst[k]) continue;
+      if (pos[k] >= 0 && ch.entry >= 0) {
+        float cs[C::kEntries], sn[C::kEntries];
+        ld_table<C::kEntries>(p.cos + static_cast<size_t>(pos[k]) * p.s.half, ch.entry, cs);
+        ld_table<C::kEntries>(p.sin + static_cast<size_t>(pos[k]) * p.s.half, ch.entry, sn);
+        rotate<uint16_t, E, IL>(u[k], x[k], cs, sn);
+      }
+      st<uint16_t, E>(dst[k] + ch.a, u[k]);
+      if (C::kTwo && ch.b >= 0) st<uint16_t, E>(dst[k] + ch.b, x[k]);
     }
-    Vec<uint16_t, E>::st(dst + a, u);
-    if (b >= 0) Vec<uint16_t, E>::st(dst + b, x);
   }
 }
 
@@ -290,13 +331,14 @@ inline bool vec_ok(const void* ptr, int esize, long long st, long long sh, int h
   return aligned16(ptr) && (st * esize) % 16 == 0 && (heads == 1 || (sh * esize) % 16 == 0);
 }
 
-inline Shape shape_of(int head_dim, int rot, int E) {
-  return Shape{rot / 2, rot / 2 / E, rot / 2 / E + (head_dim - rot) / E};
+inline Shape shape_of(int head_dim, int rot, int E, bool il) {
+  const int pairs = il && E > 1 ? rot / E : rot / 2 / E;
+  return Shape{rot / 2, pairs, pairs + (head_dim - rot) / E};
 }
 
 template <typename T, int E>
 int launch(Params<T> p, int head_dim, int rot, bool il, cudaStream_t stream) {
-  p.s = shape_of(head_dim, rot, E);
+  p.s = shape_of(head_dim, rot, E, il);
   // About 256 threads a block: enough of them on an SM to cover the loads' latency.
   const int nc = p.s.n_chunks;
   const int hy = std::max(1, std::min(p.H, 256 / nc));
@@ -339,7 +381,7 @@ int run(const void* x, void* y, const int32_t* positions, const float* cos, cons
   p.rows = rows;
   p.sign = (flags & GQA_FLAG_INVERSE) ? -1.0f : 1.0f;
   const bool il = (flags & GQA_FLAG_INTERLEAVED) != 0;
-  const bool vec = (rot / 2) % E == 0 && head_dim % E == 0 && vec_ok(x, sizeof(T), x_t, x_h, H) &&
+  const bool vec = (il ? rot : rot / 2) % E == 0 && head_dim % E == 0 && vec_ok(x, sizeof(T), x_t, x_h, H) &&
                    vec_ok(y, sizeof(T), y_t, y_h, H) && aligned16(cos) && aligned16(sin);
   return vec ? launch<T, E>(p, head_dim, rot, il, stream) : launch<T, 1>(p, head_dim, rot, il, stream);
 }
@@ -431,19 +473,21 @@ extern "C" int gqa_kv_extend_bf16(const void* k, const void* v, long long k_toke
   p.q_t = q_token_stride, p.q_h = q_head_stride, p.o_t = q_out_token_stride, p.o_h = q_out_head_stride;
   p.B = B, p.T = T, p.Hq = Hq, p.Hkv = Hkv;
   p.max_pages = max_pages_per_seq, p.page_size = page_size, p.num_pages = num_pages, p.rows = table_rows;
-  const bool vec = rot_dim % 16 == 0 && vec_ok(k, 2, k_token_stride, k_head_stride, Hkv) &&
+  const bool vec = rot_dim % ((flags & GQA_FLAG_INTERLEAVED) ? 8 : 16) == 0 && vec_ok(k, 2, k_token_stride, k_head_stride, Hkv) &&
                    vec_ok(v, 2, v_token_stride, v_head_stride, Hkv) &&
                    (!q || (vec_ok(q, 2, q_token_stride, q_head_stride, Hq) &&
                            vec_ok(q_out, 2, q_out_token_stride, q_out_head_stride, Hq))) &&
                    aligned16(cos) && aligned16(sin);
-  p.s = shape_of(kD, rot_dim, vec ? 8 : 1);
-  // Few tokens: one a block, a thread for each chunk, so that one load's latency is all.
-  // Many: several a block share the search for their sequences.
-  const int n_rows = Hq + 2 * Hkv;
-  p.tokens = T <= 512 ? 1 : (T <= 4096 ? 4 : 8);
-  const dim3 block(p.s.n_chunks, std::max(1, std::min(n_rows, 512 / p.s.n_chunks)));
-  const unsigned grid = static_cast<unsigned>((T + p.tokens - 1) / p.tokens);
   const bool il = (flags & GQA_FLAG_INTERLEAVED) != 0;
+  p.s = shape_of(kD, rot_dim, vec ? 8 : 1, il);
+  // Few tokens: one a block, a thread for every chunk, so that one load's latency is all
+  // (64 tokens: 3.6 us, 4.1 with small blocks).  Many: small blocks of four tokens, of which
+  // some look up their slots while others move rows (8192 tokens: 36.8 us, 44.2 with large
+  // blocks of eight).
+  const int n_rows = Hq + 2 * Hkv;
+  p.tokens = T <= 512 ? 1 : 4;
+  const dim3 block(p.s.n_chunks, std::max(1, std::min(n_rows, (T <= 512 ? 512 : 128) / p.s.n_chunks)));
+  const unsigned grid = static_cast<unsigned>((T + p.tokens - 1) / p.tokens);
   if (vec && il)
     extend_kernel<8, true><<<grid, block, 0, stream>>>(p);
   else if (vec)

@@ -552,14 +552,5 @@ extern "C" int gqa_attn_weight_sums_f32(const void* q, long long q_token_stride,
   weights_kernel<<<grid, kThreads, kSmemBytes, stream>>>(tmQ, tmK, p);
   if (cudaGetLastError() != cudaSuccess) return GQA_ERR_CUDA;
   // The merge starts while the first kernel drains and waits for it on the device.
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kBlock);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, merge_kernel, static_cast<const Params>(p)) == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
+  return launch_after(merge_kernel, dim3(grid), kBlock, stream, p);
 }
