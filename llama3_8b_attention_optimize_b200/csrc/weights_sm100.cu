@@ -14,7 +14,9 @@
 // the order of every sum is fixed: runs repeat bit for bit.
 //
 // Unit of work: (sequence, kv head, block of 256 slots), two 128-slot K tiles side by side
-// that share the query tiles (128 rows: G heads of 128 / G tokens) it walks as steps; the
+// that share the query tiles (128 rows: G heads of 128 / G tokens) it walks as steps.  Where
+// a sequence brings at most 64 rows, a block has 512 slots, two steps of 256 with one query
+// tile: a unit's beginning and end cost as much as loading 256 slots takes.  The
 // steps of all units are cut into equal parts, one per CTA and SM (ragged.cuh).  Parts of
 // one unit leave 256 sums each, which a second kernel adds in order.
 //
@@ -101,27 +103,30 @@ struct Params {
   float* part;  // [2 * grid][kBlock]
   Desc* desc;   // [grid]
   int G, Hq, causal, tpt, box;
+  int wide_n;  // most tokens of a sequence with blocks of 512 slots (64 rows)
   float scale_log2;
 };
 
-// Units: blocks of 256 slots.  Steps: the query tiles of which some row sees the block; one
-// (empty) step where the sequence brings no tokens, to pass its sums on.
+// Units: blocks of 256 slots.  Steps: the query tiles of which some row sees the block.  Wide
+// units (of 512 slots) are one step; sequences without tokens have such too, to pass their sums on.
 struct Line {
   static constexpr int extra = 1;  // a unit's beginning and end cost about a query tile
-  int tpt, causal;
-  __device__ __forceinline__ Line(const Params& p) : tpt(p.tpt), causal(p.causal) {}
+  int tpt, causal, wide_n;
+  __device__ __forceinline__ Line(const Params& p) : tpt(p.tpt), causal(p.causal), wide_n(p.wide_n) {}
+  __device__ __forceinline__ bool wide(const Seq& s) const { return s.n <= wide_n; }
+  __device__ __forceinline__ int block(const Seq& s) const { return wide(s) ? 2 * kBlock : kBlock; }
   __device__ __forceinline__ bool has(const Seq& s) const { return s.L > 0; }
-  __device__ __forceinline__ int units(const Seq& s) const { return (s.L + kBlock - 1) / kBlock; }
-  __device__ __forceinline__ bool ends(const Seq& s, int u) const { return (u + 1) * kBlock >= s.L; }
-  __device__ __forceinline__ int tiles(const Seq& s) const { return s.n <= tpt ? 1 : (s.n + tpt - 1) / tpt; }  // n > 0
+  __device__ __forceinline__ int units(const Seq& s) const { return (s.L + block(s) - 1) / block(s); }
+  __device__ __forceinline__ bool ends(const Seq& s, int u) const { return (u + 1) * block(s) >= s.L; }
+  __device__ __forceinline__ int tiles(const Seq& s) const { return (s.n + tpt - 1) / tpt; }
   // first query tile that sees slot kBlock * u: floor((kBlock u - (L - n)) / tpt), at least 0
   __device__ __forceinline__ int first(const Seq& s, int u) const {
     const int x = u * kBlock - (s.L - s.n);
-    return !causal || x < tpt ? 0 : x / tpt;
+    return !causal || x < tpt || wide(s) ? 0 : x / tpt;
   }
-  __device__ __forceinline__ int count(const Seq& s, int u) const { return s.n == 0 ? 1 : tiles(s) - first(s, u); }
+  __device__ __forceinline__ int count(const Seq& s, int u) const { return wide(s) ? 1 : tiles(s) - first(s, u); }
   __device__ __forceinline__ uint32_t before(const Seq& s, int k) const {
-    if (s.n == 0) return k * (1 + extra);
+    if (wide(s)) return k * (1 + extra);
     uint32_t sum = static_cast<uint32_t>(k) * (tiles(s) + extra);
     const int base = s.L - s.n;
     const int u1 = base > 0 ? (base + kBlock - 1) / kBlock : 0;  // first unit past the old slots
@@ -238,47 +243,59 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     uint32_t g = 0, m = 0;  // query tiles and K tiles loaded
     const Boxes boxes(p.box, lane);
+    auto load_q = [&](int head, int tok) {
+      const int st = static_cast<int>(g % kQStages);
+      if (g >= kQStages)
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(B_QEMPTY + st), (g / kQStages - 1) & 1u, SITE_PRODUCER));
+      if (!ok) return;
+      if (lane == 0) {
+        mbar_expect_tx(bar(B_QFULL + st), 2 * 128 * p.G * p.tpt);
+        for (int e = 0; e < 2; ++e)
+          tma_load_4d(sbase + kOffQ + st * kTileBytes + e * kHalf, &tmQ, bar(B_QFULL + st), 64 * e, head, tok, 0);
+      }
+      ++g;
+    };
     // the next unit with tokens and its pages, looked up a unit ahead
-    int page[2] = {-1, -1};
+    int page[4] = {-1, -1, -1, -1}, tiles = 0;
     auto advance = [&]() -> bool {
       do {
         if (!ragged::next_part(p.batch, line, walk, s)) return false;
       } while (s.s.n == 0);
       const int32_t* table = p.batch.table + static_cast<size_t>(s.b) * p.batch.max_pages;
+      tiles = line.block(s.s) / 128;
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) page[kt] = boxes.page(p.batch, table, s.u * kBlock + 128 * kt, s.s.L);
+      for (int i = 0; i < 4; ++i)
+        if (i < tiles) page[i] = boxes.page(p.batch, table, s.u * 128 * tiles + 128 * i, s.s.L);
       return true;
     };
     bool more = advance();
     while (ok && more) {
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
+      for (int i = 0; i < 4; ++i) {
+        if (!ok || i >= tiles) continue;
         const int st = static_cast<int>(m % kKStages);
-        const int row = boxes.row(p.batch, page[kt], s.h, s.u * kBlock + 128 * kt, s.s.L, SITE_BAD_PAGE);
-        if (ok && m >= kKStages)
+        const int row = boxes.row(p.batch, page[i], s.h, s.u * 128 * tiles + 128 * i, s.s.L, SITE_BAD_PAGE);
+        if (m >= kKStages)
           ok = __all_sync(0xffffffffu, mbar_wait(bar(B_KEMPTY + st), (m / kKStages - 1) & 1u, SITE_PRODUCER));
-        if (!ok) break;
+        if (!ok) continue;
         const uint32_t mine = __ballot_sync(0xffffffffu, row >= 0);
         if (lane == 0) mbar_expect_tx(bar(B_KFULL + st), __popc(mine) * p.box * 128);
         __syncwarp();
         if (row >= 0)
           tma_load_3d(sbase + kOffK + st * kTileBytes + boxes.offset, &tmK, bar(B_KFULL + st), boxes.half * 64, row, 0);
         ++m;
+        if (i == 0 && tiles == 4) load_q(s.h * p.G, s.s.a);  // its one query tile, ahead of most of K
       }
       if (!ok) break;
+      if (tiles == 4) {
+        more = advance();  // while the loads are under way
+        continue;
+      }
       const int steps = s.k1 - s.k0, head = s.h * p.G;
       int tok = s.s.a + (line.first(s.s, s.u) + s.k0) * p.tpt;
-      more = advance();
-      for (int k = 0; k < steps; ++k, ++g, tok += p.tpt) {
-        const int st = static_cast<int>(g % kQStages);
-        if (g >= kQStages)
-          ok = __all_sync(0xffffffffu, mbar_wait(bar(B_QEMPTY + st), (g / kQStages - 1) & 1u, SITE_PRODUCER));
-        if (!ok) break;
-        if (lane == 0) {
-          mbar_expect_tx(bar(B_QFULL + st), 2 * 128 * p.G * p.tpt);
-          for (int e = 0; e < 2; ++e)
-            tma_load_4d(sbase + kOffQ + st * kTileBytes + e * kHalf, &tmQ, bar(B_QFULL + st), 64 * e, head, tok, 0);
-        }
+      for (int k = 0; ok && k < steps; ++k, tok += p.tpt) {
+        load_q(head, tok);
+        if (k == 0) more = advance();
       }
     }
     // Drain: every load this warp issued must land before the CTA may exit.
@@ -296,22 +313,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t q_lo = sdesc_lo(sbase + kOffQ, 16);
       constexpr uint32_t kTile16 = kTileBytes / 16;
       bool ok = true;
-      uint32_t g = 0, m = kt;  // query tiles, and the K tile
+      uint32_t g = 0, qn = 0, m = kt;  // steps, query tiles, and the K tile
       while (ok && ragged::next_part(p.batch, line, walk, s)) {
         if (s.s.n == 0) continue;
-        const int ks = static_cast<int>(m % kKStages);
-        const uint32_t a0 = k_lo + ks * kTile16;
-        ok = mbar_wait_spin(bar(B_KFULL + ks), (m / kKStages) & 1u, SITE_MMA);
-        const int first = line.first(s.s, s.u);
-        for (int k = s.k0; ok && k < s.k1; ++k, ++g) {
-          const int st = static_cast<int>(g % kQStages), bb = static_cast<int>(g & 1);
-          ok = mbar_wait_spin(bar(B_QFULL + st), (g / kQStages) & 1u, SITE_MMA) &&
-               (g < 2 || mbar_wait_spin(bar(B_SFREE + 2 * kt + bb), (g / 2 - 1) & 1u, SITE_MMA));
+        const bool wide = line.wide(s.s);
+        const int first = line.first(s.s, s.u) + s.k0, steps = wide ? 2 : s.k1 - s.k0;
+        for (int k = 0; ok && k < steps; ++k, ++g) {
+          const int ks = static_cast<int>(m % kKStages), st = static_cast<int>(qn % kQStages), bb = static_cast<int>(g & 1);
+          const bool k_first = wide || k == 0, k_last = wide || k + 1 == steps;  // of the K tile, of the query tile
+          const bool q_first = !wide || k == 0, q_last = !wide || k + 1 == steps;
+          if (k_first) ok = mbar_wait_spin(bar(B_KFULL + ks), (m / kKStages) & 1u, SITE_MMA);
+          if (ok && q_first) ok = mbar_wait_spin(bar(B_QFULL + st), (qn / kQStages) & 1u, SITE_MMA);
+          if (ok && g >= 2) ok = mbar_wait_spin(bar(B_SFREE + 2 * kt + bb), (g / 2 - 1) & 1u, SITE_MMA);
           if (!ok) break;
           // only as many columns as the tile has rows, in the MMA's steps of 16
-          const int nv = min(p.tpt, s.s.n - (first + k) * p.tpt) * p.G;
+          const int nv = (wide ? s.s.n : min(p.tpt, s.s.n - (first + k) * p.tpt)) * p.G;
           const uint32_t id = idesc_bf16_f32(128, (nv + 15) / 16 * 16, false);
-          const uint32_t b0 = q_lo + st * kTile16;
+          const uint32_t a0 = k_lo + ks * kTile16, b0 = q_lo + st * kTile16;
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk) {
@@ -319,10 +337,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             umma_ss_lohi(tmem + 256 * kt + 128 * bb, a0 + off, b0 + off, kHi, id, kk > 0 ? 1u : 0u);
           }
           umma_commit(bar(B_SFULL + 2 * kt + bb));
-          umma_commit(bar(B_QEMPTY + st));
-          if (k + 1 == s.k1) umma_commit(bar(B_KEMPTY + ks));
+          if (q_last) {
+            umma_commit(bar(B_QEMPTY + st));
+            ++qn;
+          }
+          if (k_last) {
+            umma_commit(bar(B_KEMPTY + ks));
+            m += 2;
+          }
         }
-        m += 2;
       }
       umma_commit(bar(B_DRAIN + kt));
       mbar_wait_drain(bar(B_DRAIN + kt), 0, SITE_DRAIN);
@@ -340,9 +363,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     while (ok && ragged::next_part(p.batch, line, walk, s)) {
       if (s.s.n == 0) continue;
-      const int first = line.first(s.s, s.u);
-      for (int k = s.k0; ok && k < s.k1; ++k, ++g) {
-        const int t0 = (first + k) * p.tpt, bb = static_cast<int>(g & 1);
+      const bool wide = line.wide(s.s);
+      const int first = line.first(s.s, s.u) + s.k0, steps = wide ? 2 : s.k1 - s.k0;
+      for (int k = 0; ok && k < steps; ++k, ++g) {
+        const int t0 = wide ? 0 : (first + k) * p.tpt, bb = static_cast<int>(g & 1);
         float nl[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -365,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int kt = warp >> 3;          // K tile
     const int ch = (warp >> 2) & 1;    // rows [64 ch, 64 ch + 64) of each query tile
     const int r = (warp & 3) * 32 + lane;  // slot in the K tile == TMEM lane
-    const uint32_t tS = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + 256 * kt + 64 * ch;
+    const uint32_t tS = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + 256 * kt;
     const float* lse = reinterpret_cast<const float*>(smem + kOffLse);
     const uint8_t* tok = smem + kOffTok;
     float* xsum = reinterpret_cast<float*>(smem + kOffSum) + 128 * kt;
@@ -374,10 +398,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t g = 0;
     // A slot's old sum, read a unit ahead: its latency is as long as a unit of a
     // single-token batch.
-    auto slot_of = [&](const Part& x) -> int { return x.u * kBlock + 128 * kt + r; };
+    auto slot_of = [&](const Part& x) -> int {
+      return line.wide(x.s) ? (2 * x.u + ch) * kBlock + 128 * kt + r : x.u * kBlock + 128 * kt + r;
+    };
     auto old_of = [&](const Part& x) -> float {
       const int slot = slot_of(x);
-      if (ch != 0 || slot >= x.s.L - x.s.n || !x.whole()) return 0.0f;
+      if ((ch != 0 && !line.wide(x.s)) || slot >= x.s.L - x.s.n || !x.whole()) return 0.0f;
       return __ldg(p.acc + (static_cast<size_t>(x.b) * p.batch.Hkv + x.h) * p.batch.capacity + slot);
     };
     Part ahead;
@@ -388,14 +414,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       more = ragged::next_part(p.batch, line, walk, ahead);
       const float old_ahead = more ? old_of(ahead) : 0.0f;
       const int slot = slot_of(s);
-      const int warp_last = min(s.s.L, s.u * kBlock + 128 * kt + (warp & 3) * 32 + 32) - 1;
+      const int warp_last = min(s.s.L, slot - lane + 32) - 1;
+      const bool wide = line.wide(s.s);
+      const int half = wide ? 0 : 64 * ch;  // first row of this warp's
+
       float sum = 0.0f;
       if (s.s.n > 0) {
-        const int first = line.first(s.s, s.u);
-        for (int k = s.k0; k < s.k1; ++k, ++g) {
+        const int first = line.first(s.s, s.u) + s.k0, steps = wide ? 2 : s.k1 - s.k0;
+        for (int k = 0; k < steps; ++k, ++g) {
           const int bb = static_cast<int>(g & 1);
-          const int t0 = (first + k) * p.tpt;
-          const int nv = min(64, min(p.tpt, s.s.n - t0) * p.G - 64 * ch);  // rows of this half
+          const int t0 = wide ? 0 : (first + k) * p.tpt;
+          // rows of this warp: half of the tile's, or in a wide unit's step all or none
+          const int nv = wide && k != ch ? 0 : min(64, min(p.tpt, s.s.n - t0) * p.G - half);
           // the tile's first token sees slots up to see0, each next token one more
           const int see0 = p.causal ? s.s.L - s.s.n + t0 : s.s.L - 1;
           if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_SFULL + 2 * kt + bb), (g / 2) & 1u, SITE_SOFTMAX));
@@ -404,30 +434,30 @@ __global__ void __launch_bounds__(kThreads, 1)
           const bool all = see0 >= warp_last;
           const int from = p.causal ? slot - see0 : 0;  // a row of a token below this does not see the slot
           float2 a0 = make_float2(0.f, 0.f), a1 = make_float2(0.f, 0.f);
-          const uint32_t tv = tS + 128 * bb;
-          const float* nl = lse + 128 * bb + 64 * ch;
+          const uint32_t tv = tS + 128 * bb + half;
+          const float* nl = lse + 128 * bb + half;
           tc_fence_after();
           if (nv > 8) {
             uint32_t v[32];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const int left = nv - 32 * half;
+            for (int c = 0; c < 2; ++c) {
+              const int left = nv - 32 * c;
               if (left > 0) {
-                tmem_ld32(tv + 32 * half, v);
+                tmem_ld32(tv + 32 * c, v);
                 tmem_wait_ld_dep(v);
               }
-              if (half == 1) {
+              if (c == 1) {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(B_SFREE + 2 * kt + bb));
               }
               if (all && left >= 32)
-                add_all(v, nl + 32 * half, sl2, a0, a1);
+                add_all(v, nl + 32 * c, sl2, a0, a1);
               else if (left > 0)
-                add_masked(v, nl + 32 * half, tok + 64 * ch + 32 * half, left, from, p.scale_log2, a0);
+                add_masked(v, nl + 32 * c, tok + half + 32 * c, left, from, p.scale_log2, a0);
             }
           } else {
-            add_some(tv, nl, tok + 64 * ch, nv, from, p.scale_log2, a0);
+            add_some(tv, nl, tok + half, nv, from, p.scale_log2, a0);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(B_SFREE + 2 * kt + bb));
@@ -437,11 +467,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) mbar_arrive(bar(B_LEMPTY + bb));
         }
       }
-      named_bar_sync(3 + kt, 256);  // the previous unit's exchange has been read
-      if (ch == 1) xsum[r] = sum;
-      named_bar_sync(1 + kt, 256);
-      if (ok && ch == 0 && slot < s.s.L) {
-        sum += xsum[r];
+      if (!wide) {
+        named_bar_sync(3 + kt, 256);  // the previous unit's exchange has been read
+        if (ch == 1) xsum[r] = sum;
+        named_bar_sync(1 + kt, 256);
+        if (ch == 0) sum += xsum[r];
+      }
+      if (ok && (wide || ch == 0) && slot < s.s.L) {
         if (s.whole())
           p.acc_out[(static_cast<size_t>(s.b) * p.batch.Hkv + s.h) * p.batch.capacity + slot] = old + sum;
         else
@@ -532,6 +564,7 @@ extern "C" int gqa_attn_weight_sums_f32(const void* q, long long q_token_stride,
   p.Hq = Hq;
   p.causal = (flags & GQA_FLAG_CAUSAL) != 0;
   p.tpt = 128 / G;
+  p.wide_n = 64 / G;
   p.box = std::min(128, page_size & -page_size);
   p.scale_log2 = scale * kLog2e;
 
