@@ -68,8 +68,9 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 constexpr int kBlockRows = 16;             // rows of a block of the few-row form; a unit has one or two
 // What one K/V tile costs in each form, for dealing out the CTAs: a tile of the few form is
-// 64 KB from memory, one of the many form two tiles' softmax.
-constexpr int kCostFew = 3, kCostMany = 5;
+// 64 KB from memory (1.3 us), one of the many form two tiles' softmax (2.3 to 3.0 us).  A mixed
+// step took 113 us with 3 : 5, 104 with 4 : 9, 107 with 2 : 5.
+constexpr int kCostFew = 4, kCostMany = 9;
 // and what a unit's beginning and end cost, in tiles.
 constexpr int kExtraFew = 1, kExtraMany = 2;
 
@@ -602,9 +603,9 @@ __device__ __forceinline__ void softmax_many(const Params& p, uint8_t* smem, uin
         float2 sum = make_float2(0.f, 0.f), sumf = make_float2(0.f, 0.f);
         uint32_t row = prow;
         asm volatile("" : "+r"(row));  // keeps the chunks' addresses from living across the loop
-        // Chunks with no masked entry may evaluate part of the exponentials on the FMA
-        // pipe; its cubic is good to 7.5e-5, enough for a weight that is rounded to
-        // bf16 but not for the log-sum-exp.
+        // Chunks with no masked entry may evaluate part of the exponentials on the FMA pipe.
+        // Its cubic is good to 7.5e-5, enough for a weight that is rounded to bf16 but not
+        // for the log-sum-exp (where a quintic measured no faster than none).
         if (rel >= 63) {
           exp_chunk_store<!kLse, kLse>(s0, row, 0, sc2, nm2, sum, sumf);
           exp_chunk_store<!kLse, kLse>(s1, row, 4, sc2, nm2, sum, sumf);
