@@ -308,6 +308,17 @@ int gqa_kv_evict_bf16(void* kpages, void* vpages, const int32_t* block_table, in
                       size_t workspace_bytes, int B, int Hkv, int head_dim, int budget, int recent, int sink,
                       gqa_stream_t stream);
 
+/* The calls above with their arguments in one array: pointers and integers as int64 in the
+ * order of the declaration (scale and stream apart), for bindings whose cost grows with the
+ * number of arguments.  n must be the entry's count. */
+#define GQA_PACKED_ROPE_POSITIONS_BF16 0
+#define GQA_PACKED_ROPE_POSITIONS_F32 1
+#define GQA_PACKED_KV_EXTEND_BF16 2
+#define GQA_PACKED_ATTEND_CHUNK_BF16 3
+#define GQA_PACKED_ATTN_WEIGHT_SUMS_F32 4
+#define GQA_PACKED_KV_EVICT_BF16 5
+int gqa_packed_call(int entry, const int64_t* args, int n, float scale, gqa_stream_t stream);
+
 /* ---------------------------------------------------------------- projections
  * The full layer's linear maps (golden run_full_attention,
  * llama3_attention_golden_model.py:149-151 and :193-194): y = x W^T with W in the

@@ -30,6 +30,10 @@ GQA_FLAG_INVERSE = 16
 GQA_MASK_NEG_INF_BF16 = 0xFF80
 GQA_GEMM_OUT_F32 = 1
 
+# entries of gqa_packed_call and their numbers of packed arguments
+PACKED = {"gqa_rope_positions_bf16": (0, 15), "gqa_rope_positions_f32": (1, 15), "gqa_kv_extend_bf16": (2, 32),
+          "gqa_attend_chunk_bf16": (3, 24), "gqa_attn_weight_sums_f32": (4, 21), "gqa_kv_evict_bf16": (5, 21)}
+
 # (name, restype, argtypes) for every symbol include/gqa_b200.h declares.
 _vp, _i, _f, _d, _ll, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_double, ctypes.c_longlong, ctypes.c_size_t
 SIGNATURES = {
@@ -67,6 +71,7 @@ SIGNATURES = {
                                  [_f, _i, _vp]),
     "gqa_kv_evict_workspace_size": (_sz, [_i, _i, _i]),
     "gqa_kv_evict_bf16": (_i, [_vp] * 3 + [_i] * 3 + [_vp] * 8 + [_sz] + [_i] * 6 + [_vp]),
+    "gqa_packed_call": (_i, [_i, ctypes.c_char_p, _i, _f, _vp]),
     "gqa_gemm_bf16": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "gqa_qkv_proj_bf16": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "gqa_o_proj_bf16": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),

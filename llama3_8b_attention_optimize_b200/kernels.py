@@ -7,6 +7,7 @@ optional leading batch axis.  Raises ``GqaError`` on any non-zero status.
 from __future__ import annotations
 
 import math
+import struct
 
 import torch
 
@@ -353,14 +354,19 @@ def _index(t: torch.Tensor, name: str) -> int:
     return t.get_device()
 
 
-def _call(dev: int, name: str, *args) -> None:
-    """Enqueue one C entry point on the current torch stream of device index `dev`."""
-    fn = getattr(_lib.load(), name)
+_packers = {name: (entry, n, struct.Struct(f"{n}q").pack) for name, (entry, n) in _lib.PACKED.items()}
+
+
+def _call(dev: int, name: str, scale: float, *args: int) -> None:
+    """Enqueue one entry point of ``gqa_packed_call`` on the current torch stream of device
+    index `dev` (ctypes converts some 30 arguments in 4 us, one packed array in 1)."""
+    entry, n, pack = _packers[name]
+    fn = _lib.load().gqa_packed_call
     if torch._C._cuda_getDevice() == dev:
-        rc = fn(*args, _raw_stream(dev))
+        rc = fn(entry, pack(*args), n, scale, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, _raw_stream(dev))
+            rc = fn(entry, pack(*args), n, scale, _raw_stream(dev))
     if rc != 0:
         check(rc, name)
 
@@ -433,7 +439,9 @@ def rope_table(rows: int, rot_dim: int = HEAD_DIM, theta: float = ROPE_THETA, po
     inv = inv.to(device)
     cos = torch.empty(rows, rot_dim // 2, dtype=torch.float32, device=device)
     sin = torch.empty_like(cos)
-    _call(cos.get_device(), "gqa_rope_table_f32", _ptr(inv), _ptr(cos), _ptr(sin), rows, rot_dim // 2, pos0, mscale)
+    with torch.cuda.device(cos.device):
+        check(_lib.load().gqa_rope_table_f32(_ptr(inv), _ptr(cos), _ptr(sin), rows, rot_dim // 2, pos0, mscale,
+                                             _stream(cos.device)), "gqa_rope_table_f32")
     return cos, sin
 
 
@@ -459,7 +467,7 @@ def rope_positions(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, 
     if out.shape != x.shape:
         raise ValueError("out must have x's shape")
     rows, half = cos.shape
-    _call(dev, "gqa_rope_positions_bf16" if x.dtype is _BF16 else "gqa_rope_positions_f32", x.data_ptr(), out.data_ptr(),
+    _call(dev, "gqa_rope_positions_bf16" if x.dtype is _BF16 else "gqa_rope_positions_f32", 0.0, x.data_ptr(), out.data_ptr(),
           positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), T, H, d, 2 * half, rows, x.stride(0), x.stride(1),
           out.stride(0), out.stride(1), (GQA_FLAG_INTERLEAVED if interleaved else 0) | (GQA_FLAG_INVERSE if inverse else 0))
     return out
@@ -521,11 +529,11 @@ def kv_extend(k: torch.Tensor, v: torch.Tensor, kpages: torch.Tensor, vpages: to
         Hq, q_t, q_h, o_t, o_h = q.shape[1], q.stride(0), q.stride(1), q_out.stride(0), q_out.stride(1)
     if slot_pos is not None and slot_pos.shape != (B, Hkv, max_pages * page_size):
         raise ValueError("slot_pos must be [B, Hkv, max_pages * page_size]")
-    _call(dev, "gqa_kv_extend_bf16", k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+    _call(dev, "gqa_kv_extend_bf16", 0.0, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
           kpages.data_ptr(), vpages.data_ptr(), block_table.data_ptr(), max_pages, page_size, num_pages, q_start.data_ptr(),
-          lens.data_ptr(), None if positions is None else positions.data_ptr(), None if cos is None else cos.data_ptr(),
-          None if sin is None else sin.data_ptr(), rows, 2 * half, None if q is None else q.data_ptr(), q_t, q_h,
-          None if q is None else q_out.data_ptr(), o_t, o_h, None if slot_pos is None else slot_pos.data_ptr(), B, T, Hq,
+          lens.data_ptr(), 0 if positions is None else positions.data_ptr(), 0 if cos is None else cos.data_ptr(),
+          0 if sin is None else sin.data_ptr(), rows, 2 * half, 0 if q is None else q.data_ptr(), q_t, q_h,
+          0 if q is None else q_out.data_ptr(), o_t, o_h, 0 if slot_pos is None else slot_pos.data_ptr(), B, T, Hq,
           Hkv, HEAD_DIM, GQA_FLAG_INTERLEAVED if interleaved else 0)
     return q_out
 
@@ -559,11 +567,10 @@ def attend_chunk(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, bl
         raise ValueError("lse must be [T, Hq]")
     q = _no_broadcast(q)
     workspace = _workspace(workspace, attend_chunk_workspace_bytes(T, Hq, Hkv), dev)
-    _call(dev, "gqa_attend_chunk_bf16", q.data_ptr(), q.stride(0), q.stride(1), kpages.data_ptr(), vpages.data_ptr(),
+    _call(dev, "gqa_attend_chunk_bf16", _SCALE if scale is None else scale, q.data_ptr(), q.stride(0), q.stride(1), kpages.data_ptr(), vpages.data_ptr(),
           block_table.data_ptr(), max_pages, page_size, num_pages, q_start.data_ptr(), lens.data_ptr(), out.data_ptr(),
-          out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(), workspace.data_ptr(),
-          workspace.numel() * workspace.element_size(), B, T, Hq, Hkv, d, max_q_len, _SCALE if scale is None else scale,
-          GQA_FLAG_CAUSAL if causal else 0)
+          out.stride(0), out.stride(1), 0 if lse is None else lse.data_ptr(), workspace.data_ptr(),
+          workspace.numel() * workspace.element_size(), B, T, Hq, Hkv, d, max_q_len, GQA_FLAG_CAUSAL if causal else 0)
     return out
 
 
@@ -598,10 +605,10 @@ def attn_weight_sums(q: torch.Tensor, kpages: torch.Tensor, block_table: torch.T
         raise ValueError("acc and acc_out must be [B, Hkv, max_pages * page_size]")
     q = _no_broadcast(q)
     workspace = _workspace(workspace, attn_weight_sums_workspace_bytes(), dev)
-    _call(dev, "gqa_attn_weight_sums_f32", q.data_ptr(), q.stride(0), q.stride(1), kpages.data_ptr(), block_table.data_ptr(),
+    _call(dev, "gqa_attn_weight_sums_f32", _SCALE if scale is None else scale, q.data_ptr(), q.stride(0), q.stride(1), kpages.data_ptr(), block_table.data_ptr(),
           max_pages, page_size, num_pages, q_start.data_ptr(), lens.data_ptr(), lse.data_ptr(), acc.data_ptr(),
           acc_out.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(), B, T, Hq, Hkv, d,
-          _SCALE if scale is None else scale, GQA_FLAG_CAUSAL if causal else 0)
+          GQA_FLAG_CAUSAL if causal else 0)
     return acc_out
 
 
@@ -633,7 +640,7 @@ def kv_evict(kpages: torch.Tensor, vpages: torch.Tensor, block_table: torch.Tens
     if next_pos.shape != (B,) or lens_out.shape != (B,):
         raise ValueError("next_pos and lens_out must be [B]")
     workspace = _workspace(workspace, kv_evict_workspace_bytes(B, Hkv, budget), dev)
-    _call(dev, "gqa_kv_evict_bf16", kpages.data_ptr(), vpages.data_ptr(), block_table.data_ptr(), max_pages, page_size,
+    _call(dev, "gqa_kv_evict_bf16", 0.0, kpages.data_ptr(), vpages.data_ptr(), block_table.data_ptr(), max_pages, page_size,
           num_pages, lens.data_ptr(), lens_out.data_ptr(), acc.data_ptr(), acc_out.data_ptr(), slot_pos.data_ptr(),
           slot_pos_out.data_ptr(), next_pos.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
           B, Hkv, HEAD_DIM, budget, recent, sink)

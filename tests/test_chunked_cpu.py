@@ -120,6 +120,25 @@ def test_evict_validates_on_the_host(lib):
     assert call(ws_bytes=16) == E.GQA_ERR_WORKSPACE
 
 
+def test_packed_calls_match_their_declarations(lib):
+    """Packed argument counts are those of the ctypes signatures without scale and stream;
+    other counts, entries and integers too wide for their argument are refused."""
+    import struct
+    for name, (entry, n) in E.PACKED.items():
+        args = E.SIGNATURES[name][1]
+        assert n == sum(1 for a in args if a is not ctypes.c_float) - 1
+        for count in (n - 1, n + 1, 0):
+            assert lib.gqa_packed_call(entry, struct.pack(f"{n}q", *[0] * n), count, 0.1, None) == E.GQA_ERR_INVALID_ARGUMENT
+        assert lib.gqa_packed_call(entry, struct.pack(f"{n}q", *[0] * n), n, 0.1, None) == E.GQA_ERR_INVALID_ARGUMENT
+    entry, n = E.PACKED["gqa_rope_positions_bf16"]
+    good = [0x1000] * 5 + [0, 2, 128, 64, 8, 256, 128, 256, 128, 0]  # T = 0: nothing to do
+    assert lib.gqa_packed_call(entry, struct.pack(f"{n}q", *good), n, 0.0, None) == E.GQA_OK
+    good[5] = 1 << 32
+    assert lib.gqa_packed_call(entry, struct.pack(f"{n}q", *good), n, 0.0, None) == E.GQA_ERR_INVALID_ARGUMENT
+    assert lib.gqa_packed_call(99, struct.pack("1q", 0), 1, 0.0, None) == E.GQA_ERR_INVALID_ARGUMENT
+    assert lib.gqa_packed_call(0, None, 15, 0.0, None) == E.GQA_ERR_INVALID_ARGUMENT
+
+
 def test_scaled_frequencies():
     base, m = kernels.rope_inv_freq(128)
     assert m == 1.0 and base[0] == 1.0 and torch.allclose(base, 500000.0 ** (-torch.arange(64).double() / 64))
