@@ -256,3 +256,141 @@ class PagedKVCache:
         """q [B, Hq, 128] (before RoPE) at positions q_pos (int32 [B]) over the cached tokens."""
         return kernels.decode_paged(q, self.k, self.v, self.table, self.lens, q_pos=q_pos, cos=self.cos,
                                     sin=self.sin, workspace=self.ws, split_len=self.split_len, out=out)
+
+
+class ChunkedKVCache:
+    """Paged K/V cache served chunk by chunk: every step brings each sequence any number of
+    new tokens (a prompt's chunk, one token, none), and a cache that outgrows a budget keeps
+    its heaviest slots.
+
+    ``step`` rotates the new queries and keys at their positions and appends keys and values
+    (``gqa_kv_extend_bf16``), attends (``gqa_attend_chunk_bf16``) and, with ``track_weights``,
+    adds up what attention each slot received (``gqa_attn_weight_sums_f32``).  ``evict`` cuts
+    every sequence to a budget of slots (``gqa_kv_evict_bf16``) and returns the pages that fall
+    free.  Positions run on across evictions: a sequence's next token stands at
+    ``next_pos(b)``, however few slots are left.
+
+    Pools ``k``/``v`` are [num_pages, Hkv, page_size, 128] bf16; ``lens`` int32 [B] counts each
+    sequence's slots; ``acc`` float32 and ``slot_pos`` int32 [B, Hkv, capacity] hold each
+    slot's weight and token position.  Block tables and a free list are kept on the host.
+    ``rope`` is passed to ``kernels.rope_table`` (``scaling``, ``factor``, ...).
+    """
+
+    def __init__(self, B: int, num_pages: int, max_pages_per_seq: int, Hkv: int = 8, Hq: int = 32, page_size: int = 64,
+                 *, max_positions: int | None = None, rot_dim: int = 128, interleaved: bool = False,
+                 track_weights: bool = True, theta: float = kernels.ROPE_THETA, rope: dict | None = None, device=None):
+        if page_size <= 0 or page_size % 16:
+            raise ValueError("page_size must be a multiple of 16")
+        if Hq % Hkv:
+            raise ValueError("Hq must be a multiple of Hkv")
+        self.device = torch.device(device or "cuda")
+        self.B, self.Hkv, self.Hq, self.page_size = B, Hkv, Hq, page_size
+        self.max_pages, self.capacity = max_pages_per_seq, max_pages_per_seq * page_size
+        self.interleaved = interleaved
+        self.max_positions = self.capacity if max_positions is None else max_positions
+        shape = (num_pages, Hkv, page_size, kernels.HEAD_DIM)
+        # rows past a sequence's length are never read, so the pools need no clearing
+        self.k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+        self.v = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+        self.table = torch.full((B, max_pages_per_seq), -1, dtype=torch.int32, device=self.device)
+        self.lens = torch.zeros(B, dtype=torch.int32, device=self.device)
+        per_slot = (B, Hkv, self.capacity)
+        self.acc = torch.zeros(per_slot, dtype=torch.float32, device=self.device) if track_weights else None
+        self.slot_pos = torch.zeros(per_slot, dtype=torch.int32, device=self.device) if track_weights else None
+        self.cos, self.sin = kernels.rope_table(self.max_positions, rot_dim, theta, device=self.device, **(rope or {}))
+        self._table_h = [[-1] * max_pages_per_seq for _ in range(B)]
+        self._lens_h, self._pos_h = [0] * B, [0] * B
+        self._free = list(range(num_pages - 1, -1, -1))
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def seq_len(self, b: int) -> int:
+        """Slots that sequence b holds."""
+        return self._lens_h[b]
+
+    def next_pos(self, b: int) -> int:
+        """The position of sequence b's next token."""
+        return self._pos_h[b]
+
+    def _pages(self, n: int) -> int:
+        return (n + self.page_size - 1) // self.page_size
+
+    def reserve(self, new: list[int]) -> None:
+        """Give sequence b pages for new[b] more tokens (raises, with nothing changed, when they do not fit)."""
+        if len(new) != self.B or any(n < 0 for n in new):
+            raise ValueError("new needs one count per sequence")
+        wanted = []
+        for b, n in enumerate(new):
+            need = self._lens_h[b] + n
+            if need > self.capacity:
+                raise ValueError(f"sequence {b}: {need} tokens exceed the capacity {self.capacity}")
+            if n and self._pos_h[b] + n > self.max_positions:
+                raise ValueError(f"sequence {b}: position {self._pos_h[b] + n - 1} is past the rotary table")
+            wanted += [(b, lp) for lp in range(self._pages(need)) if self._table_h[b][lp] < 0]
+        if len(wanted) > len(self._free):
+            raise RuntimeError("paged KV cache: out of pages")
+        for b, lp in wanted:
+            self._table_h[b][lp] = self._free.pop()
+        if wanted:
+            self.table.copy_(torch.tensor(self._table_h, dtype=torch.int32))
+
+    def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, new: list[int],
+             out: torch.Tensor | None = None) -> torch.Tensor:
+        """One step: q [T, Hq, 128], k, v [T, Hkv, 128] (before rotation, any strides) hold the new
+        tokens of sequence 0, then 1, ...; new[b] of them belong to sequence b.  Returns the
+        attention's output [T, Hq, 128]."""
+        T = sum(new)
+        if q.shape[0] != T or k.shape[0] != T or v.shape[0] != T:
+            raise ValueError("q, k and v must hold sum(new) tokens")
+        self.reserve(new)
+        lens = [a + n for a, n in zip(self._lens_h, new)]
+        # one upload: q_start, the lengths with the new tokens, and the tokens' positions
+        ends = torch.tensor([0, *new], dtype=torch.int32).cumsum(0, dtype=torch.int32)
+        pos = [torch.arange(p, p + n, dtype=torch.int32) for p, n in zip(self._pos_h, new) if n]
+        host = torch.cat([ends, torch.tensor(lens, dtype=torch.int32), *pos])
+        plan = host.pin_memory().to(self.device, non_blocking=True)
+        # slices of their own: 4-byte alignment is all the kernels ask of them
+        q_start, positions = plan[: self.B + 1], plan[2 * self.B + 1:]
+        self.lens.copy_(plan[self.B + 1: 2 * self.B + 1])
+        q_rot = kernels.kv_extend(k, v, self.k, self.v, self.table, q_start, self.lens, positions, self.cos, self.sin, q=q,
+                                  interleaved=self.interleaved, slot_pos=self.slot_pos)
+        longest = max(new) if new else 0
+        lse = None if self.acc is None else torch.empty(T, self.Hq, dtype=torch.float32, device=self.device)
+        out = kernels.attend_chunk(q_rot, self.k, self.v, self.table, q_start, self.lens, max_q_len=longest, out=out, lse=lse)
+        if self.acc is not None:
+            kernels.attn_weight_sums(q_rot, self.k, self.table, q_start, self.lens, lse, self.acc, max_q_len=longest)
+        self._lens_h = lens
+        self._pos_h = [p + n for p, n in zip(self._pos_h, new)]
+        return out
+
+    def evict(self, budget: int, *, recent: int = 0, sink: int = 0) -> None:
+        """Cut every sequence to ``budget`` slots per kv head: the first ``sink`` and the last
+        ``recent`` positions, then the slots that received the most attention."""
+        if self.acc is None:
+            raise ValueError("evict needs a cache with track_weights")
+        if budget <= 0 or recent < 0 or sink < 0 or recent + sink > budget:
+            raise ValueError("0 <= sink + recent <= budget and a positive budget are needed")
+        if all(n <= budget for n in self._lens_h):
+            return
+        next_pos = torch.tensor(self._pos_h, dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
+        kernels.kv_evict(self.k, self.v, self.table, self.lens, self.acc, self.slot_pos, next_pos, budget, recent=recent,
+                         sink=sink)
+        for b, n in enumerate(self._lens_h):
+            self._lens_h[b] = min(n, budget)
+            self._give_back(b, self._pages(self._lens_h[b]))
+        self.table.copy_(torch.tensor(self._table_h, dtype=torch.int32))
+
+    def _give_back(self, b: int, first: int) -> None:
+        for lp in range(first, self.max_pages):
+            if self._table_h[b][lp] >= 0:
+                self._free.append(self._table_h[b][lp])
+                self._table_h[b][lp] = -1
+
+    def release(self, b: int) -> None:
+        """Return sequence b's pages to the free list; it starts again at position 0."""
+        self._give_back(b, 0)
+        self._lens_h[b] = self._pos_h[b] = 0
+        self.table[b].fill_(-1)
+        self.lens[b] = 0
