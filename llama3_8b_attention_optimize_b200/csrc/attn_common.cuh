@@ -103,25 +103,5 @@ __device__ __forceinline__ float2 exp2_poly2(float2 x) {
                      __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
 }
 
-// The same with a quintic (relative error 2.4e-7 with its 32-bit evaluation, a near-minimax
-// fit of 2^f made for these kernels): for exponentials that are summed in 32 bits.
-__device__ __forceinline__ float2 exp2_poly2_f32(float2 x) {
-  constexpr float kRound = 12582912.0f;  // 1.5 * 2^23
-  constexpr float c0 = 1.00000012f, c1 = 0.693146944f, c2 = 0.240221202f, c3 = 0.0555071309f, c4 = 0.00967554096f,
-                  c5 = 0.00132764713f;
-  x.x = fmaxf(x.x, -126.0f);
-  x.y = fmaxf(x.y, -126.0f);
-  const float2 t = __fadd2_rn(x, make_float2(kRound, kRound));
-  const float2 n = __fadd2_rn(t, make_float2(-kRound, -kRound));
-  const float2 f = __ffma2_rn(n, make_float2(-1.0f, -1.0f), x);
-  float2 q = __ffma2_rn(make_float2(c5, c5), f, make_float2(c4, c4));
-  q = __ffma2_rn(q, f, make_float2(c3, c3));
-  q = __ffma2_rn(q, f, make_float2(c2, c2));
-  q = __ffma2_rn(q, f, make_float2(c1, c1));
-  q = __ffma2_rn(q, f, make_float2(c0, c0));
-  return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
-}
-
 }  // namespace attn
 }  // namespace gqa

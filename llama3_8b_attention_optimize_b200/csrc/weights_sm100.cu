@@ -28,7 +28,6 @@
 
 #include <algorithm>
 
-#include "attn_common.cuh"
 #include "common.cuh"
 #include "gqa_internal.h"
 #include "ragged.cuh"
@@ -110,7 +109,7 @@ struct Params {
 // Units: blocks of 256 slots.  Steps: the query tiles of which some row sees the block.  Wide
 // units (of 512 slots) are one step; sequences without tokens have such too, to pass their sums on.
 struct Line {
-  static constexpr int extra = 1;  // a unit's beginning and end cost about a query tile
+  static constexpr int extra = 2;  // what a unit's beginning and end cost, in query tiles
   int tpt, causal, wide_n;
   __device__ __forceinline__ Line(const Params& p) : tpt(p.tpt), causal(p.causal), wide_n(p.wide_n) {}
   __device__ __forceinline__ bool wide(const Seq& s) const { return s.n <= wide_n; }
@@ -136,8 +135,8 @@ struct Line {
 };
 
 // p = 2^(s * sl2 + nl) of 32 rows that all see the slot.  The exponentials bound a chunk of
-// many tokens, so kPoly of every 8 pairs go to the FMA pipe.
-constexpr int kPoly = 2;
+// many tokens (a share of them on the FMA pipe, by a quintic, measured 98 to 108 us where
+// this takes 99).
 __device__ __forceinline__ void add_all(const uint32_t (&s)[32], const float* nl, float2 sl2, float2& a0, float2& a1) {
 #pragma unroll
   for (int c = 0; c < 32; c += 4) {
@@ -146,10 +145,7 @@ __device__ __forceinline__ void add_all(const uint32_t (&s)[32], const float* nl
     const float2 y =
         __ffma2_rn(make_float2(__uint_as_float(s[c + 2]), __uint_as_float(s[c + 3])), sl2, make_float2(l.z, l.w));
     a0 = __fadd2_rn(a0, make_float2(ex2_approx(x.x), ex2_approx(x.y)));
-    if ((c / 4) % 4 < kPoly)
-      a1 = __fadd2_rn(a1, attn::exp2_poly2_f32(y));
-    else
-      a1 = __fadd2_rn(a1, make_float2(ex2_approx(y.x), ex2_approx(y.y)));
+    a1 = __fadd2_rn(a1, make_float2(ex2_approx(y.x), ex2_approx(y.y)));
   }
 }
 
@@ -172,7 +168,7 @@ __device__ __forceinline__ void add_masked(const uint32_t (&s)[32], const float*
 }
 
 // The same for a few rows, eight at a time: units of single tokens are so short that the
-// fetching of more code would bound them (213 -> 115 us for 64 tokens).
+// fetching of more code would bound them (163 -> 115 us for 64 tokens when this was written).
 __device__ __forceinline__ void add_some(uint32_t taddr, const float* nl, const uint8_t* tok, int nv, int from, float sl2,
                                          float2& a0) {
 #pragma unroll 1
@@ -544,9 +540,9 @@ extern "C" int gqa_attn_weight_sums_f32(const void* q, long long q_token_stride,
   const int G = Hq / Hkv;
   const long long capacity = static_cast<long long>(max_pages_per_seq) * page_size;
   const long long pool_rows = static_cast<long long>(num_pages) * Hkv * page_size;
-  if (G > 128 || B > kMaxB || capacity > 0x7FFFFE00LL || pool_rows > 0x7FFFFFFFLL) return GQA_ERR_UNSUPPORTED;
+  if (G > 128 || B > kMaxB || capacity > (1LL << 30) || pool_rows > 0x7FFFFFFFLL) return GQA_ERR_UNSUPPORTED;
   // query tiles over all blocks of slots: counted in 32 bits
-  const long long steps = (T + 128 / G - 1) / (128 / G) + 2 * B;
+  const long long steps = (T + 128 / G - 1) / (128 / G) + 3 * B;
   if (static_cast<double>(steps) * Hkv * (capacity / kBlock + 1) >= 2147483648.0) return GQA_ERR_UNSUPPORTED;
   // a TMA dimension needs a stride: heads or tokens that share one row are the caller's to expand
   if ((T > 1 && q_token_stride == 0) || (Hq > 1 && q_head_stride == 0)) return GQA_ERR_UNSUPPORTED;
