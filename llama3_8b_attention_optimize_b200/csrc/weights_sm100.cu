@@ -49,6 +49,11 @@ constexpr int kTileBytes = 128 * 128 * 2;  // K and Q tiles: 32 KB
 constexpr int kHalf = kTileBytes / 2;
 constexpr int kQStages = 2;
 constexpr int kKStages = 5;  // K tiles in flight; tile i of the CTA (two a unit) lies in stage i % 5
+// Tiles land on barriers of their own, i % 10: even tiles are one issuer's and odd ones the
+// other's, so a stage changes hands at each use.  An issuer that waited on a stage's barrier
+// would skip every other phase, and where tile i - 5 is late (loads may land out of order)
+// the parity of the phase before it would pass for tile i's.
+constexpr int kKBars = 2 * kKStages;
 constexpr float kLog2e = 1.4426950408889634f;
 
 constexpr int kSoftmaxWarps = 16;
@@ -60,7 +65,7 @@ constexpr int kThreads = 640;
 constexpr int kOffQ = 0;
 constexpr int kOffK = kOffQ + kQStages * kTileBytes;
 constexpr int kOffBar = kOffK + kKStages * kTileBytes;
-constexpr int kNumBars = 32;
+constexpr int kNumBars = 34;
 constexpr int kOffLse = kOffBar + kNumBars * 8;     // [2][128] -lse * log2(e)
 constexpr int kOffSum = kOffLse + 2 * 128 * 4;      // [K tile][128] sums of the rows' second half
 constexpr int kOffTok = kOffSum + 2 * 128 * 4;      // [128] token of a row in its tile
@@ -74,13 +79,13 @@ static_assert(sizeof(Walk) <= 48, "room for the start");
 enum : int {
   B_QFULL = 0,    // [2]
   B_QEMPTY = 2,   // [2] one arrival per issuer
-  B_KFULL = 4,    // [5]
-  B_KEMPTY = 9,   // [5]
-  B_SFULL = 14,   // [K tile][2]
-  B_SFREE = 18,   // [K tile][2] one arrival per softmax warp
-  B_LFULL = 22,   // [2] lse of a query tile staged
-  B_LEMPTY = 24,  // [2] one arrival per softmax warp
-  B_DRAIN = 26,   // [2]
+  B_KFULL = 4,    // [10]
+  B_KEMPTY = 14,  // [5]
+  B_SFULL = 19,   // [K tile][2]
+  B_SFREE = 23,   // [K tile][2] one arrival per softmax warp
+  B_LFULL = 27,   // [2] lse of a query tile staged
+  B_LEMPTY = 29,  // [2] one arrival per softmax warp
+  B_DRAIN = 31,   // [2]
 };
 
 enum : int {
@@ -94,6 +99,8 @@ enum : int {
   SITE_LENGTH = 0x631,    // lens[b] outside [0, capacity]
   SITE_BAD_PAGE = 0x632,  // block-table entry outside [0, num_pages)
 };
+
+static_assert(B_DRAIN + 2 <= kNumBars && kOffLse % 16 == 0, "barriers, and 16-byte reads behind them");
 
 struct Params {
   ragged::Batch batch;
@@ -202,12 +209,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto bar = [&](int i) -> uint32_t { return sbase + kOffBar + 8 * i; };
 
   if (warp == kWarpHelper) {  // a barrier a lane
-    int count = 1;
-    if (lane >= B_QEMPTY && lane < B_KFULL) count = 2;
-    if (lane >= B_SFREE && lane < B_LFULL) count = 8;
-    if (lane >= B_LFULL && lane < B_LEMPTY) count = 32;
-    if (lane >= B_LEMPTY && lane < B_DRAIN) count = kSoftmaxWarps;
-    if (lane < B_DRAIN + 2) mbar_init(bar(lane), count);
+    for (int i = lane; i < B_DRAIN + 2; i += 32) {
+      int count = 1;
+      if (i >= B_QEMPTY && i < B_KFULL) count = 2;
+      if (i >= B_SFREE && i < B_LFULL) count = 8;
+      if (i >= B_LFULL && i < B_LEMPTY) count = 32;
+      if (i >= B_LEMPTY && i < B_DRAIN) count = kSoftmaxWarps;
+      mbar_init(bar(i), count);
+    }
     fence_mbar_init();
   }
   if (threadIdx.x < 128) smem[kOffTok + threadIdx.x] = static_cast<uint8_t>(threadIdx.x / p.G);
@@ -274,11 +283,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (m >= kKStages)
           ok = __all_sync(0xffffffffu, mbar_wait(bar(B_KEMPTY + st), (m / kKStages - 1) & 1u, SITE_PRODUCER));
         if (!ok) continue;
-        const uint32_t mine = __ballot_sync(0xffffffffu, row >= 0);
-        if (lane == 0) mbar_expect_tx(bar(B_KFULL + st), __popc(mine) * p.box * 128);
+        const uint32_t mine = __ballot_sync(0xffffffffu, row >= 0), full = bar(B_KFULL + static_cast<int>(m % kKBars));
+        if (lane == 0) mbar_expect_tx(full, __popc(mine) * p.box * 128);
         __syncwarp();
         if (row >= 0)
-          tma_load_3d(sbase + kOffK + st * kTileBytes + boxes.offset, &tmK, bar(B_KFULL + st), boxes.half * 64, row, 0);
+          tma_load_3d(sbase + kOffK + st * kTileBytes + boxes.offset, &tmK, full, boxes.half * 64, row, 0);
         ++m;
         if (i == 0 && tiles == 4) load_q(s.h * p.G, s.s.a);  // its one query tile, ahead of most of K
       }
@@ -298,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (uint32_t i = g > kQStages ? g - kQStages : 0u; i < g; ++i)
       mbar_wait_drain(bar(B_QFULL + static_cast<int>(i % kQStages)), (i / kQStages) & 1u, SITE_DRAIN);
     for (uint32_t i = m > kKStages ? m - kKStages : 0u; i < m; ++i)
-      mbar_wait_drain(bar(B_KFULL + static_cast<int>(i % kKStages)), (i / kKStages) & 1u, SITE_DRAIN);
+      mbar_wait_drain(bar(B_KFULL + static_cast<int>(i % kKBars)), (i / kKBars) & 1u, SITE_DRAIN);
     __syncwarp();
   } else if (warp == kWarpMma || warp == kWarpMma + 1) {
     // ------------------------------------------------------------ MMA issuers, one per K tile
@@ -318,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int ks = static_cast<int>(m % kKStages), st = static_cast<int>(qn % kQStages), bb = static_cast<int>(g & 1);
           const bool k_first = wide || k == 0, k_last = wide || k + 1 == steps;  // of the K tile, of the query tile
           const bool q_first = !wide || k == 0, q_last = !wide || k + 1 == steps;
-          if (k_first) ok = mbar_wait_spin(bar(B_KFULL + ks), (m / kKStages) & 1u, SITE_MMA);
+          if (k_first) ok = mbar_wait_spin(bar(B_KFULL + static_cast<int>(m % kKBars)), (m / kKBars) & 1u, SITE_MMA);
           if (ok && q_first) ok = mbar_wait_spin(bar(B_QFULL + st), (qn / kQStages) & 1u, SITE_MMA);
           if (ok && g >= 2) ok = mbar_wait_spin(bar(B_SFREE + 2 * kt + bb), (g / 2 - 1) & 1u, SITE_MMA);
           if (!ok) break;
@@ -542,7 +551,7 @@ extern "C" int gqa_attn_weight_sums_f32(const void* q, long long q_token_stride,
   const long long pool_rows = static_cast<long long>(num_pages) * Hkv * page_size;
   if (G > 128 || B > kMaxB || capacity > (1LL << 30) || pool_rows > 0x7FFFFFFFLL) return GQA_ERR_UNSUPPORTED;
   // query tiles over all blocks of slots: counted in 32 bits
-  const long long steps = (T + 128 / G - 1) / (128 / G) + 3 * B;
+  const long long steps = (static_cast<long long>(T) + 128 / G - 1) / (128 / G) + 3LL * B;
   if (static_cast<double>(steps) * Hkv * (capacity / kBlock + 1) >= 2147483648.0) return GQA_ERR_UNSUPPORTED;
   // a TMA dimension needs a stride: heads or tokens that share one row are the caller's to expand
   if ((T > 1 && q_token_stride == 0) || (Hq > 1 && q_head_stride == 0)) return GQA_ERR_UNSUPPORTED;

@@ -533,6 +533,32 @@ def test_weight_sums_strided_queries_and_streams():
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("new,ctx,causal", [(1, 8191, True), (1, 1500, True), (24, 4000, True), (300, 3000, True),
+                                            (3, 5000, False)])
+def test_busy_memory_changes_no_result(new, ctx, causal):
+    """Loads land late and out of order while DRAM is busy: every call gives the quiet call's bits."""
+    rng = np.random.default_rng(new + ctx)
+    B = 48 if new < 16 else 6
+    lens = [int(rng.integers(max(new, ctx // 32), ctx + 1)) for _ in range(B)]
+    bt = Batch([new] * B, lens, 32, 8, 128, seed=3)
+    lse = torch.empty(bt.T, 32, device="cuda")
+    acc = torch.rand(B, 8, bt.cap, generator=gen(4), device="cuda")
+    traffic = torch.empty(1 << 26, device="cuda")
+    out = bt.attend(causal=causal, lse=lse).clone()
+    sums = kernels.attn_weight_sums(bt.q, bt.kp, bt.table, bt.q_start, bt.lens, lse, acc, causal=causal, acc_out=acc.clone())
+    torch.cuda.synchronize()
+    lse_out = torch.empty_like(lse)
+    for i in range(60):
+        traffic.fill_(i)  # its writes go on in DRAM while the next kernel starts
+        got = bt.attend(causal=causal, lse=lse_out)
+        assert torch.equal(got, out) and torch.equal(lse_out, lse)
+        traffic.fill_(-i)
+        got = kernels.attn_weight_sums(bt.q, bt.kp, bt.table, bt.q_start, bt.lens, lse, acc, causal=causal,
+                                       acc_out=acc.clone())
+        assert torch.equal(got, sums)
+    kernels.device_check()
+
+
 # ------------------------------------------------------------------ eviction
 def evict_ref(bt, acc, slot_pos, next_pos, budget, recent, sink):
     """Plain form on the host: (kp, vp, acc, slot_pos, lens) after the cut."""
