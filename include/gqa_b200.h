@@ -255,8 +255,16 @@ int gqa_decode_paged_bf16(const void* q, const void* kpages, const void* vpages,
  * all of lens[b].  Any Hq that is a multiple of Hkv.  lse (float [T][Hq], may be NULL)
  * receives the natural logarithm of the sum of the exponentials.  A row that sees no slot gives
  * zeros and -inf.  Cache rows past lens[b] may hold anything.  max_q_len is a hint (the
- * longest sequence's number of new tokens; 0 = unknown) that only chooses the tiling.
+ * longest sequence's number of new tokens; 0 = unknown) that only sizes the second
+ * launch's grid: any value gives the same results.  A q_start that descends or leaves
+ * [0, T] writes nothing (GQA_ERR_DEVICE_INPUT), here and in the weight sums.
  * workspace: gqa_attend_chunk_workspace_size bytes, 16-byte aligned.
+ *
+ * The attention and the weight sums take Hq / Hkv <= 128, B <= 8192, a capacity of at most
+ * 2^30 slots a sequence, pools below 2^31 rows (num_pages * Hkv * page_size) and q
+ * strides above 0 where there is more than one token or head; beyond that they return
+ * GQA_ERR_UNSUPPORTED.  Their q (and o) are 16-byte aligned, strides too; the append and
+ * the rotation take any strides and are fastest with such.
  *
  * gqa_attn_weight_sums_f32: acc_out[b, h, j] = (j < lens[b] - n ? acc[b, h, j] : 0) +
  * the sum of exp(q . k_j * scale - lse) over the group's query heads and the tokens that

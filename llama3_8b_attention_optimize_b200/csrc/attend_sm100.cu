@@ -1243,7 +1243,7 @@ extern "C" int gqa_attend_chunk_bf16(const void* q, long long q_token_stride, lo
   const long long pool_rows = static_cast<long long>(num_pages) * Hkv * page_size;
   if (G > 128 || B > kMaxB || capacity > (1LL << 30) || pool_rows > 0x7FFFFFFFLL) return GQA_ERR_UNSUPPORTED;
   // K/V tiles over all units: counted in 32 bits
-  const long long units = (T + 2 * (128 / G) - 1) / (2 * (128 / G)) + std::min(B, T);
+  const long long units = (static_cast<long long>(T) + 2 * (128 / G) - 1) / (2 * (128 / G)) + std::min(B, T);
   if (static_cast<double>(units) * Hkv * (capacity / kBN + 1 + kExtraMany) >= 2147483648.0) return GQA_ERR_UNSUPPORTED;
   // a TMA dimension needs a stride: heads or tokens that share one row are the caller's to expand
   if ((T > 1 && q_token_stride == 0) || (Hq > 1 && q_head_stride == 0)) return GQA_ERR_UNSUPPORTED;

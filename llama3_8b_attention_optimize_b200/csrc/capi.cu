@@ -73,13 +73,13 @@ extern "C" const char* gqa_strerror(int code) {
   switch (code) {
     case GQA_OK: return "ok";
     case GQA_ERR_INVALID_ARGUMENT: return "invalid argument (null pointer, size or flag)";
-    case GQA_ERR_UNSUPPORTED: return "unsupported shape (head_dim must be 128 and Hq = 4*Hkv)";
+    case GQA_ERR_UNSUPPORTED: return "unsupported shape or size (head_dim must be 128; Hq = 4*Hkv, or a multiple of Hkv for the chunked calls; limits in gqa_b200.h)";
     case GQA_ERR_MISALIGNED: return "pointer not 16-byte aligned";
     case GQA_ERR_CUDA: return "CUDA error";
     case GQA_ERR_DEVICE_TIMEOUT: return "a kernel's bounded wait expired (device error flag set)";
     case GQA_ERR_WORKSPACE: return "workspace missing or too small";
     case GQA_ERR_NO_DEVICE: return "no usable sm_100 device / driver entry point";
-    case GQA_ERR_DEVICE_INPUT: return "a kernel found invalid device-side input (page index or cache capacity)";
+    case GQA_ERR_DEVICE_INPUT: return "a kernel found invalid device-side input (page index, cache length, token range or position)";
     default: return "unknown status";
   }
 }

@@ -137,6 +137,9 @@ __device__ __forceinline__ void plan(const Batch& p, const Line (&lines)[kLines]
   const int warps = max(2, min(kWarps, (p.B + 31) / 32));
   // ---- steps in front of each sequence, per line: scratch[i * kMaxB + b]
   uint32_t total[kLines] = {};
+  // A q_start out of order leaves no work at all: its sequences could share tokens, and so
+  // have more steps than the host has counted.
+  int disordered = 0;
 #pragma unroll 1
   for (int b0 = 0; b0 < p.B; b0 += kThreads) {
     const int b = b0 + threadIdx.x;
@@ -145,9 +148,13 @@ __device__ __forceinline__ void plan(const Batch& p, const Line (&lines)[kLines]
       Seq s = {0, 0, 0};
       if (b < p.B) {
         s = seq_of(p, b);
+        const int z = __ldg(p.q_start + b + 1);
+        if (s.a < 0 || z < s.a || z > p.T) {
+          disordered = 1;
+          if (blockIdx.x == 0) record_input_error(site_q_start);
+        }
         if (blockIdx.x == 0) {
-          const int z = __ldg(p.q_start + b + 1), L = __ldg(p.lens + b);
-          if (s.a < 0 || z < s.a || z > p.T) record_input_error(site_q_start);
+          const int L = __ldg(p.lens + b);
           if (L < 0 || L > p.capacity) record_input_error(site_length);
         }
       }
@@ -163,7 +170,7 @@ __device__ __forceinline__ void plan(const Batch& p, const Line (&lines)[kLines]
         if (lane == 31) wsum[i * kWarps + warp] = scan[i];
       }
     }
-    __syncthreads();
+    disordered = __syncthreads_or(disordered);
     if (warp < warps) {
 #pragma unroll
       for (int i = 0; i < kLines; ++i) {
@@ -176,6 +183,8 @@ __device__ __forceinline__ void plan(const Batch& p, const Line (&lines)[kLines]
     __syncthreads();
   }
   if (warp >= 2) return;
+  if (disordered)
+    for (uint32_t& x : total) x = 0;
   // ---- this CTA's line, its first CTA and number of CTAs
   const int n = static_cast<int>(gridDim.x);
   int on = 0, c0 = 0, nc = n;

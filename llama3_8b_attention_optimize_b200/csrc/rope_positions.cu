@@ -344,7 +344,7 @@ int launch(Params<T> p, int head_dim, int rot, bool il, cudaStream_t stream) {
   const int hy = std::max(1, std::min(p.H, 256 / nc));
   const int tz = std::max(1, std::min(16, 256 / (nc * hy)));
   const dim3 block(nc, hy, tz);
-  const unsigned grid = static_cast<unsigned>((p.T_ + tz - 1) / tz);
+  const unsigned grid = static_cast<unsigned>((static_cast<long long>(p.T_) + tz - 1) / tz);
   if (il)
     rope_kernel<T, E, true><<<grid, block, 0, stream>>>(p);
   else
@@ -487,7 +487,7 @@ extern "C" int gqa_kv_extend_bf16(const void* k, const void* v, long long k_toke
   const int n_rows = Hq + 2 * Hkv;
   p.tokens = T <= 512 ? 1 : 4;
   const dim3 block(p.s.n_chunks, std::max(1, std::min(n_rows, (T <= 512 ? 512 : 128) / p.s.n_chunks)));
-  const unsigned grid = static_cast<unsigned>((T + p.tokens - 1) / p.tokens);
+  const unsigned grid = static_cast<unsigned>((static_cast<long long>(T) + p.tokens - 1) / p.tokens);
   if (vec && il)
     extend_kernel<8, true><<<grid, block, 0, stream>>>(p);
   else if (vec)

@@ -550,8 +550,8 @@ def attend_chunk(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, bl
     that already hold their keys and values: token i of sequence b sees its slots up to
     its own (``causal``) or all lens[b].  ``lse`` (float32 [T, Hq]) receives the natural
     log of the softmax's sum.  ``max_q_len``: the longest sequence's number of new tokens
-    where the caller knows it (a hint that picks the tiling).  Tokens that see no slot give
-    zeros and -inf."""
+    where the caller knows it, a hint that only sizes the second launch.  Tokens that see no
+    slot give zeros and -inf."""
     dev = _index(q, "q")
     out = torch.empty(q.shape, dtype=_BF16, device=q.device) if out is None else out
     _check(dev, ((q, "q", _BF16), (out, "out", _BF16)),
@@ -587,7 +587,7 @@ def attn_weight_sums(q: torch.Tensor, kpages: torch.Tensor, block_table: torch.T
     group's query heads and the chunk's tokens that see slot j.  acc, acc_out float32
     [B, Hkv, capacity]; entries at lens[b] and above are left alone; acc_out defaults to
     acc (in place).  q, q_start, lens and ``lse`` are those of ``attend_chunk``, whose
-    ``max_q_len`` is accepted too (this kernel has one tiling)."""
+    ``max_q_len`` is accepted too (and not needed)."""
     if max_q_len < 0:
         raise ValueError("max_q_len must not be negative")
     dev = _index(q, "q")

@@ -464,6 +464,27 @@ def test_attend_reports_bad_device_input(what):
     bt.check_attend(bt.attend(), None)  # the next call is sound again
 
 
+@pytest.mark.parametrize("starts", [[0, 5, 0, 5], [0, 3, 9, 5], [-1, 3, 4, 5]])
+def test_q_start_out_of_order_computes_nothing(starts):
+    """Such sequences could share tokens and have more steps than the host has counted."""
+    bt = Batch([3, 1, 1], [60, 40, 300], 8, 2, 16)
+    lse = torch.zeros(bt.T, 8, device="cuda")
+    out = torch.full_like(bt.q, 7.0).contiguous()
+    acc = torch.full((3, 2, bt.cap), 3.0, device="cuda")
+    acc_out = torch.full_like(acc, 5.0)
+    q_start = i32(starts)
+    kernels.attend_chunk(bt.q, bt.kp, bt.vp, bt.table, q_start, bt.lens, out=out)
+    with pytest.raises(GqaError) as e:
+        kernels.device_check()
+    assert e.value.code == _lib.GQA_ERR_DEVICE_INPUT
+    kernels.attn_weight_sums(bt.q, bt.kp, bt.table, q_start, bt.lens, lse, acc, acc_out=acc_out)
+    with pytest.raises(GqaError) as e:
+        kernels.device_check()
+    assert e.value.code == _lib.GQA_ERR_DEVICE_INPUT
+    assert (out == 7.0).all() and (acc_out == 5.0).all()
+    kernels.device_check()
+
+
 # ------------------------------------------------------------------ accumulated weights
 def check_weights(bt, lse, acc, got, causal=True, scale=None):
     scale = D ** -0.5 if scale is None else scale
