@@ -141,12 +141,21 @@ struct Line {
   }
 };
 
+// 16 columns of this lane's row of TMEM; tmem_wait_ld_dep16 before they are used.
+__device__ __forceinline__ void ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
 // p = 2^(s * sl2 + nl) of 32 rows that all see the slot.  The exponentials bound a chunk of
 // many tokens (a share of them on the FMA pipe, by a quintic, measured 98 to 108 us where
 // this takes 99).
-__device__ __forceinline__ void add_all(const uint32_t (&s)[32], const float* nl, float2 sl2, float2& a0, float2& a1) {
+__device__ __forceinline__ void add_all(const uint32_t (&s)[16], const float* nl, float2 sl2, float2& a0, float2& a1) {
 #pragma unroll
-  for (int c = 0; c < 32; c += 4) {
+  for (int c = 0; c < 16; c += 4) {
     const float4 l = *reinterpret_cast<const float4*>(nl + c);
     const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sl2, make_float2(l.x, l.y));
     const float2 y =
@@ -158,10 +167,10 @@ __device__ __forceinline__ void add_all(const uint32_t (&s)[32], const float* nl
 
 // The same where not all of the 32 rows see the slot: only the first nv, and of those the
 // ones whose token is at least `from` within the tile.
-__device__ __forceinline__ void add_masked(const uint32_t (&s)[32], const float* nl, const uint8_t* tok, int nv, int from,
+__device__ __forceinline__ void add_masked(const uint32_t (&s)[16], const float* nl, const uint8_t* tok, int nv, int from,
                                            float sl2, float2& a0) {
 #pragma unroll
-  for (int c = 0; c < 32; c += 4) {
+  for (int c = 0; c < 16; c += 4) {
     const float4 l = *reinterpret_cast<const float4*>(nl + c);
     const uchar4 t = *reinterpret_cast<const uchar4*>(tok + c);
     const float e[4] = {ex2_approx(fmaf(__uint_as_float(s[c]), sl2, l.x)), ex2_approx(fmaf(__uint_as_float(s[c + 1]), sl2, l.y)),
@@ -433,8 +442,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int nv = wide && k != ch ? 0 : min(64, min(p.tpt, s.s.n - t0) * p.G - half);
           // the tile's first token sees slots up to see0, each next token one more
           const int see0 = p.causal ? s.s.L - s.s.n + t0 : s.s.L - 1;
-          if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_SFULL + 2 * kt + bb), (g / 2) & 1u, SITE_SOFTMAX));
-          if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(B_LFULL + bb), (g / 2) & 1u, SITE_SOFTMAX));
+          if (ok) {  // both asked before either answer is needed
+            const uint32_t parity = (g / 2) & 1u;
+            const bool l_now = mbar_try_wait(bar(B_LFULL + bb), parity);
+            const bool s_now = mbar_try_wait(bar(B_SFULL + 2 * kt + bb), parity);
+            bool both = l_now && s_now;
+            if (!both)
+              both = mbar_wait(bar(B_LFULL + bb), parity, SITE_SOFTMAX) &&
+                     mbar_wait(bar(B_SFULL + 2 * kt + bb), parity, SITE_SOFTMAX);
+            ok = __all_sync(0xffffffffu, both);
+          }
           if (!ok) continue;
           const bool all = see0 >= warp_last;
           const int from = p.causal ? slot - see0 : 0;  // a row of a token below this does not see the slot
@@ -443,23 +460,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float* nl = lse + 128 * bb + half;
           tc_fence_after();
           if (nv > 8) {
-            uint32_t v[32];
+            // 16 rows at a time, the next 16 on their way while these are added up
+            uint32_t v[2][16];
+            ld16(tv, v[0]);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int left = nv - 32 * c;
-              if (left > 0) {
-                tmem_ld32(tv + 32 * c, v);
-                tmem_wait_ld_dep(v);
-              }
-              if (c == 1) {
+            for (int c = 0; c < 4; ++c) {
+              const int left = nv - 16 * c;
+              tmem_wait_ld_dep16(v[c & 1]);
+              if (c < 3) {
+                ld16(tv + 16 * (c + 1), v[(c + 1) & 1]);
+              } else {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(B_SFREE + 2 * kt + bb));
               }
-              if (all && left >= 32)
-                add_all(v, nl + 32 * c, sl2, a0, a1);
+              if (all && left >= 16)
+                add_all(v[c & 1], nl + 16 * c, sl2, a0, a1);
               else if (left > 0)
-                add_masked(v, nl + 32 * c, tok + half + 32 * c, left, from, p.scale_log2, a0);
+                add_masked(v[c & 1], nl + 16 * c, tok + half + 16 * c, left, from, p.scale_log2, a0);
             }
           } else {
             add_some(tv, nl, tok + half, nv, from, p.scale_log2, a0);
