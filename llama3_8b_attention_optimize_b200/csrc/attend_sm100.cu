@@ -20,7 +20,7 @@
 //        O^T += V^T P^T with N = 16 or 32, so that the tensor core does no more work than
 //        there are rows.  Such units are bound by memory, and padding 4 rows to 128
 //        drew the GPU's whole power budget (1000 W at 1.39 GHz instead of 1.97: 64 tokens
-//        over 1024..32768 slots 813 us instead of what the header of few_rows says).
+//        over 1024..32768 slots took 813 us, where this form takes 650).
 //
 // Split: the units' K/V tiles form one line per form, and the CTAs (one per SM) are dealt
 // out to the two lines by what a tile of each costs; each line is cut into equal parts
@@ -34,6 +34,14 @@
 // tcgen05.mma with accumulators in TMEM; softmax warps turn S into P; a helper warp clears
 // V rows past the last slot that the unit sees (P is zero there, but a cache may hold
 // anything, and 0 * NaN would spread).
+//
+// Measured (Hq 32, Hkv 8, both launches, replayed from a graph):
+//   64 single tokens over 1024..32768 slots, 4.25 GB  650 us  6.5 TB/s, what a copy reaches
+//   2048 tokens behind 30720 slots, 1.07 TFLOP        1090 us  980 TFLOP/s, 0.60 of a GEMM's burst: the
+//     tensor pipe is busy for 52 % of the cycles, the rest is the softmax's exponentials and
+//     hand-offs (sustained, the 1000 W limit makes it 1265 us)
+//   512 tokens beside 31 sequences of 1..5, 315 MB    107 us  about half from each of the two lines
+//   4 single tokens over 37..1023 slots               14 us  latency: plan, one or two tiles, merge
 #include <cuda.h>
 
 #include <algorithm>

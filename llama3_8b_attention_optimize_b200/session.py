@@ -289,7 +289,7 @@ class ChunkedKVCache:
         self.interleaved = interleaved
         self.max_positions = self.capacity if max_positions is None else max_positions
         shape = (num_pages, Hkv, page_size, kernels.HEAD_DIM)
-        # rows past a sequence's length are never read, so the pools need no clearing
+        # rows past a sequence's length may hold anything, so the pools need no clearing
         self.k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
         self.v = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
         self.table = torch.full((B, max_pages_per_seq), -1, dtype=torch.int32, device=self.device)
