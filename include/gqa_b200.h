@@ -277,7 +277,8 @@ int gqa_decode_paged_bf16(const void* q, const void* kpages, const void* vpages,
  * largest acc (equal ones: the lower slot; NaN counts as lowest).  The i-th slot below
  * the new length that goes receives the i-th kept slot above it (K, V, acc, slot_pos).
  * acc_out, slot_pos_out [B][Hkv][capacity] get the first min(lens[b], budget) entries;
- * lens_out the new lengths.  Each may be its input.  sink + recent <= budget, capacity
+ * lens_out the new lengths.  Each may be its input.  Rows move in place, so the pages of
+ * a sequence longer than budget must be its own.  sink + recent <= budget, capacity
  * at most 2^20 slots; workspace: gqa_kv_evict_workspace_size bytes.                   */
 int gqa_rope_table_f32(const double* inv_freq, float* cos, float* sin, int rows, int half_dim, int pos0, double mscale,
                        gqa_stream_t stream);

@@ -411,19 +411,19 @@ def test_attend_other_stream_and_repeat():
 def test_attend_large_pool_offsets():
     """Pages at the far end of a pool of more than 2^31 values, everything else uninitialised."""
     pages = 2200
-    bt = Batch([3, 1], [1500, 2000], 32, 8, 1024, pool_pages=5)
+    bt = Batch([3, 1], [1500, 2000], 32, 8, 1024, pool_pages=5, extra_table=2)
     kp = torch.empty(pages, 8, 1024, D, dtype=torch.bfloat16, device="cuda")
     vp = torch.empty_like(kp)
     kp[-4:] = randn(4, 8, 1024, D, seed=1)
     vp[-4:] = randn(4, 8, 1024, D, seed=2)
     bt.kp, bt.vp = kp, vp
-    bt.table_list = np.array([[pages - 1, pages - 3, -1], [pages - 4, pages - 2, -1]], np.int32)
+    bt.table_list = np.array([[pages - 1, pages - 3, -1, -1], [pages - 4, pages - 2, -1, -1]], np.int32)
     bt.table = torch.from_numpy(bt.table_list).cuda()
     lse = torch.empty(bt.T, 32, device="cuda")
     out = bt.attend(lse=lse)
     kernels.device_check()
     bt.check_attend(out, lse)
-    acc = torch.zeros(2, 8, 3 * 1024, device="cuda")
+    acc = torch.zeros(2, 8, bt.cap, device="cuda")
     check_weights(bt, lse, acc, kernels.attn_weight_sums(bt.q, kp, bt.table, bt.q_start, bt.lens, lse, acc.clone()))
 
 
