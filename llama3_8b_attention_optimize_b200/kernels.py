@@ -624,8 +624,9 @@ def kv_evict(kpages: torch.Tensor, vpages: torch.Tensor, block_table: torch.Tens
     the first ``sink`` positions or of the last ``recent`` before next_pos[b] (int32 [B]),
     then those with the largest ``acc``, equal ones by the lower slot.  The i-th slot
     below the new length that goes receives the i-th kept one above it; K and V rows move
-    in place, so a sequence that is cut may share no page with another.  acc, slot_pos [B, Hkv, capacity] (float32, int32) follow into acc_out,
-    slot_pos_out, the lengths into lens_out; each defaults to its input."""
+    in place, so a sequence that is cut may share no page with another.  acc, slot_pos
+    [B, Hkv, capacity] (float32, int32) follow into acc_out, slot_pos_out, the lengths into
+    lens_out; each defaults to its input."""
     dev = _index(kpages, "kpages")
     acc_out = acc if acc_out is None else acc_out
     slot_pos_out = slot_pos if slot_pos_out is None else slot_pos_out
