@@ -340,7 +340,7 @@ class ChunkedKVCache:
              out: torch.Tensor | None = None) -> torch.Tensor:
         """One step: q [T, Hq, 128], k, v [T, Hkv, 128] (before rotation, any strides) hold the new
         tokens of sequence 0, then 1, ...; new[b] of them belong to sequence b.  Returns the
-        attention's output [T, Hq, 128]."""
+        attention's output [T, Hq, 128].  Where it raises, lengths and positions are as before."""
         T = sum(new)
         if q.shape[0] != T or k.shape[0] != T or v.shape[0] != T:
             raise ValueError("q, k and v must hold sum(new) tokens")
@@ -353,14 +353,17 @@ class ChunkedKVCache:
         plan = host.pin_memory().to(self.device, non_blocking=True)
         # slices of their own: 4-byte alignment is all the kernels ask of them
         q_start, positions = plan[: self.B + 1], plan[2 * self.B + 1:]
-        self.lens.copy_(plan[self.B + 1: 2 * self.B + 1])
-        q_rot = kernels.kv_extend(k, v, self.k, self.v, self.table, q_start, self.lens, positions, self.cos, self.sin, q=q,
+        # The cache's own lengths move on, here and on the device, when every call has been
+        # accepted: where one raises, what was written lies past them and is written again.
+        new_lens = plan[self.B + 1: 2 * self.B + 1]
+        q_rot = kernels.kv_extend(k, v, self.k, self.v, self.table, q_start, new_lens, positions, self.cos, self.sin, q=q,
                                   interleaved=self.interleaved, slot_pos=self.slot_pos)
         longest = max(new) if new else 0
         lse = None if self.acc is None else torch.empty(T, self.Hq, dtype=torch.float32, device=self.device)
-        out = kernels.attend_chunk(q_rot, self.k, self.v, self.table, q_start, self.lens, max_q_len=longest, out=out, lse=lse)
+        out = kernels.attend_chunk(q_rot, self.k, self.v, self.table, q_start, new_lens, max_q_len=longest, out=out, lse=lse)
         if self.acc is not None:
-            kernels.attn_weight_sums(q_rot, self.k, self.table, q_start, self.lens, lse, self.acc, max_q_len=longest)
+            kernels.attn_weight_sums(q_rot, self.k, self.table, q_start, new_lens, lse, self.acc, max_q_len=longest)
+        self.lens.copy_(new_lens)
         self._lens_h = lens
         self._pos_h = [p + n for p, n in zip(self._pos_h, new)]
         return out
