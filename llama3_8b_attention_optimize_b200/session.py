@@ -319,6 +319,10 @@ class ChunkedKVCache:
 
     def reserve(self, new: list[int]) -> None:
         """Give sequence b pages for new[b] more tokens (raises, with nothing changed, when they do not fit)."""
+        self._take(new)
+
+    def _take(self, new: list[int]) -> list[tuple[int, int]]:
+        """Reserve; returns the (sequence, logical page) pairs that were not there yet."""
         if len(new) != self.B or any(n < 0 for n in new):
             raise ValueError("new needs one count per sequence")
         wanted = []
@@ -334,17 +338,35 @@ class ChunkedKVCache:
         for b, lp in wanted:
             self._table_h[b][lp] = self._free.pop()
         if wanted:
-            self.table.copy_(torch.tensor(self._table_h, dtype=torch.int32))
+            self._upload_table()
+        return wanted
+
+    def _upload_table(self) -> None:
+        self.table.copy_(torch.tensor(self._table_h, dtype=torch.int32))
 
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, new: list[int],
              out: torch.Tensor | None = None) -> torch.Tensor:
         """One step: q [T, Hq, 128], k, v [T, Hkv, 128] (before rotation, any strides) hold the new
         tokens of sequence 0, then 1, ...; new[b] of them belong to sequence b.  Returns the
-        attention's output [T, Hq, 128].  Where it raises, lengths and positions are as before."""
+        attention's output [T, Hq, 128].  Where it raises, lengths, positions and pages are
+        as before."""
         T = sum(new)
         if q.shape[0] != T or k.shape[0] != T or v.shape[0] != T:
             raise ValueError("q, k and v must hold sum(new) tokens")
-        self.reserve(new)
+        taken = self._take(new)
+        try:
+            return self._run(q, k, v, new, T, out)
+        except Exception:
+            for b, lp in reversed(taken):
+                self._free.append(self._table_h[b][lp])
+                self._table_h[b][lp] = -1
+            if taken:
+                self._upload_table()
+            raise
+
+    def _run(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, new: list[int], T: int,
+             out: torch.Tensor | None) -> torch.Tensor:
+        """The kernels of a step whose pages are there."""
         lens = [a + n for a, n in zip(self._lens_h, new)]
         # one upload: q_start, the lengths with the new tokens, and the tokens' positions
         ends = torch.tensor([0, *new], dtype=torch.int32).cumsum(0, dtype=torch.int32)
@@ -383,7 +405,7 @@ class ChunkedKVCache:
         for b, n in enumerate(self._lens_h):
             self._lens_h[b] = min(n, budget)
             self._give_back(b, self._pages(self._lens_h[b]))
-        self.table.copy_(torch.tensor(self._table_h, dtype=torch.int32))
+        self._upload_table()
 
     def _give_back(self, b: int, first: int) -> None:
         for lp in range(first, self.max_pages):

@@ -47,17 +47,19 @@ def step(cache, new):
 
 @pytest.mark.parametrize("where", ["kv_extend", "attend_chunk", "attn_weight_sums"])
 def test_a_step_that_raises_changes_nothing(monkeypatch, where):
-    """Lengths and positions stay as they were, on the device too, so that an eviction
+    """Lengths, positions and pages stay as they were, on the device too, so that an eviction
     (what a server does when memory runs out) and the next step go by real slots only."""
     stubs = Stubs(monkeypatch)
     cache = ChunkedKVCache(2, num_pages=40, max_pages_per_seq=20, Hkv=1, Hq=4, page_size=16, device="cpu")
     step(cache, [100, 20])
+    free, table = cache.free_pages, cache.table.tolist()
     stubs.fail = where
     with pytest.raises(torch.OutOfMemoryError):
         step(cache, [50, 1])
     stubs.fail = None
     assert cache.lens.tolist() == [100, 20] == [cache.seq_len(b) for b in range(2)]
     assert [cache.next_pos(b) for b in range(2)] == [100, 20]
+    assert cache.free_pages == free and cache.table.tolist() == table
     cache.evict(64, sink=4)
     assert stubs.seen["kv_evict"]["lens"] == [100, 20] and stubs.seen["kv_evict"]["next_pos"] == [100, 20]
     assert cache.lens.tolist() == [64, 20] == [cache.seq_len(b) for b in range(2)]
@@ -65,3 +67,18 @@ def test_a_step_that_raises_changes_nothing(monkeypatch, where):
     assert stubs.seen["attend_chunk"]["lens"] == [65, 20] and stubs.seen["kv_extend"]["positions"] == [100]
     assert cache.lens.tolist() == [65, 20]
 
+
+def test_pages_reserved_ahead_stay_reserved_when_a_step_raises(monkeypatch):
+    stubs = Stubs(monkeypatch)
+    cache = ChunkedKVCache(2, num_pages=10, max_pages_per_seq=5, Hkv=1, Hq=4, page_size=16, device="cpu")
+    cache.reserve([40, 0])
+    assert cache.free_pages == 7
+    stubs.fail = "attend_chunk"
+    with pytest.raises(torch.OutOfMemoryError):
+        step(cache, [50, 17])
+    assert cache.free_pages == 7
+    held = {p for row in cache.table.tolist() for p in row if p >= 0}
+    stubs.fail = None
+    step(cache, [80, 80])
+    pages = [p for row in cache.table.tolist() for p in row]
+    assert sorted(pages) == list(range(10)) and held <= set(pages[:5]) and cache.free_pages == 0
