@@ -305,7 +305,8 @@ def decode_paged(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, bl
 
 _BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 _SCALE = default_scale()
-_raw_stream = torch._C._cuda_getCurrentRawStream  # (device index) -> cudaStream_t, without a Stream object
+# (device index) -> cudaStream_t, without a Stream object; None in a torch built without CUDA
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _rows3(t: torch.Tensor, name: str, dtype=torch.bfloat16) -> None:

@@ -184,3 +184,16 @@ def test_wrappers_refuse_cpu_tensors():
         kernels.kv_evict(x, x, i, i, c, i, i, 4)
     with pytest.raises(TypeError):
         kernels.rope_positions([1.0], i, c, c)
+
+
+def test_package_imports_under_a_torch_without_cuda():
+    """Such a torch has no _cuda_ names in torch._C; what needs no GPU works there."""
+    import subprocess
+    import sys
+    code = ("import torch\n"
+            "for name in ('_cuda_getCurrentRawStream', '_cuda_getDevice'):\n"
+            "    delattr(torch._C, name)\n"
+            "from llama3_8b_attention_optimize_b200 import kernels, golden_model, cpu_baseline\n"
+            "print(kernels.rope_inv_freq(4)[0].tolist()[0])\n")
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert run.returncode == 0 and run.stdout.strip() == "1.0", run.stderr
