@@ -279,7 +279,9 @@ int gqa_decode_paged_bf16(const void* q, const void* kpages, const void* vpages,
  * acc_out, slot_pos_out [B][Hkv][capacity] get the first min(lens[b], budget) entries;
  * lens_out the new lengths.  Each may be its input.  Rows move in place, so the pages of
  * a sequence longer than budget must be its own.  sink + recent <= budget, capacity
- * at most 2^20 slots; workspace: gqa_kv_evict_workspace_size bytes.                   */
+ * at most 2^20 slots; workspace: gqa_kv_evict_workspace_size bytes for the rows of a head
+ * that can move, min(budget, capacity - budget), or for any larger number such as budget;
+ * none where budget >= capacity.                                                      */
 int gqa_rope_table_f32(const double* inv_freq, float* cos, float* sin, int rows, int half_dim, int pos0, double mscale,
                        gqa_stream_t stream);
 int gqa_rope_positions_bf16(const void* x, void* y, const int32_t* positions, const float* cos, const float* sin, int T,
@@ -310,7 +312,7 @@ int gqa_attn_weight_sums_f32(const void* q, long long q_token_stride, long long 
                              const int32_t* q_start, const int32_t* lens, const float* lse, const float* acc,
                              float* acc_out, void* workspace, size_t workspace_bytes, int B, int T, int Hq, int Hkv,
                              int head_dim, float scale, int flags, gqa_stream_t stream);
-size_t gqa_kv_evict_workspace_size(int B, int Hkv, int budget);
+size_t gqa_kv_evict_workspace_size(int B, int Hkv, int rows);
 int gqa_kv_evict_bf16(void* kpages, void* vpages, const int32_t* block_table, int max_pages_per_seq, int page_size,
                       int num_pages, const int32_t* lens, int32_t* lens_out, const float* acc, float* acc_out,
                       const int32_t* slot_pos, int32_t* slot_pos_out, const int32_t* next_pos, void* workspace,

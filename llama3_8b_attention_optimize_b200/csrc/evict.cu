@@ -49,8 +49,9 @@ struct Params {
   const float* acc;
   float* acc_out;
   int32_t *pos_out, *lens_out;
-  int32_t *src, *dst, *count;  // workspace: [B * Hkv][budget] twice, [B * Hkv]
+  int32_t *src, *dst, *count;  // workspace: [B * Hkv][rows] twice, [B * Hkv]; none where rows is 0
   int Hkv, capacity, max_pages, page_size, num_pages, budget, recent, sink, cached, page_shift;
+  int rows;  // rows of one (b, h) that can move at most
 };
 
 // Order-preserving key: larger weight, larger key; NaN below every number, -0 equals +0,
@@ -82,7 +83,7 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
   int32_t* pos_out = p.pos_out + base;
   if (bh % p.Hkv == 0 && tid == 0 && p.lens_out != p.lens) p.lens_out[b] = left;
   if (n <= p.budget) {
-    if (tid == 0) p.count[bh] = 0;
+    if (tid == 0 && p.rows > 0) p.count[bh] = 0;
     if (acc_out != acc)
       for (int i = tid; i < n; i += kThreads) acc_out[i] = acc[i];
     if (pos_out != pos)
@@ -191,8 +192,8 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
     hole += counts[0][w];
     mover += counts[1][w];
   }
-  int32_t* src = p.src + static_cast<size_t>(bh) * p.budget;
-  int32_t* dst = p.dst + static_cast<size_t>(bh) * p.budget;
+  int32_t* src = p.src + static_cast<size_t>(bh) * p.rows;
+  int32_t* dst = p.dst + static_cast<size_t>(bh) * p.rows;
   const uint32_t below = (1u << lane) - 1;
   for (int i0 = r0; i0 < r1; i0 += 32) {
     const uint32_t kept = bits[i0 >> 5], is_hole = ~kept & low(i0), is_mover = kept & ~low(i0);
@@ -254,8 +255,8 @@ __global__ void __launch_bounds__(kMoveWarps * 32) move_kernel(const Params p) {
   const int bh = blockIdx.y, b = bh / p.Hkv, h = bh % p.Hkv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int count = p.count[bh];
-  const int32_t* src = p.src + static_cast<size_t>(bh) * p.budget;
-  const int32_t* dst = p.dst + static_cast<size_t>(bh) * p.budget;
+  const int32_t* src = p.src + static_cast<size_t>(bh) * p.rows;
+  const int32_t* dst = p.dst + static_cast<size_t>(bh) * p.rows;
   uint16_t* pool = (lane < 16 ? p.kp : p.vp) + (lane & 15) * 8;
   const int32_t* table = p.table + static_cast<long long>(b) * p.max_pages;
   const int32_t* list = lane < 16 ? src : dst;
@@ -302,9 +303,9 @@ GQA_ERROR_FLAG_ACCESSOR(error_flag_evict)
 
 }  // namespace gqa
 
-extern "C" size_t gqa_kv_evict_workspace_size(int B, int Hkv, int budget) {
-  if (B <= 0 || Hkv <= 0 || budget <= 0) return 0;
-  return static_cast<size_t>(B) * Hkv * (2 * static_cast<size_t>(budget) + 1) * sizeof(int32_t);
+extern "C" size_t gqa_kv_evict_workspace_size(int B, int Hkv, int rows) {
+  if (B <= 0 || Hkv <= 0 || rows <= 0) return 0;
+  return static_cast<size_t>(B) * Hkv * (2 * static_cast<size_t>(rows) + 1) * sizeof(int32_t);
 }
 
 extern "C" int gqa_kv_evict_bf16(void* kpages, void* vpages, const int32_t* block_table, int max_pages_per_seq,
@@ -330,7 +331,9 @@ extern "C" int gqa_kv_evict_bf16(void* kpages, void* vpages, const int32_t* bloc
                           static_cast<const void*>(slot_pos_out), static_cast<const void*>(next_pos),
                           static_cast<const void*>(workspace)})
     if (reinterpret_cast<uintptr_t>(ptr) % 4) return GQA_ERR_MISALIGNED;
-  if (!workspace || workspace_bytes < gqa_kv_evict_workspace_size(B, Hkv, budget)) return GQA_ERR_WORKSPACE;
+  // kept slots at `budget` or above move into holes below it
+  const int rows = static_cast<int>(std::min<long long>(budget, std::max(0LL, capacity - budget)));
+  if (rows > 0 && (!workspace || workspace_bytes < gqa_kv_evict_workspace_size(B, Hkv, rows))) return GQA_ERR_WORKSPACE;
   Params p;
   p.kp = static_cast<uint16_t*>(kpages);
   p.vp = static_cast<uint16_t*>(vpages);
@@ -342,7 +345,7 @@ extern "C" int gqa_kv_evict_bf16(void* kpages, void* vpages, const int32_t* bloc
   p.acc_out = acc_out;
   p.pos_out = slot_pos_out;
   p.lens_out = lens_out;
-  const size_t n_list = static_cast<size_t>(B) * Hkv * budget;
+  const size_t n_list = static_cast<size_t>(B) * Hkv * rows;
   p.src = static_cast<int32_t*>(workspace);
   p.dst = p.src + n_list;
   p.count = p.dst + n_list;
@@ -352,6 +355,7 @@ extern "C" int gqa_kv_evict_bf16(void* kpages, void* vpages, const int32_t* bloc
   p.page_size = page_size;
   p.num_pages = num_pages;
   p.budget = budget;
+  p.rows = rows;
   p.recent = recent;
   p.sink = sink;
   p.cached = capacity <= kCachedKeys ? 1 : 0;
@@ -362,11 +366,10 @@ extern "C" int gqa_kv_evict_bf16(void* kpages, void* vpages, const int32_t* bloc
   if ((rc = ensure_smem_attr(select_kernel, (kCachedKeys + kCachedKeys / 32) * 4, attr_done)) != GQA_OK) return rc;
   select_kernel<<<B * Hkv, kThreads, smem, stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return GQA_ERR_CUDA;
-  // as many rows as can move at most, and no more blocks than fill the GPU a few times
-  const long long moves = std::min<long long>(budget, capacity - budget);
-  if (moves > 0) {
+  // no more blocks than fill the GPU a few times
+  if (rows > 0) {
     const long long per_block = kMoveWarps * kRowsPerWarp;
-    const long long want = (moves + per_block - 1) / per_block;
+    const long long want = (rows + per_block - 1) / per_block;
     const long long cap = std::max<long long>(1, 148 * 16 / (static_cast<long long>(B) * Hkv));
     if ((rc = launch_after(move_kernel, dim3(static_cast<unsigned>(std::min(want, cap)), B * Hkv), kMoveWarps * 32, stream,
                            p)) != GQA_OK)

@@ -613,8 +613,10 @@ def attn_weight_sums(q: torch.Tensor, kpages: torch.Tensor, block_table: torch.T
     return acc_out
 
 
-def kv_evict_workspace_bytes(B: int, Hkv: int, budget: int) -> int:
-    return int(_lib.load().gqa_kv_evict_workspace_size(B, Hkv, budget))
+def kv_evict_workspace_bytes(B: int, Hkv: int, budget: int, capacity: int | None = None) -> int:
+    """Bytes that a call with this budget needs: for `capacity` slots a sequence, else for any capacity."""
+    rows = budget if capacity is None else min(budget, max(capacity - budget, 0))
+    return int(_lib.load().gqa_kv_evict_workspace_size(B, Hkv, rows))
 
 
 def kv_evict(kpages: torch.Tensor, vpages: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
@@ -641,7 +643,7 @@ def kv_evict(kpages: torch.Tensor, vpages: torch.Tensor, block_table: torch.Tens
         raise ValueError("acc, acc_out, slot_pos and slot_pos_out must be [B, Hkv, max_pages * page_size]")
     if next_pos.shape != (B,) or lens_out.shape != (B,):
         raise ValueError("next_pos and lens_out must be [B]")
-    workspace = _workspace(workspace, kv_evict_workspace_bytes(B, Hkv, budget), dev)
+    workspace = _workspace(workspace, kv_evict_workspace_bytes(B, Hkv, budget, shape[2]), dev)
     _call(dev, "gqa_kv_evict_bf16", 0.0, kpages.data_ptr(), vpages.data_ptr(), block_table.data_ptr(), max_pages, page_size,
           num_pages, lens.data_ptr(), lens_out.data_ptr(), acc.data_ptr(), acc_out.data_ptr(), slot_pos.data_ptr(),
           slot_pos_out.data_ptr(), next_pos.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(),

@@ -197,3 +197,12 @@ def test_package_imports_under_a_torch_without_cuda():
             "print(kernels.rope_inv_freq(4)[0].tolist()[0])\n")
     run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
     assert run.returncode == 0 and run.stdout.strip() == "1.0", run.stderr
+
+
+def test_evict_workspace_goes_by_the_rows_that_can_move(lib):
+    """Of a sequence's slots at most min(budget, capacity - budget) change their place."""
+    assert kernels.kv_evict_workspace_bytes(32, 8, 1 << 30, 32768) == 0  # nothing is ever cut
+    assert kernels.kv_evict_workspace_bytes(32, 8, 32768, 32768) == 0
+    assert kernels.kv_evict_workspace_bytes(2, 8, 4096, 4097) == lib.gqa_kv_evict_workspace_size(2, 8, 1)
+    assert kernels.kv_evict_workspace_bytes(2, 8, 100, 32768) == lib.gqa_kv_evict_workspace_size(2, 8, 100)
+    assert kernels.kv_evict_workspace_bytes(2, 8, 100) == lib.gqa_kv_evict_workspace_size(2, 8, 100)

@@ -764,3 +764,26 @@ def test_no_tokens_is_no_work():
     for b, n in enumerate((5, 9)):
         assert torch.equal(got[b, :, :n], acc[b, :, :n]) and (got[b, :, n:] == 0).all()
     kernels.device_check()
+
+
+# ------------------------------------------------------------------ eviction's workspace
+@pytest.mark.parametrize("lens,budget", [([300, 200], 1 << 30), ([336, 40], 336), ([336, 300, 1], 335), ([40, 30], 300)])
+def test_evict_workspace_of_the_rows_that_can_move(lens, budget):
+    """A budget that cuts little or nothing asks for as little memory; what lies behind it stays."""
+    bt = Batch([0] * len(lens), lens, 4, 2, 16, extra_table=336 // 16 - -(-max(lens) // 16))
+    assert bt.cap == 336
+    slot_pos = torch.arange(bt.cap, dtype=torch.int32, device="cuda").expand(bt.B, 2, -1).contiguous()
+    acc = weights_for(bt, "plain")
+    next_pos = i32(lens)
+    need = kernels.kv_evict_workspace_bytes(bt.B, 2, budget, bt.cap)
+    assert need == (0 if budget >= 336 else bt.B * 2 * (2 * min(budget, 336 - budget) + 1) * 4)
+    room = torch.full((need + 64,), 0x5A, dtype=torch.uint8, device="cuda")
+    kp, vp, a, s, left = evict_ref(bt, acc, slot_pos, lens, budget, 8, 2)
+    short = bt.lens.clone()
+    kernels.kv_evict(bt.kp, bt.vp, bt.table, short, acc, slot_pos, next_pos, budget, recent=8, sink=2, workspace=room[:need])
+    kernels.device_check()
+    assert (room[need:] == 0x5A).all() and short.tolist() == left
+    assert np.array_equal(bt.kp.view(torch.int16).cpu().numpy(), kp)
+    assert np.array_equal(bt.vp.view(torch.int16).cpu().numpy(), vp)
+    assert np.array_equal(acc.cpu().numpy(), a) and np.array_equal(slot_pos.cpu().numpy(), s)
+    run_evict(bt, acc, slot_pos, next_pos, budget, 8, 2)  # workspace from the allocator
