@@ -301,7 +301,8 @@ def decode_paged(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, bl
 # ------------------------------------------------------------------ serving a paged cache chunk by chunk
 # A step brings a ragged batch of new tokens: sequence b owns tokens
 # [q_start[b], q_start[b + 1]) and lens[b] counts its cached slots with those tokens
-# included, so its token i of n sits in slot lens[b] - n + i.
+# included, so its token i of n sits in slot lens[b] - n + i.  For serving: of these calls only
+# rope_positions takes part in autograd, the others' results carry no gradient.
 
 _BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 _SCALE = default_scale()
@@ -452,14 +453,21 @@ def rope_positions(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, 
     (int32 [T]) over its first 2 * cos.shape[1] dims; the others pass through.
 
     cos, sin: ``rope_table``.  Pairs are (i, i + rot/2), or (2i, 2i + 1) when ``interleaved``.
-    ``inverse`` rotates backwards, which is the gradient's way through this operator.
-    ``out`` may be x."""
+    ``inverse`` rotates backwards, which is the gradient's way through this operator: where x
+    requires a gradient autograd takes it, in x's type (the tables get none, and ``out``
+    carries none: both are refused).  ``out`` may be x."""
     dev = _index(x, "x")
     if x.dtype is not _BF16 and x.dtype is not _F32:
         raise TypeError(f"x must be bfloat16 or float32, got {x.dtype}")
+    if x.requires_grad and torch.is_grad_enabled():
+        if out is not None:
+            raise ValueError("out carries no gradient: leave it away, or pass x detached")
+        return _RopePositions.apply(x, positions, cos, sin, interleaved, inverse)
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
     _check(dev, ((x, "x", x.dtype), (out, "out", x.dtype)),
            ((positions, "positions", _I32), (cos, "cos", _F32), (sin, "sin", _F32)))
+    if (cos.requires_grad or sin.requires_grad) and torch.is_grad_enabled():
+        raise ValueError("cos and sin get no gradient: pass them detached")
     T, H, d = x.shape
     if positions.shape != (T,):
         raise ValueError("positions must be [T]")
@@ -472,6 +480,26 @@ def rope_positions(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, 
           positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), T, H, d, 2 * half, rows, x.stride(0), x.stride(1),
           out.stride(0), out.stride(1), (GQA_FLAG_INTERLEAVED if interleaved else 0) | (GQA_FLAG_INVERSE if inverse else 0))
     return out
+
+
+class _RopePositions(torch.autograd.Function):
+    """``rope_positions`` of an x that requires a gradient: the rotation is linear in x, and its
+    transpose is the rotation backwards (times the same scale of the tables)."""
+
+    @staticmethod
+    def forward(ctx, x, positions, cos, sin, interleaved, inverse):
+        if any(ctx.needs_input_grad[1:4]):
+            raise ValueError("cos and sin get no gradient: pass them detached")
+        ctx.save_for_backward(positions, cos, sin)
+        ctx.interleaved, ctx.inverse = interleaved, inverse
+        return rope_positions(x, positions, cos, sin, interleaved=interleaved, inverse=inverse)
+
+    @staticmethod
+    def backward(ctx, grad):
+        positions, cos, sin = ctx.saved_tensors
+        grad = grad if grad.stride(-1) == 1 else grad.contiguous()  # a broadcast one, as a sum's
+        g = rope_positions(grad, positions, cos, sin, interleaved=ctx.interleaved, inverse=not ctx.inverse)
+        return g, None, None, None, None, None
 
 
 def _paged(kpages: torch.Tensor, vpages: torch.Tensor | None, block_table: torch.Tensor, q_start: torch.Tensor | None,

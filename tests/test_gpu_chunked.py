@@ -787,3 +787,59 @@ def test_evict_workspace_of_the_rows_that_can_move(lens, budget):
     assert np.array_equal(bt.vp.view(torch.int16).cpu().numpy(), vp)
     assert np.array_equal(acc.cpu().numpy(), a) and np.array_equal(slot_pos.cpu().numpy(), s)
     run_evict(bt, acc, slot_pos, next_pos, budget, 8, 2)  # workspace from the allocator
+
+
+# ------------------------------------------------------------------ the rotation under autograd
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("interleaved,inverse", [(False, False), (True, False), (True, True)])
+def test_rope_positions_carries_its_gradient(dtype, interleaved, inverse):
+    """backward is the formula's transpose, held to the rotation's own bound, and it agrees with
+    differences: the rotation is linear, so <w, R(x + e) - R(x)> = <R^T w, e> up to the roundings
+    of two rotations (in 32 bits, where they are small beside a step)."""
+    T, H, d, rot = 21, 3, 96, 64
+    cos, sin = kernels.rope_table(3000, rot, scaling="yarn", factor=4.0, original_len=1024)
+    inv, m = kernels.rope_inv_freq(rot, scaling="yarn", factor=4.0, original_len=1024)
+    pos = torch.randint(0, 3000, (T,), generator=gen(1), device="cuda", dtype=torch.int32)
+    kw = dict(interleaved=interleaved, inverse=inverse)
+    base = randn(T, H + 2, d, seed=2, dtype=dtype).requires_grad_()
+    x = base[:, 1:1 + H]  # strided, as a slice of a fused projection
+    y = kernels.rope_positions(x, pos, cos, sin, **kw)
+    assert y.requires_grad and torch.equal(y, kernels.rope_positions(x.detach(), pos, cos, sin, **kw))
+    w = randn(T, H, d, seed=3, dtype=dtype)
+    g, = torch.autograd.grad(y, base, w)
+    ref, mag = rope_ref(w, pos, inv, m, interleaved, not inverse)
+    d_fp = 2.0 ** -22 * mag
+    bound = d_fp if dtype == torch.float32 else U * (ref.abs() + d_fp) + d_fp
+    assert ((g[:, 1:1 + H].double() - ref).abs() <= bound).all()
+    assert (g[:, 0] == 0).all() and (g[:, 1 + H:] == 0).all()
+    if dtype == torch.float32:
+        e = randn(T, H, d, seed=4, dtype=dtype)
+        with torch.no_grad():
+            diff = kernels.rope_positions(x + e, pos, cos, sin, **kw).double() - y.double()
+        lhs, rhs = (w.double() * diff).sum().item(), (g[:, 1:1 + H].double() * e.double()).sum().item()
+        assert abs(lhs - rhs) <= 2.0 ** -20 * (w.double().abs() * (2 * x.double().abs() + 2 * e.double().abs())).sum().item()
+    # a sum's gradient is broadcast over every dim
+    ones = torch.ones(T, H, d, dtype=dtype, device="cuda")
+    g, = torch.autograd.grad(kernels.rope_positions(x, pos, cos, sin, **kw).sum(), base)
+    assert torch.equal(g[:, 1:1 + H], kernels.rope_positions(ones, pos, cos, sin, interleaved=interleaved, inverse=not inverse))
+    # and the gradient is differentiable itself
+    v = w.clone().requires_grad_()
+    g, = torch.autograd.grad(kernels.rope_positions(x, pos, cos, sin, **kw), x, v, create_graph=True)
+    gg, = torch.autograd.grad(g, v, w)
+    assert torch.equal(gg, kernels.rope_positions(w, pos, cos, sin, **kw))
+    kernels.device_check()
+
+
+def test_rope_positions_refuses_gradients_that_it_does_not_carry():
+    cos, sin = kernels.rope_table(8, 128)
+    x, pos = randn(2, 3, D, seed=1).requires_grad_(), i32([1, 2])
+    with pytest.raises(ValueError, match="out"):
+        kernels.rope_positions(x, pos, cos, sin, out=torch.empty_like(x))
+    with pytest.raises(ValueError, match="cos and sin"):
+        kernels.rope_positions(x.detach(), pos, cos.clone().requires_grad_(), sin)
+    with pytest.raises(ValueError, match="cos and sin"):
+        kernels.rope_positions(x, pos, cos, sin.clone().requires_grad_())
+    with torch.no_grad():  # nothing to carry
+        out = torch.empty_like(x)
+        assert kernels.rope_positions(x, pos, cos, sin, out=out) is out and not out.requires_grad
+    kernels.device_check()
