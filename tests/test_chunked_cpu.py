@@ -206,3 +206,12 @@ def test_evict_workspace_goes_by_the_rows_that_can_move(lib):
     assert kernels.kv_evict_workspace_bytes(2, 8, 4096, 4097) == lib.gqa_kv_evict_workspace_size(2, 8, 1)
     assert kernels.kv_evict_workspace_bytes(2, 8, 100, 32768) == lib.gqa_kv_evict_workspace_size(2, 8, 100)
     assert kernels.kv_evict_workspace_bytes(2, 8, 100) == lib.gqa_kv_evict_workspace_size(2, 8, 100)
+
+
+def test_attend_workspace_holds_two_parts_a_cta(lib):
+    """148 CTAs leave at most two parts of a unit, each 128 values, a maximum and two sums a row, and
+    a descriptor of 32 bytes; without tokens nothing is needed."""
+    assert lib.gqa_attend_chunk_workspace_size(0, 8, 2) == 0
+    for T, Hq, Hkv, rows in [(1, 8, 2, 4), (32, 8, 2, 128), (33, 8, 2, 256), (5000, 32, 8, 256), (1, 128, 1, 128), (2, 100, 1, 256)]:
+        sums = -(-(2 * 148 * 3 * rows * 4) // 16) * 16
+        assert lib.gqa_attend_chunk_workspace_size(T, Hq, Hkv) == 2 * 148 * 128 * rows * 4 + sums + 148 * 32

@@ -843,3 +843,62 @@ def test_rope_positions_refuses_gradients_that_it_does_not_carry():
         out = torch.empty_like(x)
         assert kernels.rope_positions(x, pos, cos, sin, out=out) is out and not out.requires_grad
     kernels.device_check()
+
+
+# ------------------------------------------------------------------ sizes at the ends of the ranges
+def test_more_sequences_than_threads_in_a_block():
+    """The split of the work takes sequences in rounds of 640: here a third begins, and a prompt lies in it."""
+    B = 1500
+    new = [i % 4 for i in range(B)]
+    lens = [n + (7 * i) % 45 for i, n in enumerate(new)]
+    new[1400], lens[1400] = 90, 400
+    new[639], lens[639] = 70, 70
+    bt = Batch(new, lens, 4, 1, 16, seed=41)
+    lse = torch.empty(bt.T, 4, device="cuda")
+    out = bt.attend(lse=lse)
+    kernels.device_check()
+    bt.check_attend(out, lse)
+    acc = torch.rand(B, 1, bt.cap, generator=gen(8), device="cuda")
+    check_weights(bt, lse, acc, kernels.attn_weight_sums(bt.q, bt.kp, bt.table, bt.q_start, bt.lens, lse, acc,
+                                                         acc_out=acc.clone()))
+    kernels.device_check()
+    bt.kp.copy_(randn(*bt.kp.shape, seed=2))
+    bt.vp.copy_(randn(*bt.vp.shape, seed=3))
+    slot_pos = torch.arange(bt.cap, dtype=torch.int32, device="cuda").expand(B, 1, -1).contiguous()
+    run_evict(bt, acc, slot_pos, i32(lens), 24, 4, 2)
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(17, 1), (128, 2), (100, 1), (256, 2)])
+def test_large_groups(Hq, Hkv):
+    """Up to 128 query heads share a kv head: no few-row form from 17 on, one token a tile from 65 on."""
+    bt = Batch([1, 3, 0, 40], [130, 700, 20, 300], Hq, Hkv, 16, seed=43)
+    for causal in (True, False):
+        lse = torch.empty(bt.T, Hq, device="cuda")
+        out = bt.attend(causal=causal, lse=lse)
+        kernels.device_check()
+        bt.check_attend(out, lse, causal)
+        acc = torch.rand(4, Hkv, bt.cap, generator=gen(8), device="cuda")
+        got = kernels.attn_weight_sums(bt.q, bt.kp, bt.table, bt.q_start, bt.lens, lse, acc, causal=causal, acc_out=acc.clone())
+        check_weights(bt, lse, acc, got, causal)
+    kernels.device_check()
+
+
+@pytest.mark.parametrize("new,lens,Hq,Hkv", [([300, 1], [2300, 900], 32, 8), ([65, 40], [1025, 999], 20, 4)])
+def test_attend_with_and_without_lse(new, lens, Hq, Hkv):
+    """Without lse a share of the exponentials of many-row units is good to 2^-13 only, which may
+    also turn a weight's rounding to bf16.  So a weight differs by at most 2 u + 2^-13 of
+    itself between the calls, numerator and sum each, and the output is rounded in both."""
+    bt = Batch(new, lens, Hq, Hkv, 64, seed=45)
+    lse = torch.empty(bt.T, Hq, device="cuda")
+    a, c = bt.attend(lse=lse).double(), bt.attend().double()
+    kernels.device_check()
+    G = Hq // Hkv
+    for b in range(bt.B):
+        n, t0 = bt.new[b], sum(bt.new[:b])
+        for h in range(Hkv):
+            s, _ = bt.scores(b, h, True, D ** -0.5)
+            v = bt.kv(bt.vp, b, h)
+            w = s.softmax(-1)
+            sl = (slice(t0, t0 + n), slice(h * G, (h + 1) * G))
+            bound = (2 * (2 * U + 2.0 ** -13) + 2.0 ** -12) * (w @ v.abs()) + 2 * U * (w @ v).abs()
+            assert ((a[sl] - c[sl]).abs() <= bound).all()

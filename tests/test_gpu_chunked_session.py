@@ -129,3 +129,59 @@ def test_refusals():
     with pytest.raises(ValueError):
         ChunkedKVCache(1, 2, 2, page_size=24)
     kernels.device_check()
+
+
+def test_evictions_keep_the_heaviest():
+    """A 64-bit sum of the weight that each position of each head received, kept by position: the
+    cache's sums follow it through evictions and reused slots, and what an eviction drops weighs
+    no more than any unprotected position that it keeps.
+
+    Tolerance 2^-13 of a sum: a weight's score and lse are each off by 2^-20 sum |q_i k_i| scale,
+    below 2^-16 here, the exponential by 2^-18, and up to 1100 fp32 terms enter the sums, 2^-24 each."""
+    B, Hq, Hkv, page, budget = 3, 8, 2, 16, 96
+    G, M = Hq // Hkv, 1024
+    cache = ChunkedKVCache(B, num_pages=90, max_pages_per_seq=30, Hkv=Hkv, Hq=Hq, page_size=page, max_positions=M)
+    gen = torch.Generator("cuda").manual_seed(7)
+    keys = torch.zeros(B, Hkv, M, D, dtype=torch.float64, device="cuda")
+    weight = torch.zeros(B, Hkv, M, dtype=torch.float64, device="cuda")
+    dropped = 0
+    for new in ([200, 9, 0], [1, 1, 0], "evict", [30, 1, 120], [1, 1, 1], "evict", [1, 0, 1], "evict", [64, 150, 1], "evict", [2, 1, 1]):
+        if new == "evict":
+            before = [[cache.slot_pos[b, h, :cache.seq_len(b)].tolist() for h in range(Hkv)] for b in range(B)]
+            cache.evict(budget, recent=8, sink=2)
+            kernels.device_check()
+            for b in range(B):
+                for h in range(Hkv):
+                    kept = set(cache.slot_pos[b, h, :cache.seq_len(b)].tolist())
+                    gone = set(before[b][h]) - kept
+                    assert kept <= set(before[b][h]) and len(kept) == min(len(before[b][h]), budget)
+                    free = [p for p in kept if 2 <= p < cache.next_pos(b) - 8]
+                    if gone:
+                        w = weight[b, h]
+                        assert w[free].min() >= w[sorted(gone)].max() * (1 - 2.0 ** -12)
+                    dropped += len(gone)
+        else:
+            T = sum(new)
+            x = torch.randn(T, Hq + 2 * Hkv, D, generator=gen, device="cuda").to(torch.bfloat16)
+            pos = torch.cat([torch.arange(cache.next_pos(b), cache.next_pos(b) + n, device="cuda") for b, n in enumerate(new)])
+            rot = kernels.rope_positions(x[:, :Hq + Hkv], pos.to(torch.int32), cache.cos, cache.sin).double()
+            held = [[cache.slot_pos[b, h, :cache.seq_len(b)].long() for h in range(Hkv)] for b in range(B)]
+            cache.step(x[:, :Hq], x[:, Hq:Hq + Hkv], x[:, Hq + Hkv:], new)
+            kernels.device_check()
+            t = 0
+            for b, n in enumerate(new):
+                for h in range(Hkv if n else 0):
+                    mine = pos[t:t + n]
+                    keys[b, h, mine] = rot[t:t + n, Hq + h]
+                    at = torch.cat([held[b][h], mine])
+                    s = torch.einsum("ngd,ld->ngl", rot[t:t + n, h * G:(h + 1) * G], keys[b, h, at]) * D ** -0.5
+                    L = at.numel()
+                    unseen = torch.arange(L, device="cuda")[None] > torch.arange(L - n, L, device="cuda")[:, None]
+                    weight[b, h, at] += s.masked_fill(unseen[:, None], -torch.inf).softmax(-1).sum((0, 1))
+                t += n
+        for b in range(B):
+            for h in range(Hkv):
+                L = cache.seq_len(b)
+                want = weight[b, h, cache.slot_pos[b, h, :L].long()]
+                assert ((cache.acc[b, h, :L].double() - want).abs() <= 2.0 ** -13 * want).all()
+    assert dropped > 300
