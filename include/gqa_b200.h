@@ -254,7 +254,12 @@ int gqa_decode_paged_bf16(const void* q, const void* kpages, const void* vpages,
  * (q[t, h] . k * scale) times v; GQA_FLAG_CAUSAL: slots up to the token's own, else
  * all of lens[b].  Any Hq that is a multiple of Hkv.  lse (float [T][Hq], may be NULL)
  * receives the natural logarithm of the sum of the exponentials.  A row that sees no slot gives
- * zeros and -inf.  Cache rows past lens[b] may hold anything.  max_q_len is a hint (the
+ * zeros and -inf.  Cache rows past lens[b] may hold anything.  The V rows below it are
+ * expected to be finite: a NaN or infinity in one reaches the earlier tokens of its sequence
+ * within the same 256 rows (token, query head of the group) too, through a weight of zero.
+ * Weights are rounded to bf16 for the product with V; without lse some of those of sequences
+ * with more than 32 rows are good to 7.5e-5 before that, so the last bits of o depend on
+ * whether lse is asked for.  max_q_len is a hint (the
  * longest sequence's number of new tokens; 0 = unknown) that only sizes the second
  * launch's grid: any value gives the same results.  A q_start that descends or leaves
  * [0, T] writes nothing (GQA_ERR_DEVICE_INPUT), here and in the weight sums.

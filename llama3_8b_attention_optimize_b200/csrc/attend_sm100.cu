@@ -20,7 +20,7 @@
 //        O^T += V^T P^T with N = 16 or 32, so that the tensor core does no more work than
 //        there are rows.  Such units are bound by memory, and padding 4 rows to 128
 //        drew the GPU's whole power budget (1000 W at 1.39 GHz instead of 1.97: 64 tokens
-//        over 1024..32768 slots took 813 us, where this form takes 650).
+//        over 1024..32768 slots took 813 us, where this form takes 652).
 //
 // Split: the units' K/V tiles form one line per form, and the CTAs (one per SM) are dealt
 // out to the two lines by what a tile of each costs; each line is cut into equal parts
@@ -36,12 +36,13 @@
 // anything, and 0 * NaN would spread).
 //
 // Measured (Hq 32, Hkv 8, both launches, replayed from a graph):
-//   64 single tokens over 1024..32768 slots, 4.25 GB  650 us  6.5 TB/s, what a copy reaches
-//   2048 tokens behind 30720 slots, 1.07 TFLOP        1090 us  980 TFLOP/s, 0.60 of a GEMM's burst: the
+//   64 single tokens over 1024..32768 slots, 4.25 GB  652 us  6.5 TB/s, what a copy reaches
+//   2048 tokens behind 30720 slots, 1.07 TFLOP        1102 us  970 TFLOP/s, 0.60 of a GEMM's burst: the
 //     tensor pipe is busy for 52 % of the cycles, the rest is the softmax's exponentials and
-//     hand-offs (sustained, the 1000 W limit makes it 1265 us)
-//   512 tokens beside 31 sequences of 1..5, 315 MB    107 us  about half from each of the two lines
-//   4 single tokens over 37..1023 slots               14 us  latency: plan, one or two tiles, merge
+//     hand-offs (sustained, the 1000 W limit makes it 1271 us)
+//   512 tokens beside 31 sequences of 1..5, 315 MB    114 us  about half from each of the two lines (107
+//     on another machine)
+//   4 single tokens over 37..1023 slots               14.3 us  latency: plan, one or two tiles, merge
 #include <cuda.h>
 
 #include <algorithm>
@@ -76,8 +77,10 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 constexpr int kBlockRows = 16;             // rows of a block of the few-row form; a unit has one or two
 // What one K/V tile costs in each form, for dealing out the CTAs: a tile of the few form is
-// 64 KB from memory (1.3 us), one of the many form two tiles' softmax (2.3 to 3.0 us).  A mixed
-// step took 113 us with 3 : 5, 104 with 4 : 9, 107 with 2 : 5.
+// 64 KB from memory (1.3 us), one of the many form two tiles' softmax (2.3 to 3.0 us).  Tried on
+// one step alone, 512 tokens beside 31 sequences of 1..5 with 32 and 8 heads: 3 : 5 took 9 % longer
+// than 4 : 9, 2 : 5 took 3 % longer.  How many SMs stream, and units of a single Q tile, are not
+// in it.
 constexpr int kCostFew = 4, kCostMany = 9;
 // and what a unit's beginning and end cost, in tiles.
 constexpr int kExtraFew = 1, kExtraMany = 2;
@@ -270,9 +273,10 @@ __device__ __forceinline__ float ld_shared(uint32_t addr) {
 
 // One 32-column chunk of S -> p = 2^(s*scale_log2 - m) as bf16, stored straight into the
 // K-major SW128 P tile: 16-byte chunk c of the row lies at row ^ 16 c (the swizzle flips address bits
-// 4-6 by the row, which `row` holds already).  acc sums the rounded p that P V
-// multiplies, so that O / l is a mean whose weights add up to one; accf sums them
-// unrounded, for the log-sum-exp.
+// 4-6 by the row, which `row` holds already).  bf16 is the tensor core's operand type; outputs'
+// error against 64 bits is 0.0023 of their norm, 0.0017 being the bf16 output's own.  acc sums
+// the rounded p that P V multiplies, so that O / l is a mean whose weights add up to one; accf
+// sums them unrounded, for the log-sum-exp.
 template <bool kEmulate, bool kLse>
 __device__ __forceinline__ void exp_chunk_store(const uint32_t (&s)[32], uint32_t row, int c0, float2 sc2, float2 nm2,
                                                 float2& acc, float2& accf) {
@@ -613,7 +617,8 @@ __device__ __forceinline__ void softmax_many(const Params& p, uint8_t* smem, uin
         asm volatile("" : "+r"(row));  // keeps the chunks' addresses from living across the loop
         // Chunks with no masked entry may evaluate part of the exponentials on the FMA pipe.
         // Its cubic is good to 7.5e-5, enough for a weight that is rounded to bf16 but not
-        // for the log-sum-exp (where a quintic measured no faster than none).
+        // for the log-sum-exp (where a quintic measured no faster than none).  So the output's
+        // last bits depend on whether the log-sum-exp is wanted.
         if (rel >= 63) {
           exp_chunk_store<!kLse, kLse>(s0, row, 0, sc2, nm2, sum, sumf);
           exp_chunk_store<!kLse, kLse>(s1, row, 4, sc2, nm2, sum, sumf);

@@ -15,9 +15,10 @@
 // addresses by one lane each, K by lanes 0-15 and V by 16-31, 16 bytes a lane.
 //
 // Measured (8 kv heads, both launches, replayed from a graph): 16 sequences of 20000..32768
-// slots cut to 16384, 806 MB in 164 us, 4.9 TB/s (the selection about 32 us of it; the moved
-// weights and positions copied by kernel 2 instead: 170 us); 4 of 1100..2048 cut to 1024,
-// 13.3 us, latency.
+// slots cut to 16384, 806 MB in 165 us, 4.9 TB/s (the selection about 32 us of it; the moved
+// weights and positions copied by kernel 2 instead: 3 % longer); 4 of 1100..2048 cut to 1024,
+// 13.2 us, latency; one slot a sequence, as a cache at its budget is cut: 16 of 16385 25 us, 64 of
+// 4097 43 us: the selection, and a launch for a row a head.
 #include <algorithm>
 
 #include "common.cuh"

@@ -49,7 +49,8 @@ __device__ __forceinline__ Seq seq_of(const Batch& p, int b) {
   return s;
 }
 
-// sum_{i < n} floor((a i + b) / m), by Euclid's steps on (a, m).  The caller knows that the
+// sum_{i < n} floor((a i + b) / m), by Euclid's steps on (a, m) (the reciprocity of floor sums:
+// Graham, Knuth, Patashnik, Concrete Mathematics, 3.5).  The caller knows that the
 // sum is below 2^31; what wraps on the way is multiplied by zero.
 __device__ __forceinline__ uint32_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
   uint32_t sum = 0;

@@ -14,8 +14,9 @@
 //
 // Both kernels move each value once, 16 bytes a thread, and are bound by memory.  Measured
 // (replayed from a graph): 8191 x 40 rows of 128 fp32, half of each rotated, 338 MB in 54 us,
-// 6.2 TB/s; the append of 8192 tokens with 32 + 2 x 8 heads into pages of 16, 205 MB in 39.6 us,
-// 5.2 TB/s; 4 x 32 rows 2.1 us and an append of 64 tokens 3.8 us, latency.
+// 6.2 TB/s; as many rows in bf16, all of each rotated, 172 MB in 46 us (half layout) and 38 us
+// (interleaved); the append of 8192 tokens with 32 + 2 x 8 heads into pages of 16, 205 MB in
+// 39.6 us, 5.2 TB/s; 4 x 32 rows 2.1 us and an append of 64 tokens 3.6 us, latency.
 #include <algorithm>
 
 #include "common.cuh"
@@ -485,10 +486,10 @@ extern "C" int gqa_kv_extend_bf16(const void* k, const void* v, long long k_toke
                    aligned16(cos) && aligned16(sin);
   const bool il = (flags & GQA_FLAG_INTERLEAVED) != 0;
   p.s = shape_of(kD, rot_dim, vec ? 8 : 1, il);
-  // Few tokens: one a block, a thread for every chunk, so that one load's latency is all
-  // (64 tokens: 3.6 us, 4.1 with small blocks).  Many: small blocks of four tokens, of which
-  // some look up their slots while others move rows (8192 tokens: 36.8 us, 44.2 with large
-  // blocks of eight).
+  // Few tokens: one a block, a thread for every chunk, so that one load's latency is all.
+  // Many: small blocks of four tokens, of which some look up their slots while others move
+  // rows.  Both at 32 + 2 x 8 heads, us for few / many: 256 tokens 4 to 6 / 8 to 9, 512
+  // tokens 7 to 9 / 8 to 10, 768 level, 1024 tokens 10 / 9, 2048 tokens 18 / 12, 8192 tokens 80 / 40.
   const int n_rows = Hq + 2 * Hkv;
   p.tokens = T <= 512 ? 1 : 4;
   const dim3 block(p.s.n_chunks, std::max(1, std::min(n_rows, (T <= 512 ? 512 : 128) / p.s.n_chunks)));

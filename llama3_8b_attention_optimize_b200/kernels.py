@@ -580,7 +580,9 @@ def attend_chunk(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, bl
     its own (``causal``) or all lens[b].  ``lse`` (float32 [T, Hq]) receives the natural
     log of the softmax's sum.  ``max_q_len``: the longest sequence's number of new tokens
     where the caller knows it, a hint that only sizes the second launch.  Tokens that see no
-    slot give zeros and -inf."""
+    slot give zeros and -inf.  The last bits of the output depend on whether ``lse`` is given
+    (some exponentials are coarser without, by 7.5e-5 at most).  V rows are expected to be
+    finite: a NaN or infinity can reach earlier tokens of its sequence through a weight of zero."""
     dev = _index(q, "q")
     out = torch.empty(q.shape, dtype=_BF16, device=q.device) if out is None else out
     _check(dev, ((q, "q", _BF16), (out, "out", _BF16)),

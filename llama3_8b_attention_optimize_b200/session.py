@@ -268,7 +268,9 @@ class ChunkedKVCache:
     adds up what attention each slot received (``gqa_attn_weight_sums_f32``).  ``evict`` cuts
     every sequence to a budget of slots (``gqa_kv_evict_bf16``) and returns the pages that fall
     free.  Positions run on across evictions: a sequence's next token stands at
-    ``next_pos(b)``, however few slots are left.
+    ``next_pos(b)``, however few slots are left.  The rotary table ends them: ``max_positions``
+    (by default the capacity, so set it where a cache that evicts is to run on).  With
+    ``track_weights`` the output's last bits may differ from those without (``attend_chunk``).
 
     Pools ``k``/``v`` are [num_pages, Hkv, page_size, 128] bf16; ``lens`` int32 [B] counts each
     sequence's slots; ``acc`` float32 and ``slot_pos`` int32 [B, Hkv, capacity] hold each
